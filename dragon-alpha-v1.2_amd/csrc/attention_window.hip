@@ -1,0 +1,444 @@
+// Attention in which a query sees the keys up to its own position, of those only the last `window` (0: all) and the first
+// `sinks`, with key / value heads that several query heads share, sequences of their own lengths in a padded batch, and
+// fewer queries than keys (the queries are the LAST ones of the sequence: a prompt's next piece, a single token on a cache):
+//     position(i) = i + vl - ql;   i sees j  <=>  i < ql, j < vl, j <= position(i), (j > position(i) - window or j < sinks)
+//     Y[i] = sum_j softmax_j(scale * <Q[i], K[j]>) * V[j] over the keys seen;   lse[i] = log sum_j exp(scale * <Q[i], K[j]>)
+// A row that sees nothing (also the rows behind a sequence's queries) is zeros with lse = -infinity.
+//
+// Two kernels, chosen by the number of queries:
+//   window_tiles: 128 queries of one head per workgroup, the keys they see in steps, S^T = K.Q^T and Y^T = V^T.P^T with
+//     v_mfma_f32_32x32x2_f32 and a running maximum and sum per query (token_mixer.h has the register layouts).  The steps
+//     are the sinks below the window's reach, then the keys from the first one that some query of the tile sees: no other
+//     key is read.  Bound by the FP32 matrix pipe.
+//   window_rows: up to 16 (query, head) rows that share a key / value head per wavefront; keys and values go from memory
+//     straight into v_mfma_f32_16x16x4_f32 operands, 16 keys at a time.  Bound by reading K and V.
+// Where either leaves compute units idle the keys are cut: every part leaves its maximum, sum and un-normalised output in the
+// caller's buffer and window_join adds them in order (a second launch, so the result does not depend on who is last).
+#include "token_mixer.h"
+#include "attention_window.h"
+#include "runtime_internal.h"
+#include "../../include/dragon_hip_mixer.h"
+
+namespace dragon {
+namespace {
+
+constexpr int AQ = 128;          // queries per workgroup of the tiled kernel: 32 per wavefront
+constexpr int LAG = 8;           // the reference maximum may lag the true one by 2^LAG
+constexpr float NEG = -__builtin_inff();
+constexpr float LOWEST = -3.0e38f;
+
+// ---------------------------------------------------------------- many queries
+template <int DB, int DC, int KB>
+__global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p) {
+    constexpr int AK = KB * 32, DW = DB * 32, NG = DC * 4;
+    __shared__ __attribute__((aligned(16))) float Ks[2][AK * DW];
+    __shared__ __attribute__((aligned(16))) float Vs[2][AK * DW];
+
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 31, h = lane >> 5;
+    const WindowJob job = window_job(p, blockIdx.x);
+    const WindowLens len = window_lens(p, job.n);
+    const int q0 = job.qt * AQ;
+    const int i = q0 + wave * 32 + r;                       // this lane's query
+    float* Yb = p.Y + job.n * p.y.n + job.hd * p.y.h;
+    const size_t stat = ((size_t)job.n * p.head + job.hd) * p.QL;
+
+    // the keys that the tile's queries see: [0, sink_end) and [low, hi)
+    const int qn = min(q0 + AQ, len.ql);                    // the tile's queries end here
+    const int off = len.vl - len.ql;
+    const WindowRange range = window_range(p, q0 + off, qn - 1 + off, q0 < qn, len.vl);
+    const int nsink = (range.sink_end + AK - 1) / AK, nwin = (max(range.hi - range.low, 0) + AK - 1) / AK;
+    const int first = (int)((long long)(nsink + nwin) * job.part / p.parts);
+    const int last = (int)((long long)(nsink + nwin) * (job.part + 1) / p.parts);
+
+    const bool live = i < len.ql;
+    const int pos = live ? i + off : -1;
+    const int w0 = q0 + wave * 32 + off, w1 = min(q0 + wave * 32 + 32, len.ql) - 1 + off;   // the wavefront's positions
+
+    v4f qf[NG];
+    mix_load_cols<NG>(qf, p.Q + job.n * p.q.n + job.hd * p.q.h + (size_t)min(i, p.QL - 1) * p.q.l, live, p.dk4, h);
+#pragma unroll
+    for (int g = 0; g < NG; g++) qf[g] *= p.c;              // scores in units of log2
+
+    const float* Kb = p.K + job.n * p.k.n + job.kvh * p.k.h;
+    const float* Vb = p.V + job.n * p.v.n + job.kvh * p.v.h;
+    MixTile<DW, AK, true> kt;
+    MixTile<DW, AK, false> vt;
+    MixColumns<DW, false> vcols;
+    vcols.init(r, h);
+    kt.init(t, p.k.l, p.dk4);
+    vt.init(t, p.v.l, p.dv4);
+    auto key_of = [&](int s) { return s < nsink ? s * AK : range.low + (s - nsink) * AK; };
+    auto fetch = [&](int s) {
+        const int key0 = key_of(s), left = (s < nsink ? range.sink_end : range.hi) - key0;
+        kt.fetch(Kb + (size_t)key0 * p.k.l, left, p.k.l);
+        vt.fetch(Vb + (size_t)key0 * p.v.l, left, p.v.l);
+    };
+
+    v16f o[DC];
+#pragma unroll
+    for (int b = 0; b < DC; b++) o[b] = (v16f)(0.0f);
+    float m = NEG, l = 0.0f;                                // reference maximum (shared by the halves), this half's sum
+
+    if (first < last) {
+        fetch(first);
+        kt.store(Ks[0]);
+        vt.store(Vs[0]);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int s = first; s < last; s++) {
+        const bool more = s + 1 < last;
+        if (more) fetch(s + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        const int key0 = key_of(s), limit = s < nsink ? range.sink_end : range.hi, end = min(key0 + AK, limit);
+        // a wavefront none of whose queries sees a key of this step has nothing to do
+        const bool sees = s < nsink ? w0 <= w1 : (w0 <= w1 && key0 <= w1 && (end - 1 > w0 - p.window || key0 < p.sinks));
+        if (sees) {
+            v16f sc[KB];
+            const float* ks = Ks[buf];
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) {
+                sc[kb] = (v16f)(0.0f);
+                mix_rows_product<DW, NG>(sc[kb], ks + kb * 32 * DW, qf, r, h);
+            }
+            // every query of the wavefront sees every key of the step: no test per score
+            const bool whole = key0 + AK <= limit && key0 + AK - 1 <= w0 && (s < nsink || key0 > w1 - p.window) && q0 + wave * 32 + 32 <= len.ql;
+            if (!whole) {
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) {
+                        const int j = key0 + 32 * kb + mix_row(v, h);
+                        if (!(j < limit && window_sees(p, pos, j))) sc[kb][v] = NEG;
+                    }
+            }
+            float mt = sc[0][0];
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                for (int v = (kb == 0); v < 16; v++) mt = fmaxf(mt, sc[kb][v]);
+            mt = fmaxf(mt, mix_xhalf(mt));
+            if (__builtin_amdgcn_ballot_w64(mt > m + (float)LAG) != 0) {
+                const float m_new = fmaxf(m, mt);
+                const float alpha = m == NEG ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
+                m = m_new;
+                l *= alpha;
+#pragma unroll
+                for (int b = 0; b < DC; b++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) o[b][v] *= alpha;
+            }
+            const float ref = fmaxf(m, LOWEST);             // a query that has seen nothing yet: exp2(-inf) below, not -inf + inf
+            float sum = 0.0f;
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    sc[kb][v] = __builtin_amdgcn_exp2f(sc[kb][v] - ref);
+                    sum += sc[kb][v];
+                }
+            l += sum;
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) mix_columns_product<DW, DC, false>(o, Vs[buf] + kb * 32 * DW, sc[kb], vcols, r, h);
+        }
+        if (more) {
+            kt.store(Ks[buf ^ 1]);
+            vt.store(Vs[buf ^ 1]);
+        }
+        __syncthreads();
+        buf ^= 1;
+    }
+
+    l += mix_xhalf(l);
+    if (i >= p.QL) return;
+    if (p.parts == 1) {
+        mix_store_row<DC>(Yb + (size_t)i * p.y.l, o, l == 0.0f ? 0.0f : 1.0f / l, p.dv4, h);
+        if (p.Lse != nullptr && h == 0) p.Lse[stat + i] = window_lse(m, l);
+    } else {
+        float* part = p.part_o(stat + i, job.part);
+        mix_store_row<DC>(part, o, 1.0f, p.dv4, h);
+        if (h == 0) p.part_ml(stat + i, job.part) = make_float2(m, l);
+    }
+}
+
+// ---------------------------------------------------------------- few queries
+// A wavefront's 16 rows are (query, head of the group) pairs: row = query * group + head.  Lane (c, k4) = (lane & 15,
+// lane >> 4).  S^T = K.Q^T: lane holds 16 bytes of key c per 16 floats of the head dimension, at 4 * k4; MFMA step u of that
+// chunk multiplies d = 16s + 4*k4 + u.  Result register v of lane (c, k4) is key 4*k4 + v, row c: the B operand of step v of
+// Y^T = V^T.P^T, whose A operand is key 4*k4 + v.  A lane loads 16 bytes of that key at 64*e + 4*c; its float u belongs to
+// the 16 outputs 64e + 4*(0..15) + u, so the four floats feed four blocks.
+template <int DE>   // head dimension in 64s
+__global__ __launch_bounds__(NTHREADS, 2) void window_rows(const WindowParams p) {
+    constexpr int NS = DE * 4;
+    __shared__ __attribute__((aligned(16))) float So[4][16][DE * 64 + 4];
+    __shared__ float Sm[4][16], Sl[4][16];
+
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, k4 = lane >> 4;
+    const WindowJob job = window_row_job(p, blockIdx.x);
+    const WindowLens len = window_lens(p, job.n);
+    const int group = p.head / p.kv_head, rows = p.QL * group;
+    const int row0 = job.qt * 16, row = row0 + c;
+    const int i = row / group, hd = job.kvh * group + (row - i * group);
+    const int off = len.vl - len.ql;
+    const bool live = row < rows && i < len.ql;
+    const int pos = live ? i + off : -1;
+
+    const int i0 = row0 / group, i1 = min((min(row0 + 16, rows) - 1) / group, len.ql - 1);
+    const WindowRange range = window_range(p, i0 + off, i1 + off, i0 <= i1, len.vl);
+    const int nsink = (range.sink_end + 15) / 16, nwin = (max(range.hi - range.low, 0) + 15) / 16;
+    const int first = (int)((long long)(nsink + nwin) * job.part / p.parts);
+    const int last = (int)((long long)(nsink + nwin) * (job.part + 1) / p.parts);
+
+    const float* qrow = p.Q + job.n * p.q.n + (size_t)min(hd, p.head - 1) * p.q.h + (size_t)min(i, p.QL - 1) * p.q.l;
+    v4f qf[NS];
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+        const int d = 16 * s + 4 * k4;
+        qf[s] = (live && d < p.dk4) ? *(const v4f*)(qrow + d) * p.c : (v4f)(0.0f);
+    }
+
+    const float* Kb = p.K + job.n * p.k.n + job.kvh * p.k.h;
+    const float* Vb = p.V + job.n * p.v.n + job.kvh * p.v.h;
+    int koff[NS], voff[4 * DE];
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+        const int d = 16 * s + 4 * k4;
+        koff[s] = d < p.dk4 ? (c * p.k.l + d) * 4 : OOB_OFFSET;
+    }
+#pragma unroll
+    for (int v = 0; v < 4; v++)
+#pragma unroll
+        for (int e = 0; e < DE; e++) {
+            const int d = 64 * e + 4 * c;
+            voff[v * DE + e] = d < p.dv4 ? ((4 * k4 + v) * p.v.l + d) * 4 : OOB_OFFSET;
+        }
+    v4f kr[NS], vr[4 * DE];
+    auto fetch = [&](int s) {
+        const int key0 = s < nsink ? s * 16 : range.low + (s - nsink) * 16;
+        const int left = min((s < nsink ? range.sink_end : range.hi) - key0, 16);
+        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)(Kb + (size_t)key0 * p.k.l), 0, left * p.k.l * 4, RSRC_FLAGS);
+        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)(Vb + (size_t)key0 * p.v.l), 0, left * p.v.l * 4, RSRC_FLAGS);
+#pragma unroll
+        for (int s2 = 0; s2 < NS; s2++) kr[s2] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rk, koff[s2], 0, 0));
+#pragma unroll
+        for (int s2 = 0; s2 < 4 * DE; s2++) vr[s2] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rv, voff[s2], 0, 0));
+    };
+
+    v4f o[DE][4];
+#pragma unroll
+    for (int e = 0; e < DE; e++)
+#pragma unroll
+        for (int u = 0; u < 4; u++) o[e][u] = (v4f)(0.0f);
+    float m = NEG, l = 0.0f;
+
+    const int uwave = __builtin_amdgcn_readfirstlane(wave);
+    if (first + uwave < last) fetch(first + uwave);
+    for (int s = first + uwave; s < last; s += 4) {
+        const int key0 = s < nsink ? s * 16 : range.low + (s - nsink) * 16;
+        const int limit = s < nsink ? range.sink_end : range.hi;
+        v4f kc[NS], vc[4 * DE];
+#pragma unroll
+        for (int s2 = 0; s2 < NS; s2++) kc[s2] = kr[s2];
+#pragma unroll
+        for (int s2 = 0; s2 < 4 * DE; s2++) vc[s2] = vr[s2];
+        if (s + 4 < last) fetch(s + 4);
+        v4f sc = (v4f)(0.0f);
+#pragma unroll
+        for (int s2 = 0; s2 < NS; s2++)
+#pragma unroll
+            for (int u = 0; u < 4; u++) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kc[s2][u], qf[s2][u], sc, 0, 0, 0);
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            const int j = key0 + 4 * k4 + v;
+            if (!(j < limit && window_sees(p, pos, j))) sc[v] = NEG;
+        }
+        float mt = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+        mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+        mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+        if (__builtin_amdgcn_ballot_w64(mt > m + (float)LAG) != 0) {
+            const float m_new = fmaxf(m, mt);
+            const float alpha = m == NEG ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
+            m = m_new;
+            l *= alpha;
+#pragma unroll
+            for (int e = 0; e < DE; e++)
+#pragma unroll
+                for (int u = 0; u < 4; u++) o[e][u] *= alpha;
+        }
+        const float ref = fmaxf(m, LOWEST);
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            sc[v] = __builtin_amdgcn_exp2f(sc[v] - ref);
+            l += sc[v];
+        }
+#pragma unroll
+        for (int v = 0; v < 4; v++)
+#pragma unroll
+            for (int e = 0; e < DE; e++)
+#pragma unroll
+                for (int u = 0; u < 4; u++) o[e][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(vc[v * DE + e][u], sc[v], o[e][u], 0, 0, 0);
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+
+    // ---- the four wavefronts' parts of the keys, added through LDS; register w of block (e, u) is d = 64e + 16*k4 + 4w + u ----
+#pragma unroll
+    for (int e = 0; e < DE; e++)
+#pragma unroll
+        for (int w = 0; w < 4; w++)
+            *(v4f*)&So[wave][c][64 * e + 16 * k4 + 4 * w] = (v4f){o[e][0][w], o[e][1][w], o[e][2][w], o[e][3][w]};
+    if (k4 == 0) { Sm[wave][c] = m; Sl[wave][c] = l; }
+    __syncthreads();
+    for (int x = t; x < 16 * (p.dv4 / 4); x += NTHREADS) {
+        const int rr = x / (p.dv4 / 4), d = 4 * (x - rr * (p.dv4 / 4));
+        if (row0 + rr >= rows) break;
+        const float M = fmaxf(fmaxf(Sm[0][rr], Sm[1][rr]), fmaxf(Sm[2][rr], Sm[3][rr]));
+        float L = 0.0f;
+        v4f y = (v4f)(0.0f);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float f = Sm[w][rr] == NEG ? 0.0f : __builtin_amdgcn_exp2f(Sm[w][rr] - M);
+            L += Sl[w][rr] * f;
+            y += *(const v4f*)&So[w][rr][d] * f;
+        }
+        const int qi = (row0 + rr) / group, qh = job.kvh * group + (row0 + rr - qi * group);
+        const size_t stat = ((size_t)job.n * p.head + qh) * p.QL + qi;
+        if (p.parts == 1) {
+            *(v4f*)(p.Y + job.n * p.y.n + qh * p.y.h + (size_t)qi * p.y.l + d) = L == 0.0f ? (v4f)(0.0f) : y * (1.0f / L);
+            if (p.Lse != nullptr && d == 0) p.Lse[stat] = window_lse(M, L);
+        } else {
+            *(v4f*)(p.part_o(stat, job.part) + d) = y;
+            if (d == 0) p.part_ml(stat, job.part) = make_float2(M, L);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- the parts of a row, added in order
+__global__ __launch_bounds__(NTHREADS) void window_join(const WindowParams p) {
+    const int per = p.dv4 / 4;
+    const long long x = (long long)blockIdx.x * NTHREADS + threadIdx.x;
+    const long long stat = x / per;
+    if (stat >= (long long)p.N * p.head * p.QL) return;
+    const int d = 4 * (int)(x - stat * per);
+    float M = NEG;
+    for (int s = 0; s < p.parts; s++) M = fmaxf(M, p.part_ml(stat, s).x);
+    float L = 0.0f;
+    v4f y = (v4f)(0.0f);
+    for (int s = 0; s < p.parts; s++) {
+        const float2 ml = p.part_ml(stat, s);
+        const float f = ml.x == NEG ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
+        L += ml.y * f;
+        y += *(const v4f*)(p.part_o(stat, s) + d) * f;
+    }
+    const long long nh = stat / p.QL;
+    const int n = (int)(nh / p.head), hd = (int)(nh - (long long)n * p.head), i = (int)(stat - nh * p.QL);
+    *(v4f*)(p.Y + n * p.y.n + hd * p.y.h + (size_t)i * p.y.l + d) = L == 0.0f ? (v4f)(0.0f) : y * (1.0f / L);
+    if (p.Lse != nullptr && d == 0) p.Lse[stat] = window_lse(M, L);
+}
+
+// ---------------------------------------------------------------- host side
+constexpr int ROWS_MAX_QL = 16;      // up to here the row kernel: a tile of the other has 128 queries
+
+struct WindowPlan { bool rows; int qtiles, parts; };
+
+// One decision for the launch and for the size of the caller's buffer: from the sizes alone.
+WindowPlan window_plan(int N, int head, int kv_head, int QL, int VL, int window, int sinks) {
+    WindowPlan x;
+    const long long group = head / kv_head;
+    x.rows = QL <= ROWS_MAX_QL;
+    const long long per = x.rows ? 16 : AQ;
+    x.qtiles = (int)(x.rows ? (QL * group + 15) / 16 : (QL + AQ - 1) / AQ);
+    const long long base = (long long)N * x.qtiles * (x.rows ? kv_head : head);
+    const long long reach = window == 0 ? VL : (long long)window + sinks + (x.rows ? QL : per);
+    const long long steps = ((reach < VL ? reach : VL) + (x.rows ? 15 : 31)) / (x.rows ? 16 : 32);
+    const long long want = x.rows ? 1024 : 512, least = x.rows ? 8 : 4;   // workgroups on the chip; steps worth a part
+    long long parts = base >= want / 2 ? 1 : (want + base - 1) / base;
+    if (parts > steps / least) parts = steps / least;
+    x.parts = (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
+    return x;
+}
+
+long long window_buffer(const WindowPlan& x, int N, int head, int QL, int dv4) {
+    return x.parts == 1 ? 0 : (long long)N * head * QL * x.parts * (dv4 + 2) * 4;
+}
+
+}  // namespace
+
+bool window_arguments_ok(int N, int head, int kv_head, int QL, int VL, int dk4, int dv4, int window, int sinks) {
+    if (N <= 0 || head <= 0 || kv_head <= 0 || head % kv_head != 0 || QL <= 0 || VL <= 0 || dk4 <= 0 || dv4 <= 0 || (dk4 & 3) ||
+        (dv4 & 3) || dk4 > 128 || dv4 > 128 || window < 0 || sinks < 0)
+        return false;
+    // positions are 32-bit, a tile's offsets 32-bit bytes, a launch's workgroups 31 bits
+    const long long row = (long long)head * (dk4 > dv4 ? dk4 : dv4);
+    return (long long)QL + VL < 0x3fffff00LL && row * AQ * 4 < 0x7ffffff0LL &&
+           (long long)N * head * ((QL + 15LL) / 16) * 64 < 0x7fffffffLL;
+}
+
+}  // namespace dragon
+
+using namespace dragon;
+
+extern "C" {
+
+int64_t dragon_Cuda_attention_window_bufsize(int32_t N, int32_t head, int32_t kv_head, int32_t QL, int32_t VL, int32_t dK4,
+                                             int32_t dV4, int32_t window, int32_t sinks) {
+    if (!window_arguments_ok(N, head, kv_head, QL, VL, dK4, dV4, window, sinks)) return -1;
+    return window_buffer(window_plan(N, head, kv_head, QL, VL, window, sinks), N, head, QL, dV4);
+}
+
+int dragon_Cuda_attention_window_forward(const int64_t* streams, int32_t length, int64_t dQ, int64_t dK, int64_t dV, int64_t dY,
+                                         int64_t dLse, int64_t dQLens, int64_t dVLens, int64_t dBuf, int64_t buf_size, int32_t N,
+                                         int32_t head, int32_t kv_head, int32_t QL, int32_t VL, int32_t dK4, int32_t dV4,
+                                         int32_t head_inner, float scale, int32_t window, int32_t sinks) {
+    if (streams == nullptr || length < 1 || length > 10) return hipErrorInvalidValue;
+    if (dQ == 0 || dK == 0 || dV == 0 || dY == 0 || !mix_aligned16(dQ) || !mix_aligned16(dK) || !mix_aligned16(dV) ||
+        !mix_aligned16(dY) || (dLse & 3) || (dQLens & 3) || (dVLens & 3))
+        return hipErrorInvalidValue;
+    if (!window_arguments_ok(N, head, kv_head, QL, VL, dK4, dV4, window, sinks) || !(scale - scale == 0.0f))
+        return hipErrorInvalidValue;
+    const WindowPlan plan = window_plan(N, head, kv_head, QL, VL, window, sinks);
+    const long long need = window_buffer(plan, N, head, QL, dV4);
+    if (need > 0 && (dBuf == 0 || !mix_aligned16(dBuf) || buf_size < need)) return hipErrorInvalidValue;
+
+    WindowParams p;
+    p.Q = (const float*)(intptr_t)dQ; p.K = (const float*)(intptr_t)dK; p.V = (const float*)(intptr_t)dV;
+    p.Y = (float*)(intptr_t)dY; p.Lse = (float*)(intptr_t)dLse;
+    p.QLens = (const int*)(intptr_t)dQLens; p.VLens = (const int*)(intptr_t)dVLens;
+    p.N = N; p.head = head; p.kv_head = kv_head; p.QL = QL; p.VL = VL; p.dk4 = dK4; p.dv4 = dV4;
+    p.q = mix_layout(head_inner, head, QL, dK4); p.y = mix_layout(head_inner, head, QL, dV4);
+    p.k = mix_layout(head_inner, kv_head, VL, dK4); p.v = mix_layout(head_inner, kv_head, VL, dV4);
+    p.window = window == 0 || window > QL + VL ? QL + VL : window;
+    p.sinks = sinks;
+    p.c = scale * MIX_LOG2E;
+    p.qtiles = plan.qtiles; p.parts = plan.parts;
+    p.part = need > 0 ? (float*)(intptr_t)dBuf : nullptr;
+    split_ledger_touch(p.Y, (size_t)N * head * QL * dV4 * 4);
+    if (p.Lse != nullptr) split_ledger_touch(p.Lse, (size_t)N * head * QL * 4);
+    if (p.part != nullptr) split_ledger_touch(p.part, (size_t)need);
+
+    hipStream_t s = (hipStream_t)(intptr_t)streams[0];
+    const int dmax = dK4 > dV4 ? dK4 : dV4;
+    const dim3 block(NTHREADS);
+    if (plan.rows) {
+        const dim3 grid((unsigned)((long long)N * kv_head * plan.qtiles * plan.parts));
+        if (dmax <= 64) hipLaunchKernelGGL(window_rows<1>, grid, block, 0, s, p);
+        else hipLaunchKernelGGL(window_rows<2>, grid, block, 0, s, p);
+    } else {
+        const dim3 grid((unsigned)((long long)N * head * plan.qtiles * plan.parts));
+        switch ((dmax + 31) / 32) {
+            case 1: hipLaunchKernelGGL((window_tiles<1, 1, 2>), grid, block, 0, s, p); break;
+            case 2: hipLaunchKernelGGL((window_tiles<2, 2, 2>), grid, block, 0, s, p); break;
+            case 3: hipLaunchKernelGGL((window_tiles<4, 3, 1>), grid, block, 0, s, p); break;
+            default: hipLaunchKernelGGL((window_tiles<4, 4, 1>), grid, block, 0, s, p); break;
+        }
+    }
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && plan.parts > 1) {
+        const long long items = (long long)N * head * QL * (dV4 / 4);
+        hipLaunchKernelGGL(window_join, dim3((unsigned)((items + NTHREADS - 1) / NTHREADS)), block, 0, s, p);
+        e = hipGetLastError();
+    }
+    return e;
+}
+
+}  // extern "C"

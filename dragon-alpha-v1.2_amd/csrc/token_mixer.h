@@ -1,0 +1,142 @@
+// Shared by the kernels that mix the tokens of a sequence (windowed attention, linear attention with a decay).
+//
+// All of them multiply with v_mfma_f32_32x32x2_f32 and let a wavefront own 32 rows of the one operand as COLUMNS of the
+// result: lane (r, h) holds column r, result register v is row 8*(v/4) + 4*h + v%4.  A first product's result is then, register
+// for register, the B operand of a second product whose MFMA step v consumes row 8*(v/4) + 4*h + v%4 from lane half h.
+//
+// A tile of ROWS sequence rows sits in LDS as [row][DW]; a row is read in two ways:
+//   chunk-wise (4 consecutive floats of row r per lane: the A operand of a product along the head dimension), from a
+//              tile whose 16-byte chunk c of row r lies at position c ^ kin_swizzle<DW>(r);
+//   column-wise (lane r takes float 32b + r: the A operand of a product along the sequence).
+// A tile that is read in both ways is stored with the swizzle: 32 lanes that read 32 consecutive floats of one row touch
+// the same eight chunks in another order, still every bank once.
+#pragma once
+#include "gemm_mfma_kernel.h"
+
+namespace dragon {
+namespace {
+
+constexpr float MIX_LOG2E = 1.44269504088896340736f;
+constexpr float MIX_LN2 = 0.69314718055994530942f;
+
+__device__ __forceinline__ float mix_xhalf(float x) { return __shfl_xor(x, 32, 64); }
+
+// the sequence row that result register v of lane half h stands for
+__device__ __forceinline__ constexpr int mix_row(int v, int h) { return 8 * (v / 4) + 4 * h + (v % 4); }
+
+// Staging of one [ROWS][DW] tile by the 256 threads of a workgroup, through registers.  A lane's byte offsets inside the
+// tile never change; the tile's first row goes into the descriptor's base and the rows that exist into its size, so rows
+// beyond them and chunks beyond the row's d4 floats read as zeros and a fetch costs scalar instructions only.
+template <int DW, int ROWS, bool SWIZZLE>
+struct MixTile {
+    static constexpr int CPR = DW / 4, RPP = NTHREADS / CPR, PASSES = ROWS / RPP;
+    static_assert(PASSES * RPP == ROWS && PASSES >= 1, "the tile divides over the workgroup");
+    int off[PASSES], at[PASSES];
+    v4f reg[PASSES];
+    __device__ __forceinline__ void init(int t, int pitch, int d4) {
+        const int chunk = t % CPR, row0 = t / CPR;
+#pragma unroll
+        for (int s = 0; s < PASSES; s++) {
+            const int row = row0 + s * RPP;
+            off[s] = chunk * 4 < d4 ? (row * pitch + chunk * 4) * 4 : OOB_OFFSET;
+            at[s] = row * DW + 4 * (SWIZZLE ? (chunk ^ kin_swizzle<DW>(row)) : chunk);
+        }
+    }
+    // rows [0, left) of the tile that starts at `base`; left < 1 reads nothing
+    __device__ __forceinline__ void fetch(const float* base, int left, int pitch) {
+        const int rows = left < 0 ? 0 : (left < ROWS ? left : ROWS);
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, rows * pitch * 4, RSRC_FLAGS);
+#pragma unroll
+        for (int s = 0; s < PASSES; s++)
+            reg[s] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(r, off[s], 0, 0));
+    }
+    __device__ __forceinline__ void store(float* lds) const {
+#pragma unroll
+        for (int s = 0; s < PASSES; s++) *(v4f*)(lds + at[s]) = reg[s];
+    }
+};
+
+// result[row of the tile][column] += tile . cols^T over the head dimension: cols[g] holds d = 8g + 4h .. +3 of the lane's
+// column; the tile is swizzled
+template <int DW, int NG>
+__device__ __forceinline__ void mix_rows_product(v16f& s, const float* tile, const v4f (&cols)[NG], int r, int h) {
+    const float* row = tile + r * DW;
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        const v4f a = *(const v4f*)(row + 4 * ((2 * g + h) ^ kin_swizzle<DW>(r)));
+        s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, cols[g].x, s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, cols[g].y, s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, cols[g].z, s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, cols[g].w, s, 0, 0, 0);
+    }
+}
+
+// Where lane (r, h) finds float 32b + r of tile row mix_row(v, h).  With the swizzle the place is a lane's part that depends
+// on v % 4 only (the chunk's low three bits are exchanged with the row's) plus a constant.
+template <int DW, bool SWIZZLE>
+struct MixColumns {
+    int at[SWIZZLE && DW > 32 ? 4 : 1];
+    __device__ __forceinline__ void init(int r, int h) {
+        if constexpr (SWIZZLE && DW > 32) {
+#pragma unroll
+            for (int w = 0; w < 4; w++) at[w] = 4 * h * DW + 4 * ((r >> 2) ^ (4 * h) ^ w) + (r & 3);
+        } else {
+            at[0] = SWIZZLE ? (r & 3) : 4 * h * DW + r;
+        }
+    }
+    __device__ __forceinline__ float read(const float* tile, int v, int b, int r, int h) const {
+        if constexpr (!SWIZZLE) return tile[at[0] + (8 * (v / 4) + v % 4) * DW + 32 * b];
+        else if constexpr (DW > 32) return tile[at[v % 4] + (8 * (v / 4) + v % 4) * DW + 4 * ((8 * b) ^ (8 * ((v / 4) & 1)))];
+        else return tile[mix_row(v, h) * DW + 4 * ((8 * b + (r >> 2)) ^ kin_swizzle<DW>(mix_row(v, h))) + at[0]];
+    }
+};
+
+// out^T[d][column] += sum over the tile's rows of tile[row][d] * p[row][column]
+template <int DW, int DC, bool SWIZZLE>
+__device__ __forceinline__ void mix_columns_product(v16f (&o)[DC], const float* tile, const v16f& p, const MixColumns<DW, SWIZZLE>& cols, int r, int h) {
+#pragma unroll
+    for (int v = 0; v < 16; v++) {
+#pragma unroll
+        for (int b = 0; b < DC; b++) o[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(cols.read(tile, v, b, r, h), p[v], o[b], 0, 0, 0);
+    }
+}
+
+// a lane's column of a result, times f: float 32b + 8g + 4h .. +3 of the row at `row`
+template <int DC>
+__device__ __forceinline__ void mix_store_row(float* row, const v16f (&o)[DC], float f, int d4, int h) {
+#pragma unroll
+    for (int b = 0; b < DC; b++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const int d = 32 * b + 8 * g + 4 * h;
+            if (d < d4) *(v4f*)(row + d) = (v4f){o[b][4 * g] * f, o[b][4 * g + 1] * f, o[b][4 * g + 2] * f, o[b][4 * g + 3] * f};
+        }
+}
+
+// the lane's column of an operand: 4 consecutive floats per group of 8, zeros where the row does not exist
+template <int NG>
+__device__ __forceinline__ void mix_load_cols(v4f (&c)[NG], const float* row, bool exists, int d4, int h) {
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        const int d = 8 * g + 4 * h;
+        c[g] = (exists && d < d4) ? *(const v4f*)(row + d) : (v4f)(0.0f);
+    }
+}
+
+inline bool mix_aligned16(int64_t a) { return (a & 15) == 0; }
+
+// element strides of a tensor [N, L, head, d4] (head_inner) or [N, head, L, d4]
+struct MixLayout {
+    long long n, h;
+    int l;
+};
+inline MixLayout mix_layout(int head_inner, int head, int L, int d4) {
+    MixLayout x;
+    x.l = head_inner ? head * d4 : d4;
+    x.h = head_inner ? (long long)d4 : (long long)L * d4;
+    x.n = (long long)head * L * d4;
+    return x;
+}
+
+}  // namespace
+}  // namespace dragon

@@ -8,6 +8,8 @@ Thin, one-to-one wrappers over the C ABI (no compute happens in Python):
   Cuda_conv3D      -- forward-convolution natives of ...impl.math.Cuda_conv3D
   Cuda_expk2       -- transpose2D / 3D / 4D of ...impl.Cuda_expk2 (dimension swap)
   Cuda_function    -- linear_dual2D_row of ...impl.math.Cuda_function (the bias row)
+  Cuda_attention   -- the attention block in one launch; attention with a sliding window and sinks, and its gradient
+  Cuda_linear_attention -- linear attention with a decay for each head, and its gradient
   CudaException    -- the error type the reference's natives throw
 
 Method names and argument order follow the Java declarations
@@ -42,6 +44,12 @@ def _check(code):
 def _stream_array(streams):
     arr = (ctypes.c_int64 * len(streams))(*[int(s) for s in streams])
     return arr, len(streams)
+
+
+def _size(nbytes):
+    if nbytes < 0:
+        raise CudaException(1)      # the sizes are refused
+    return nbytes
 
 
 def _host_ptr(a):
@@ -393,6 +401,64 @@ class Cuda_attention:
         arr, _ = _stream_array(streams)
         _check(lib.dragon_Cuda_attention_forward_masked(arr, length, dQ, dK, dV, dMask, dY, N, head, QL, VL, dK4, dV4,
                                                         int(head_inner), scale, mask_pitch, int(mask_per_head)))
+
+
+    @staticmethod
+    def window_bufsize(N, head, kv_head, QL, VL, dK4, dV4, window, sinks):
+        """Bytes of work buffer that window_forward needs for these sizes (0: none)."""
+        return _size(lib.dragon_Cuda_attention_window_bufsize(N, head, kv_head, QL, VL, dK4, dV4, window, sinks))
+
+    @staticmethod
+    def window_forward(streams, length, dQ, dK, dV, dY, dLse, dQLens, dVLens, dBuf, buf_size, N, head, kv_head, QL, VL,
+                       dK4, dV4, head_inner, scale, window, sinks):
+        """Causal attention over the last `window` keys (0: all) and the first `sinks`; dLse, dQLens, dVLens may be 0."""
+        arr, _ = _stream_array(streams)
+        _check(lib.dragon_Cuda_attention_window_forward(arr, length, dQ, dK, dV, dY, dLse, dQLens, dVLens, dBuf, buf_size,
+                                                        N, head, kv_head, QL, VL, dK4, dV4, int(head_inner), scale,
+                                                        window, sinks))
+
+    @staticmethod
+    def window_backward_bufsize(N, head, kv_head, QL, VL, dK4, dV4, window, sinks):
+        return _size(lib.dragon_Cuda_attention_window_backward_bufsize(N, head, kv_head, QL, VL, dK4, dV4, window, sinks))
+
+    @staticmethod
+    def window_backward(streams, length, dQ, dK, dV, dY, dLse, dDeltaY, dDeltaQ, dDeltaK, dDeltaV, dQLens, dVLens, dBuf,
+                        buf_size, N, head, kv_head, QL, VL, dK4, dV4, head_inner, scale, window, sinks):
+        """Gradients of window_forward with respect to Q, K and V; dY and dLse are what it left."""
+        arr, _ = _stream_array(streams)
+        _check(lib.dragon_Cuda_attention_window_backward(arr, length, dQ, dK, dV, dY, dLse, dDeltaY, dDeltaQ, dDeltaK,
+                                                         dDeltaV, dQLens, dVLens, dBuf, buf_size, N, head, kv_head, QL,
+                                                         VL, dK4, dV4, int(head_inner), scale, window, sinks))
+
+
+class Cuda_linear_attention:
+    """Linear attention with a decay for each head: S = e^g S + k^T v, y = scale q S."""
+
+    @staticmethod
+    def bufsize(N, head, L, dK4, dV4):
+        """Bytes of work buffer that forward needs for these sizes (0: none)."""
+        return _size(lib.dragon_Cuda_linear_attention_bufsize(N, head, L, dK4, dV4))
+
+    @staticmethod
+    def forward(streams, length, dQ, dK, dV, dDecay, dState, dY, dStateOut, dLens, dBuf, buf_size, N, head, L, dK4, dV4,
+                head_inner, scale):
+        """dState, dStateOut (may be the same) and dLens may be 0; dDecay holds g of every head."""
+        arr, _ = _stream_array(streams)
+        _check(lib.dragon_Cuda_linear_attention_forward(arr, length, dQ, dK, dV, dDecay, dState, dY, dStateOut, dLens,
+                                                        dBuf, buf_size, N, head, L, dK4, dV4, int(head_inner), scale))
+
+    @staticmethod
+    def backward_bufsize(N, head, L, dK4, dV4):
+        return _size(lib.dragon_Cuda_linear_attention_backward_bufsize(N, head, L, dK4, dV4))
+
+    @staticmethod
+    def backward(streams, length, dQ, dK, dV, dDecay, dState, dDeltaY, dDeltaStateOut, dDeltaQ, dDeltaK, dDeltaV,
+                 dDeltaState, dLens, dBuf, buf_size, N, head, L, dK4, dV4, head_inner, scale):
+        """Gradients of forward with respect to Q, K, V and the first state (dDeltaState may be 0)."""
+        arr, _ = _stream_array(streams)
+        _check(lib.dragon_Cuda_linear_attention_backward(arr, length, dQ, dK, dV, dDecay, dState, dDeltaY, dDeltaStateOut,
+                                                         dDeltaQ, dDeltaK, dDeltaV, dDeltaState, dLens, dBuf, buf_size, N,
+                                                         head, L, dK4, dV4, int(head_inner), scale))
 
 
 class Cuda_expk2:

@@ -1,4 +1,5 @@
-"""ctypes binding of libdragon_hip.so: the C ABI declared in include/dragon_hip_gemm.h
+"""ctypes binding of libdragon_hip.so: the C ABI declared in include/dragon_hip_gemm.h,
+include/dragon_hip_conv.h, include/dragon_hip_mixer.h
 and include/dragon_hip_runtime.h, the host-side engine of include/dragon_hip_engine.h and the
 test hooks of include/dragon_hip_testing.h.
 
@@ -25,6 +26,8 @@ _BMM = [p_i64, i32, i64, i64, i64, i32, i32, i32, i32, i32]
 # streams, length, X, IH, IW, W, FH, FW, Y, OH, OW, N, IC, OC, sh, sw, ph, pw  (and with CW after W)
 _CONV = [p_i64, i32, i64, i32, i32, i64, i32, i32, i64, i32, i32, i32, i32, i32, i32, i32, i32, i32]
 _CONVR = [p_i64, i32, i64, i32, i32, i64, i64, i32, i32, i64, i32, i32, i32, i32, i32, i32, i32, i32, i32]
+# N, head, kv_head, QL, VL, dK4, dV4, head_inner, scale, window, sinks
+_WINDOW = [i32] * 8 + [f32, i32, i32]
 SIGNATURES = {
     # include/dragon_hip_gemm.h
     "dragon_Cuda_matMul_matMul": (i32, _MM2D),
@@ -42,6 +45,15 @@ SIGNATURES = {
     "dragon_Cuda_attention_forward": (i32, [p_i64, i32, i64, i64, i64, i64, i32, i32, i32, i32, i32, i32, i32, f32]),
     "dragon_Cuda_attention_forward_masked": (i32, [p_i64, i32, i64, i64, i64, i64, i64, i32, i32, i32, i32, i32, i32, i32,
                                                    f32, i32, i32]),
+    # include/dragon_hip_mixer.h
+    "dragon_Cuda_attention_window_bufsize": (i64, [i32] * 9),
+    "dragon_Cuda_attention_window_backward_bufsize": (i64, [i32] * 9),
+    "dragon_Cuda_attention_window_forward": (i32, [p_i64, i32] + [i64] * 9 + _WINDOW),
+    "dragon_Cuda_attention_window_backward": (i32, [p_i64, i32] + [i64] * 13 + _WINDOW),
+    "dragon_Cuda_linear_attention_bufsize": (i64, [i32] * 5),
+    "dragon_Cuda_linear_attention_backward_bufsize": (i64, [i32] * 5),
+    "dragon_Cuda_linear_attention_forward": (i32, [p_i64, i32] + [i64] * 10 + [i32] * 6 + [f32]),
+    "dragon_Cuda_linear_attention_backward": (i32, [p_i64, i32] + [i64] * 14 + [i32] * 6 + [f32]),
     "dragon_Cuda_expk2_transpose2D": (i32, [i64, i64, i64, i32, i32, i32, i32, i32]),
     "dragon_Cuda_expk2_transpose3D": (i32, [i64, i64, i64] + [i32] * 9),
     "dragon_Cuda_expk2_transpose4D": (i32, [i64, i64, i64] + [i32] * 11),
