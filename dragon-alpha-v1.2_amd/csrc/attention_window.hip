@@ -17,7 +17,7 @@
 #include "token_mixer.h"
 #include "attention_window.h"
 #include "runtime_internal.h"
-#include "../../include/dragon_hip_mixer.h"
+#include "../../include/dragon_hip_gemm.h"
 
 namespace dragon {
 namespace {

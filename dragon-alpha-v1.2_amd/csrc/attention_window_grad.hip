@@ -12,7 +12,7 @@
 #include "token_mixer.h"
 #include "attention_window.h"
 #include "runtime_internal.h"
-#include "../../include/dragon_hip_mixer.h"
+#include "../../include/dragon_hip_gemm.h"
 
 namespace dragon {
 bool window_arguments_ok(int N, int head, int kv_head, int QL, int VL, int dk4, int dv4, int window, int sinks);

@@ -19,7 +19,7 @@
 // powers are FP32; the exponent g n is rounded once, which is an error of |g n| 2^-24 in a factor e^{g n}.
 #include "token_mixer.h"
 #include "runtime_internal.h"
-#include "../../include/dragon_hip_mixer.h"
+#include "../../include/dragon_hip_gemm.h"
 
 namespace dragon {
 namespace {

@@ -1,5 +1,4 @@
-"""ctypes binding of libdragon_hip.so: the C ABI declared in include/dragon_hip_gemm.h,
-include/dragon_hip_conv.h, include/dragon_hip_mixer.h
+"""ctypes binding of libdragon_hip.so: the C ABI declared in include/dragon_hip_gemm.h
 and include/dragon_hip_runtime.h, the host-side engine of include/dragon_hip_engine.h and the
 test hooks of include/dragon_hip_testing.h.
 
@@ -45,7 +44,6 @@ SIGNATURES = {
     "dragon_Cuda_attention_forward": (i32, [p_i64, i32, i64, i64, i64, i64, i32, i32, i32, i32, i32, i32, i32, f32]),
     "dragon_Cuda_attention_forward_masked": (i32, [p_i64, i32, i64, i64, i64, i64, i64, i32, i32, i32, i32, i32, i32, i32,
                                                    f32, i32, i32]),
-    # include/dragon_hip_mixer.h
     "dragon_Cuda_attention_window_bufsize": (i64, [i32] * 9),
     "dragon_Cuda_attention_window_backward_bufsize": (i64, [i32] * 9),
     "dragon_Cuda_attention_window_forward": (i32, [p_i64, i32] + [i64] * 9 + _WINDOW),
