@@ -21,11 +21,12 @@ struct WindowParams {
     }
 };
 
+// (n is the same for the whole wavefront wherever this is called but in window_delta, which has lengths of its own)
 struct WindowLens { int ql, vl; };
 __device__ __forceinline__ WindowLens window_lens(const WindowParams& p, int n) {
     WindowLens x;
-    x.ql = p.QLens ? min(max(p.QLens[n], 0), p.QL) : p.QL;
-    x.vl = p.VLens ? min(max(p.VLens[n], 0), p.VL) : p.VL;
+    x.ql = p.QLens ? min(max(mix_uniform(p.QLens[n]), 0), p.QL) : p.QL;
+    x.vl = p.VLens ? min(max(mix_uniform(p.VLens[n]), 0), p.VL) : p.VL;
     return x;
 }
 
@@ -56,12 +57,12 @@ struct WindowJob { int n, kvh, hd, qt, part; };
 __device__ __forceinline__ WindowJob window_job(const WindowParams& p, int id) {
     const int nkv = p.N * p.kv_head, group = p.head / p.kv_head;
     WindowJob x;
-    const int a = id / nkv, kv = id - a * nkv;
-    const int b = a / group, g = a - b * group;
-    const int qx = b / p.parts;
+    const int a = mix_uniform(id / nkv), kv = id - a * nkv;
+    const int b = mix_uniform(a / group), g = a - b * group;
+    const int qx = mix_uniform(b / p.parts);
     x.part = b - qx * p.parts;
     x.qt = p.qtiles - 1 - qx;
-    x.n = kv / p.kv_head;
+    x.n = mix_uniform(kv / p.kv_head);
     x.kvh = kv - x.n * p.kv_head;
     x.hd = x.kvh * group + g;
     return x;
@@ -69,10 +70,10 @@ __device__ __forceinline__ WindowJob window_job(const WindowParams& p, int id) {
 __device__ __forceinline__ WindowJob window_row_job(const WindowParams& p, int id) {
     const int nkv = p.N * p.kv_head;
     WindowJob x;
-    const int a = id / nkv, kv = id - a * nkv;
-    x.qt = a / p.parts;
+    const int a = mix_uniform(id / nkv), kv = id - a * nkv;
+    x.qt = mix_uniform(a / p.parts);
     x.part = a - x.qt * p.parts;
-    x.n = kv / p.kv_head;
+    x.n = mix_uniform(kv / p.kv_head);
     x.kvh = kv - x.n * p.kv_head;
     x.hd = 0;
     return x;

@@ -34,7 +34,7 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p
     __shared__ __attribute__((aligned(16))) float Ks[2][AK * DW];
     __shared__ __attribute__((aligned(16))) float Vs[2][AK * DW];
 
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 31, h = lane >> 5;
+    const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
     const WindowJob job = window_job(p, blockIdx.x);
     const WindowLens len = window_lens(p, job.n);
     const int q0 = job.qt * AQ;
@@ -47,8 +47,8 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p
     const int off = len.vl - len.ql;
     const WindowRange range = window_range(p, q0 + off, qn - 1 + off, q0 < qn, len.vl);
     const int nsink = (range.sink_end + AK - 1) / AK, nwin = (max(range.hi - range.low, 0) + AK - 1) / AK;
-    const int first = (int)((long long)(nsink + nwin) * job.part / p.parts);
-    const int last = (int)((long long)(nsink + nwin) * (job.part + 1) / p.parts);
+    const int first = mix_uniform((int)((long long)(nsink + nwin) * job.part / p.parts));
+    const int last = mix_uniform((int)((long long)(nsink + nwin) * (job.part + 1) / p.parts));
 
     const bool live = i < len.ql;
     const int pos = live ? i + off : -1;
@@ -68,10 +68,11 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p
     kt.init(t, p.k.l, p.dk4);
     vt.init(t, p.v.l, p.dv4);
     auto key_of = [&](int s) { return s < nsink ? s * AK : range.low + (s - nsink) * AK; };
-    auto fetch = [&](int s) {
+    const unsigned klds = mix_lds(Ks[0]) + wave * 1024, vlds = mix_lds(Vs[0]) + wave * 1024;
+    auto fetch = [&](int s, int into) {
         const int key0 = key_of(s), left = (s < nsink ? range.sink_end : range.hi) - key0;
-        kt.fetch(Kb + (size_t)key0 * p.k.l, left, p.k.l);
-        vt.fetch(Vb + (size_t)key0 * p.v.l, left, p.v.l);
+        kt.fetch(Kb + (size_t)key0 * p.k.l, left, p.k.l, klds + into * (AK * DW * 4));
+        vt.fetch(Vb + (size_t)key0 * p.v.l, left, p.v.l, vlds + into * (AK * DW * 4));
     };
 
     v16f o[DC];
@@ -80,15 +81,14 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p
     float m = NEG, l = 0.0f;                                // reference maximum (shared by the halves), this half's sum
 
     if (first < last) {
-        fetch(first);
-        kt.store(Ks[0]);
-        vt.store(Vs[0]);
+        fetch(first, 0);
+        mix_wait();
     }
     __syncthreads();
     int buf = 0;
     for (int s = first; s < last; s++) {
         const bool more = s + 1 < last;
-        if (more) fetch(s + 1);
+        if (more) fetch(s + 1, buf ^ 1);                    // nobody reads that buffer during this step
         __builtin_amdgcn_sched_barrier(0);
         const int key0 = key_of(s), limit = s < nsink ? range.sink_end : range.hi, end = min(key0 + AK, limit);
         // a wavefront none of whose queries sees a key of this step has nothing to do
@@ -141,10 +141,7 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) mix_columns_product<DW, DC, false>(o, Vs[buf] + kb * 32 * DW, sc[kb], vcols, r, h);
         }
-        if (more) {
-            kt.store(Ks[buf ^ 1]);
-            vt.store(Vs[buf ^ 1]);
-        }
+        mix_wait();
         __syncthreads();
         buf ^= 1;
     }
@@ -186,8 +183,8 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_rows(const WindowParams p)
     const int i0 = row0 / group, i1 = min((min(row0 + 16, rows) - 1) / group, len.ql - 1);
     const WindowRange range = window_range(p, i0 + off, i1 + off, i0 <= i1, len.vl);
     const int nsink = (range.sink_end + 15) / 16, nwin = (max(range.hi - range.low, 0) + 15) / 16;
-    const int first = (int)((long long)(nsink + nwin) * job.part / p.parts);
-    const int last = (int)((long long)(nsink + nwin) * (job.part + 1) / p.parts);
+    const int first = mix_uniform((int)((long long)(nsink + nwin) * job.part / p.parts));
+    const int last = mix_uniform((int)((long long)(nsink + nwin) * (job.part + 1) / p.parts));
 
     const float* qrow = p.Q + job.n * p.q.n + (size_t)min(hd, p.head - 1) * p.q.h + (size_t)min(i, p.QL - 1) * p.q.l;
     v4f qf[NS];

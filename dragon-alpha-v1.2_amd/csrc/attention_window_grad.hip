@@ -38,7 +38,8 @@ __global__ __launch_bounds__(NTHREADS) void window_delta(const WindowGrad p) {
     const int n = (int)(nh / p.w.head), hd = (int)(nh - (long long)n * p.w.head), i = (int)(row - nh * p.w.QL);
     const int d = 4 * (threadIdx.x & 31);
     float sum = 0.0f;
-    if (i < window_lens(p.w, n).ql && d < p.w.dv4) {
+    const int ql = p.w.QLens ? min(p.w.QLens[n], p.w.QL) : p.w.QL;
+    if (i < ql && d < p.w.dv4) {
         const size_t at = n * p.w.y.n + hd * p.w.y.h + (size_t)i * p.w.y.l + d;
         const v4f a = *(const v4f*)(p.dY + at), b = *(const v4f*)(p.w.Y + at);
         sum = (a.x * b.x + a.y * b.y) + (a.z * b.z + a.w * b.w);
@@ -55,7 +56,7 @@ __global__ __launch_bounds__(NTHREADS, DB > 2 ? 1 : 2) void window_grad_q(const 
     const WindowParams& p = a.w;
     __shared__ __attribute__((aligned(16))) float Ks[2][32 * DW];
     __shared__ __attribute__((aligned(16))) float Vs[2][32 * DW];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 31, h = lane >> 5;
+    const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
     const WindowJob job = window_job(p, blockIdx.x);
     const WindowLens len = window_lens(p, job.n);
     const int q0 = job.qt * GQ, i = q0 + wave * 32 + r;
@@ -82,24 +83,24 @@ __global__ __launch_bounds__(NTHREADS, DB > 2 ? 1 : 2) void window_grad_q(const 
     kt.init(t, p.k.l, p.dk4);
     vt.init(t, p.v.l, p.dv4);
     auto key_of = [&](int s) { return s < nsink ? s * 32 : range.low + (s - nsink) * 32; };
-    auto fetch = [&](int s) {
+    const unsigned klds = mix_lds(Ks[0]) + wave * 1024, vlds = mix_lds(Vs[0]) + wave * 1024;
+    auto fetch = [&](int s, int into) {
         const int key0 = key_of(s), left = (s < nsink ? range.sink_end : range.hi) - key0;
-        kt.fetch(Kb + (size_t)key0 * p.k.l, left, p.k.l);
-        vt.fetch(Vb + (size_t)key0 * p.v.l, left, p.v.l);
+        kt.fetch(Kb + (size_t)key0 * p.k.l, left, p.k.l, klds + into * (32 * DW * 4));
+        vt.fetch(Vb + (size_t)key0 * p.v.l, left, p.v.l, vlds + into * (32 * DW * 4));
     };
     v16f o[DC];
 #pragma unroll
     for (int b = 0; b < DC; b++) o[b] = (v16f)(0.0f);
     if (steps > 0) {
-        fetch(0);
-        kt.store(Ks[0]);
-        vt.store(Vs[0]);
+        fetch(0, 0);
+        mix_wait();
     }
     __syncthreads();
     int buf = 0;
     for (int s = 0; s < steps; s++) {
         const bool more = s + 1 < steps;
-        if (more) fetch(s + 1);
+        if (more) fetch(s + 1, buf ^ 1);
         __builtin_amdgcn_sched_barrier(0);
         const int key0 = key_of(s), limit = s < nsink ? range.sink_end : range.hi, end = min(key0 + 32, limit);
         const bool sees = s < nsink ? w0 <= w1 : (w0 <= w1 && key0 <= w1 && (end - 1 > w0 - p.window || key0 < p.sinks));
@@ -108,17 +109,19 @@ __global__ __launch_bounds__(NTHREADS, DB > 2 ? 1 : 2) void window_grad_q(const 
             mix_rows_product<DW, NG>(sc, Ks[buf], qf, r, h);
             mix_rows_product<DW, NG>(dp, Vs[buf], gf, r, h);
 #pragma unroll
-            for (int v = 0; v < 16; v++) {
-                const int j = key0 + mix_row(v, h);
-                const float ds = __builtin_amdgcn_exp2f(sc[v] - lse) * (dp[v] - D);
-                sc[v] = (j < limit && window_sees(p, pos, j)) ? ds : 0.0f;
+            for (int v = 0; v < 16; v++) sc[v] = __builtin_amdgcn_exp2f(sc[v] - lse) * (dp[v] - D);
+            // every query of the wavefront sees every key of the step: no test per score
+            const bool whole = key0 + 32 <= limit && key0 + 31 <= w0 && (s < nsink || key0 > w1 - p.window) && q0 + wave * 32 + 32 <= len.ql;
+            if (!whole) {
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    const int j = key0 + mix_row(v, h);
+                    if (!(j < limit && window_sees(p, pos, j))) sc[v] = 0.0f;
+                }
             }
             mix_columns_product<DW, DC, true>(o, Ks[buf], sc, cols, r, h);
         }
-        if (more) {
-            kt.store(Ks[buf ^ 1]);
-            vt.store(Vs[buf ^ 1]);
-        }
+        mix_wait();
         __syncthreads();
         buf ^= 1;
     }
@@ -133,16 +136,16 @@ __global__ __launch_bounds__(NTHREADS, DB > 2 ? 1 : 2) void window_grad_kv(const
     __shared__ __attribute__((aligned(16))) float Qs[2][32 * DW];
     __shared__ __attribute__((aligned(16))) float Gs[2][32 * DW];
     __shared__ __attribute__((aligned(16))) float Ls[2][32], Ds[2][32];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 31, h = lane >> 5;
+    const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
 
     // key tiles in order (the first are seen by the most queries), the sinks' in sink_parts each
     const int nkv = p.N * p.kv_head, group = p.head / p.kv_head;
-    const int x = blockIdx.x / nkv, kv = blockIdx.x - x * nkv;
+    const int x = mix_uniform(blockIdx.x / nkv), kv = blockIdx.x - x * nkv;
     const bool sink_tile = x < a.sink_tiles * a.sink_parts;
     const int parts = sink_tile ? a.sink_parts : a.parts;
     const int y = sink_tile ? x : x - a.sink_tiles * a.sink_parts;
-    const int tile = y / parts, part = y - tile * parts;
-    const int n = kv / p.kv_head, kvh = kv - n * p.kv_head;
+    const int tile = mix_uniform(y / parts), part = y - tile * parts;
+    const int n = mix_uniform(kv / p.kv_head), kvh = kv - n * p.kv_head;
     const int k0 = (sink_tile ? tile : a.sink_tiles + tile) * GK;
     const WindowLens len = window_lens(p, n);
     const int off = len.vl - len.ql;
@@ -154,7 +157,7 @@ __global__ __launch_bounds__(NTHREADS, DB > 2 ? 1 : 2) void window_grad_kv(const
     const int lo = max(k0 - off, 0);
     const int hi = k0 < k1 ? (k0 < p.sinks ? len.ql : min(len.ql, k1 - 1 + p.window - off)) : 0;
     const int per_head = (max(hi - lo, 0) + 31) / 32, total = per_head * group;
-    const int first = (int)((long long)total * part / parts), last = (int)((long long)total * (part + 1) / parts);
+    const int first = mix_uniform((int)((long long)total * part / parts)), last = mix_uniform((int)((long long)total * (part + 1) / parts));
 
     v4f kf[NG], vf[NG];
     mix_load_cols<NG>(kf, p.K + n * p.k.n + kvh * p.k.h + (size_t)min(key, p.VL - 1) * p.k.l, live, p.dk4, h);
@@ -168,33 +171,38 @@ __global__ __launch_bounds__(NTHREADS, DB > 2 ? 1 : 2) void window_grad_kv(const
     qt.init(t, p.q.l, p.dk4);
     gt.init(t, p.y.l, p.dv4);
     float stat_reg = 0.0f;
-    auto fetch = [&](int s) {
-        const int g = s / per_head, i0 = lo + (s - g * per_head) * 32, hd = kvh * group + g;
-        qt.fetch(p.Q + n * p.q.n + hd * p.q.h + (size_t)i0 * p.q.l, hi - i0, p.q.l);
-        gt.fetch(a.dY + n * p.y.n + hd * p.y.h + (size_t)i0 * p.y.l, hi - i0, p.y.l);
+    const unsigned qlds = mix_lds(Qs[0]) + wave * 1024, glds = mix_lds(Gs[0]) + wave * 1024;
+    // the step after (head g0 of the group, query tile i0) is (g0, i0 + 32) or the next head's first
+    auto fetch = [&](int g, int i0, int into) {
+        const int hd = kvh * group + g;
+        qt.fetch(p.Q + n * p.q.n + hd * p.q.h + (size_t)i0 * p.q.l, hi - i0, p.q.l, qlds + into * (32 * DW * 4));
+        gt.fetch(a.dY + n * p.y.n + hd * p.y.h + (size_t)i0 * p.y.l, hi - i0, p.y.l, glds + into * (32 * DW * 4));
         const size_t row = ((size_t)n * p.head + hd) * p.QL + i0 + (t & 31);
         if (t < 64) stat_reg = i0 + (t & 31) < hi ? (t < 32 ? p.Lse[row] * MIX_LOG2E : a.D[row]) : 0.0f;
     };
     auto store = [&](int into) {
-        qt.store(Qs[into]);
-        gt.store(Gs[into]);
         if (t < 32) Ls[into][t] = stat_reg;
         else if (t < 64) Ds[into][t - 32] = stat_reg;
     };
     v16f dk[DC], dv[DC];
 #pragma unroll
     for (int b = 0; b < DC; b++) { dk[b] = (v16f)(0.0f); dv[b] = (v16f)(0.0f); }
+    int g = 0, i0 = lo;
     if (first < last) {
-        fetch(first);
+        g = mix_uniform(first / per_head);
+        i0 = lo + (first - g * per_head) * 32;
+        fetch(g, i0, 0);
+        mix_wait();
         store(0);
     }
     __syncthreads();
     int buf = 0;
     for (int s = first; s < last; s++) {
         const bool more = s + 1 < last;
-        if (more) fetch(s + 1);
+        const bool turn = i0 + 32 >= hi;
+        const int next_g = turn ? g + 1 : g, next_i0 = turn ? lo : i0 + 32;
+        if (more) fetch(next_g, next_i0, buf ^ 1);
         __builtin_amdgcn_sched_barrier(0);
-        const int g = s / per_head, i0 = lo + (s - g * per_head) * 32;
         const int p0 = i0 + off, p1 = min(i0 + 32, hi) - 1 + off;      // the step's positions
         const bool sees = u0 <= u1 && p1 >= u0 && (p0 < u1 + p.window || u0 < p.sinks);
         if (sees) {
@@ -206,19 +214,31 @@ __global__ __launch_bounds__(NTHREADS, DB > 2 ? 1 : 2) void window_grad_kv(const
                 const v4f lse = *(const v4f*)&Ls[buf][8 * q + 4 * h], D = *(const v4f*)&Ds[buf][8 * q + 4 * h];
 #pragma unroll
                 for (int w = 0; w < 4; w++) {
-                    const int v = 4 * q + w, i = i0 + mix_row(v, h);
-                    const bool on = live && i < hi && window_sees(p, i + off, key);
-                    const float e = on ? __builtin_amdgcn_exp2f(sc[v] - lse[w]) : 0.0f;
-                    dp[v] = on ? e * (dp[v] - D[w]) : 0.0f;
-                    sc[v] = e;
+                    sc[4 * q + w] = __builtin_amdgcn_exp2f(sc[4 * q + w] - lse[w]);
+                    dp[4 * q + w] = dp[4 * q + w] - D[w];
                 }
             }
+            // every query of the step sees every key of the wavefront: no test per score
+            const bool whole = u0 + 32 <= len.vl && i0 + 32 <= hi && p0 >= u0 + 31 && p1 < u0 + p.window;
+            if (!whole) {
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    const int i = i0 + mix_row(v, h);
+                    // both: dP may be anything where nothing is seen
+                    if (!(live && i < hi && window_sees(p, i + off, key))) sc[v] = dp[v] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int v = 0; v < 16; v++) dp[v] *= sc[v];
             mix_columns_product<DW, DC, true>(dv, Gs[buf], sc, cols, r, h);
             mix_columns_product<DW, DC, true>(dk, Qs[buf], dp, cols, r, h);
         }
+        mix_wait();
         if (more) store(buf ^ 1);
         __syncthreads();
         buf ^= 1;
+        g = next_g;
+        i0 = next_i0;
     }
     if (key >= p.VL) return;
     if (parts == 1) {

@@ -22,7 +22,11 @@ for s in gemm_mfma.hip gemm_mfma_biased.hip gemm_mfma_dma.hip gemm_mfma_streamk.
     OBJS="$OBJS $o"
     continue
   fi
-  ( $HIPCC $HIPFLAGS -c "$s" -o "$o" 2>&1 | grep -v "packed-fp32-ops" >&2; exit ${PIPESTATUS[0]} ) &
+  # accumulators of matrix instructions stay in the vector registers that the vector instructions reach: with the
+  # compiler's own choice window_grad_kv moved all 128 of them out and in again in every step
+  EXTRA=""
+  [ "$s" = attention_window_grad.hip ] && EXTRA="-mllvm -amdgpu-mfma-vgpr-form=true"
+  ( $HIPCC $HIPFLAGS $EXTRA -c "$s" -o "$o" 2>&1 | grep -v "packed-fp32-ops" >&2; exit ${PIPESTATUS[0]} ) &
   PIDS="$PIDS $!"
   OBJS="$OBJS $o"
 done

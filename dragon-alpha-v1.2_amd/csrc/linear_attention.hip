@@ -25,6 +25,7 @@ namespace dragon {
 namespace {
 
 constexpr int TQ = 128;       // tokens per workgroup of decay_mix: 32 per wavefront
+constexpr int MAX_CHUNK = 256;
 
 struct DecayParams {
     const float* x; const float* y; const float* z; float* out;   // [L, xd], [L, xd], [L, zd], [L, zd] per (image, head)
@@ -53,13 +54,13 @@ __global__ __launch_bounds__(NTHREADS, 2) void decay_mix(const DecayParams p) {
     constexpr int DW = DB * 32, NG = DC * 4;
     __shared__ __attribute__((aligned(16))) float Ys[2][32 * DW];
     __shared__ __attribute__((aligned(16))) float Zs[2][32 * DW];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 31, h = lane >> 5;
+    const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
     const int lid = xcd_contiguous_id(blockIdx.x, gridDim.x);
-    const int nh = lid / p.tiles, tile = lid - nh * p.tiles;
-    const int n = nh / p.head, hd = nh - n * p.head;
-    const int len = decay_len(p.lens, n, p.L);
+    const int nh = mix_uniform(lid / p.tiles), tile = lid - nh * p.tiles;
+    const int n = mix_uniform(nh / p.head), hd = nh - n * p.head;
+    const int len = mix_uniform(decay_len(p.lens, n, p.L));
     const int q0 = tile * TQ, i = q0 + wave * 32 + r;
-    const int chunk = q0 / p.C, c0 = chunk * p.C, c1 = min(c0 + p.C, len);
+    const int chunk = mix_uniform(q0 / p.C), c0 = chunk * p.C, c1 = min(c0 + p.C, len);
     const float g2 = decay_log2(p.g, hd);
     const float* xb = p.x + n * p.lx.n + hd * p.lx.h;
     const float* yb = p.y + n * p.ly.n + hd * p.ly.h;
@@ -74,6 +75,9 @@ __global__ __launch_bounds__(NTHREADS, 2) void decay_mix(const DecayParams p) {
     MixColumns<DW, false> zcols;
     zcols.init(r, h);
 
+    const unsigned ylds = mix_lds(Ys[0]) + wave * 1024, zlds = mix_lds(Zs[0]) + wave * 1024;
+    constexpr unsigned TILE = 32 * DW * 4;
+
     // ---- x . S: 32 rows of the state per step ----
     const bool first_chunk = p.back ? c1 == len : chunk == 0;
     if (q0 < len && p.state != nullptr && !(first_chunk && p.empty_first)) {
@@ -81,23 +85,25 @@ __global__ __launch_bounds__(NTHREADS, 2) void decay_mix(const DecayParams p) {
         if constexpr (ST) {
             MixTile<DW, 32, true> st;
             st.init(t, p.xd, p.xd);
-            st.fetch(sb, p.zd, p.xd);
+            st.fetch(sb, p.zd, p.xd, ylds);
             static_for<DC>([&](auto bc) {
                 constexpr int b = decltype(bc)::value;
-                st.store(Ys[b & 1]);
+                mix_wait();
                 __syncthreads();
-                if (b + 1 < DC) st.fetch(sb + (size_t)(b + 1) * 32 * p.xd, p.zd - (b + 1) * 32, p.xd);
+                if (b + 1 < DC) st.fetch(sb + (size_t)(b + 1) * 32 * p.xd, p.zd - (b + 1) * 32, p.xd, ylds + ((b + 1) & 1) * TILE);
+                __builtin_amdgcn_sched_barrier(0);
                 mix_rows_product<DW, NG>(o[b], Ys[b & 1], xf, r, h);
             });
         } else {
             MixTile<DW, 32, false> st;
             st.init(t, p.zd, p.zd);
-            st.fetch(sb, p.xd, p.zd);
+            st.fetch(sb, p.xd, p.zd, zlds);
             static_for<DC>([&](auto bc) {
                 constexpr int b = decltype(bc)::value;
-                st.store(Zs[b & 1]);
+                mix_wait();
                 __syncthreads();
-                if (b + 1 < DC) st.fetch(sb + (size_t)(b + 1) * 32 * p.zd, p.xd - (b + 1) * 32, p.zd);
+                if (b + 1 < DC) st.fetch(sb + (size_t)(b + 1) * 32 * p.zd, p.xd - (b + 1) * 32, p.zd, zlds + ((b + 1) & 1) * TILE);
+                __builtin_amdgcn_sched_barrier(0);
                 v16f w;
 #pragma unroll
                 for (int v = 0; v < 16; v++) w[v] = xf[4 * b + v / 4][v % 4];
@@ -118,36 +124,43 @@ __global__ __launch_bounds__(NTHREADS, 2) void decay_mix(const DecayParams p) {
     MixTile<DW, 32, false> zt;
     yt.init(t, p.ly.l, p.xd);
     zt.init(t, p.lz.l, p.zd);
-    auto fetch = [&](int j0) {
-        yt.fetch(yb + (size_t)j0 * p.ly.l, to - j0, p.ly.l);
-        zt.fetch(zb + (size_t)j0 * p.lz.l, to - j0, p.lz.l);
+    auto fetch = [&](int j0, int into) {
+        yt.fetch(yb + (size_t)j0 * p.ly.l, to - j0, p.ly.l, ylds + into * TILE);
+        zt.fetch(zb + (size_t)j0 * p.lz.l, to - j0, p.lz.l, zlds + into * TILE);
     };
     if (from < to) {
-        fetch(from);
-        yt.store(Ys[0]);
-        zt.store(Zs[0]);
+        fetch(from, 0);
+        mix_wait();
     }
     __syncthreads();
     int buf = 0;
     const int w0 = q0 + wave * 32;
+    // e^(g distance) for 32 tokens that lie at least 32 away, but for a factor that is the same for all: both powers >= 0
+    float near[16];
+#pragma unroll
+    for (int v = 0; v < 16; v++) near[v] = decay_pow(g2, p.back ? 31 + mix_row(v, h) - r : 31 + r - mix_row(v, h));
     for (int j0 = from; j0 < to; j0 += 32) {
         const bool more = j0 + 32 < to;
-        if (more) fetch(j0 + 32);
+        if (more) fetch(j0 + 32, buf ^ 1);
         __builtin_amdgcn_sched_barrier(0);
         if (p.back ? j0 + 31 >= w0 : j0 <= w0 + 31) {
             v16f s = (v16f)(0.0f);
             mix_rows_product<DW, NG>(s, Ys[buf], xf, r, h);
+            const int away = p.back ? j0 - w0 : w0 - j0;       // of the step's 32 tokens from the wavefront's
+            if (away >= 32) {
+                const float f = decay_pow(g2, away - 31) * p.near_scale;
 #pragma unroll
-            for (int v = 0; v < 16; v++) {
-                const int j = j0 + mix_row(v, h), far = p.back ? j - i : i - j;
-                s[v] = far < 0 ? 0.0f : s[v] * (decay_pow(g2, far) * p.near_scale);
+                for (int v = 0; v < 16; v++) s[v] *= near[v] * f;
+            } else {
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    const int j = j0 + mix_row(v, h), far = p.back ? j - i : i - j;
+                    s[v] = far < 0 ? 0.0f : s[v] * (decay_pow(g2, far) * p.near_scale);
+                }
             }
             mix_columns_product<DW, DC, false>(o, Zs[buf], s, zcols, r, h);
         }
-        if (more) {
-            yt.store(Ys[buf ^ 1]);
-            zt.store(Zs[buf ^ 1]);
-        }
+        mix_wait();
         __syncthreads();
         buf ^= 1;
     }
@@ -172,10 +185,11 @@ __global__ __launch_bounds__(NTHREADS, 2) void decay_states(const DecayStates p)
     constexpr int TB = DC > 2 ? 2 : 1;
     __shared__ __attribute__((aligned(16))) float As[2][32 * DW];
     __shared__ __attribute__((aligned(16))) float Bs[2][32 * DW];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 31, h = lane >> 5;
-    const int nh = blockIdx.x / p.chunks, chunk = blockIdx.x - nh * p.chunks;
-    const int n = nh / p.head, hd = nh - n * p.head;
-    const int c0 = chunk * p.C, cnt = min(p.C, decay_len(p.lens, n, p.L) - c0);
+    __shared__ __attribute__((aligned(16))) float Ws[MAX_CHUNK];      // a token's power
+    const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
+    const int nh = mix_uniform(blockIdx.x / p.chunks), chunk = blockIdx.x - nh * p.chunks;
+    const int n = mix_uniform(nh / p.head), hd = nh - n * p.head;
+    const int c0 = chunk * p.C, cnt = min(p.C, mix_uniform(decay_len(p.lens, n, p.L)) - c0);
     if (cnt <= 0) return;                                // decay_scan does not read it
     const float g2 = decay_log2(p.g, hd);
     const float* ab = p.A + n * p.la.n + hd * p.la.h + (size_t)c0 * p.la.l;
@@ -183,18 +197,10 @@ __global__ __launch_bounds__(NTHREADS, 2) void decay_states(const DecayStates p)
     MixTile<DW, 32, false> at, bt;
     at.init(t, p.la.l, p.ad);
     bt.init(t, p.lb.l, p.bd);
-    auto fetch = [&](int j0) {
-        at.fetch(ab + (size_t)j0 * p.la.l, cnt - j0, p.la.l);
-        bt.fetch(bb + (size_t)j0 * p.lb.l, cnt - j0, p.lb.l);
-    };
-    auto store = [&](int j0, int into) {
-#pragma unroll
-        for (int s = 0; s < bt.PASSES; s++) {
-            const int j = j0 + t / bt.CPR + s * bt.RPP;
-            bt.reg[s] *= decay_pow(g2, max(p.back ? j + 1 : cnt - 1 - j, 0)) * p.scale;
-        }
-        at.store(As[into]);
-        bt.store(Bs[into]);
+    const unsigned alds = mix_lds(As[0]) + wave * 1024, blds = mix_lds(Bs[0]) + wave * 1024;
+    auto fetch = [&](int j0, int into) {
+        at.fetch(ab + (size_t)j0 * p.la.l, cnt - j0, p.la.l, alds + into * (32 * DW * 4));
+        bt.fetch(bb + (size_t)j0 * p.lb.l, cnt - j0, p.lb.l, blds + into * (32 * DW * 4));
     };
     const int wa = DC > 1 ? (wave >> 1) * TB : 0, wb = DC > 1 ? (wave & 1) * TB : 0;
     const bool works = DC > 1 ? (wa * 32 < p.ad && wb * 32 < p.bd) : wave == 0;
@@ -203,29 +209,34 @@ __global__ __launch_bounds__(NTHREADS, 2) void decay_states(const DecayStates p)
     for (int a = 0; a < TB; a++)
 #pragma unroll
         for (int b = 0; b < TB; b++) u[a][b] = (v16f)(0.0f);
-    fetch(0);
-    store(0, 0);
+    for (int j = t; j < MAX_CHUNK; j += NTHREADS) Ws[j] = decay_pow(g2, max(p.back ? j + 1 : cnt - 1 - j, 0)) * p.scale;
+    fetch(0, 0);
+    mix_wait();
     __syncthreads();
     int buf = 0;
     for (int j0 = 0; j0 < cnt; j0 += 32) {
-        const bool more = j0 + 32 < cnt;
-        if (more) fetch(j0 + 32);
+        if (j0 + 32 < cnt) fetch(j0 + 32, buf ^ 1);
         __builtin_amdgcn_sched_barrier(0);
         if (works) {
 #pragma unroll
-            for (int s = 0; s < 16; s++) {
-                float fa[TB], fb[TB];
+            for (int q = 0; q < 4; q++) {
+                const v4f w = *(const v4f*)&Ws[j0 + 8 * q + 4 * h];
 #pragma unroll
-                for (int a = 0; a < TB; a++) fa[a] = As[buf][(2 * s + h) * DW + (wa + a) * 32 + r];
+                for (int x = 0; x < 4; x++) {
+                    const int row = mix_row(4 * q + x, h);
+                    float fa[TB], fb[TB];
 #pragma unroll
-                for (int b = 0; b < TB; b++) fb[b] = Bs[buf][(2 * s + h) * DW + (wb + b) * 32 + r];
+                    for (int a = 0; a < TB; a++) fa[a] = As[buf][row * DW + (wa + a) * 32 + r];
 #pragma unroll
-                for (int a = 0; a < TB; a++)
+                    for (int b = 0; b < TB; b++) fb[b] = Bs[buf][row * DW + (wb + b) * 32 + r] * w[x];
 #pragma unroll
-                    for (int b = 0; b < TB; b++) u[a][b] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[a], fb[b], u[a][b], 0, 0, 0);
+                    for (int a = 0; a < TB; a++)
+#pragma unroll
+                        for (int b = 0; b < TB; b++) u[a][b] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[a], fb[b], u[a][b], 0, 0, 0);
+                }
             }
         }
-        if (more) store(j0 + 32, buf ^ 1);
+        mix_wait();
         __syncthreads();
         buf ^= 1;
     }

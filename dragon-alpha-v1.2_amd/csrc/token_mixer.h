@@ -24,35 +24,44 @@ __device__ __forceinline__ float mix_xhalf(float x) { return __shfl_xor(x, 32, 6
 // the sequence row that result register v of lane half h stands for
 __device__ __forceinline__ constexpr int mix_row(int v, int h) { return 8 * (v / 4) + 4 * h + (v % 4); }
 
-// Staging of one [ROWS][DW] tile by the 256 threads of a workgroup, through registers.  A lane's byte offsets inside the
-// tile never change; the tile's first row goes into the descriptor's base and the rows that exist into its size, so rows
-// beyond them and chunks beyond the row's d4 floats read as zeros and a fetch costs scalar instructions only.
+__device__ __forceinline__ int mix_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// the byte address of LDS memory, for transfers
+__device__ __forceinline__ unsigned mix_lds(const float* lds) {
+    return (unsigned)(unsigned long long)(__attribute__((address_space(3))) const float*)lds;
+}
+// this wavefront's transfers have landed
+__device__ __forceinline__ void mix_wait() { __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); }
+
+// One [ROWS][DW] tile from memory straight into LDS by the 256 threads of a workgroup: no staging registers, no vector
+// instructions (which the matrix pipe would wait for).  The hardware puts lane l's 16 bytes at the wave's base + 16 * l, so
+// the swizzle moves to the global side: the lane at slot c of row r fetches chunk c ^ swizzle(r).  A lane's byte offset
+// never changes; the tile's first row goes into the descriptor's base and the rows that exist into its size, so rows beyond
+// them and chunks beyond the row's d4 floats arrive as zeros.  Everything but the offsets has to be uniform.
 template <int DW, int ROWS, bool SWIZZLE>
 struct MixTile {
     static constexpr int CPR = DW / 4, RPP = NTHREADS / CPR, PASSES = ROWS / RPP;
     static_assert(PASSES * RPP == ROWS && PASSES >= 1, "the tile divides over the workgroup");
-    int off[PASSES], at[PASSES];
-    v4f reg[PASSES];
+    int off[PASSES];
     __device__ __forceinline__ void init(int t, int pitch, int d4) {
-        const int chunk = t % CPR, row0 = t / CPR;
+        const int slot = t % CPR, row0 = t / CPR;
 #pragma unroll
         for (int s = 0; s < PASSES; s++) {
-            const int row = row0 + s * RPP;
+            const int row = row0 + s * RPP, chunk = SWIZZLE ? (slot ^ kin_swizzle<DW>(row)) : slot;
             off[s] = chunk * 4 < d4 ? (row * pitch + chunk * 4) * 4 : OOB_OFFSET;
-            at[s] = row * DW + 4 * (SWIZZLE ? (chunk ^ kin_swizzle<DW>(row)) : chunk);
         }
     }
-    // rows [0, left) of the tile that starts at `base`; left < 1 reads nothing
-    __device__ __forceinline__ void fetch(const float* base, int left, int pitch) {
+    // rows [0, left) of the tile that starts at `base` into the LDS tile whose address for this wavefront is `lds`
+    // (mix_lds of the tile + 1024 * wavefront); left < 1: zeros
+    __device__ __forceinline__ void fetch(const float* base, int left, int pitch, unsigned lds) const {
         const int rows = left < 0 ? 0 : (left < ROWS ? left : ROWS);
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, rows * pitch * 4, RSRC_FLAGS);
-#pragma unroll
-        for (int s = 0; s < PASSES; s++)
-            reg[s] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(r, off[s], 0, 0));
-    }
-    __device__ __forceinline__ void store(float* lds) const {
-#pragma unroll
-        for (int s = 0; s < PASSES; s++) *(v4f*)(lds + at[s]) = reg[s];
+        const unsigned long long b = (unsigned long long)base;
+        const v4u rsrc = {(unsigned)mix_uniform((int)b), (unsigned)mix_uniform((int)(b >> 32)) & 0xffffu,
+                          (unsigned)mix_uniform(rows * pitch * 4), (unsigned)RSRC_FLAGS};
+        const unsigned to = (unsigned)mix_uniform((int)lds);
+        static_for<PASSES>([&](auto sc) {
+            constexpr int s = decltype(sc)::value;
+            dma_f4_lean<s * NTHREADS * 16>(rsrc, to, off[s]);
+        });
     }
 };
 
