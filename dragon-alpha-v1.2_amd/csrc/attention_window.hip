@@ -25,7 +25,7 @@ namespace {
 constexpr int AQ = 128;          // queries per workgroup of the tiled kernel: 32 per wavefront
 constexpr int LAG = 8;           // the reference maximum may lag the true one by 2^LAG
 constexpr float NEG = -__builtin_inff();
-constexpr float LOWEST = -3.0e38f;
+constexpr float LOWEST = -3.0e38f;   // below every score that is not -infinity
 
 // ---------------------------------------------------------------- many queries
 template <int DB, int DC, int KB>
@@ -78,63 +78,73 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p
     v16f o[DC];
 #pragma unroll
     for (int b = 0; b < DC; b++) o[b] = (v16f)(0.0f);
-    float m = NEG, l = 0.0f;                                // reference maximum (shared by the halves), this half's sum
+    // Scores are formed relative to a reference: the accumulators start at its negative, so the exponentials need no
+    // subtraction.  It starts at the first scores' maximum (until then it is 0 and `raise` lets any score through) and is
+    // raised only when some score exceeds it by 2^LAG -- any reference gives the same result after the final division.
+    v16f from = (v16f)(0.0f);                               // minus the reference, 16 times
+    float raise = LOWEST, l = 0.0f;                         // l: this half's sum
 
-    if (first < last) {
-        fetch(first, 0);
-        mix_wait();
-    }
+    if (first < last) fetch(first, 0);
+    mix_wait();               // also for the loads above: the compiler would wait for them, and the step's transfers, in every step
     __syncthreads();
-    int buf = 0;
-    for (int s = first; s < last; s++) {
-        const bool more = s + 1 < last;
-        if (more) fetch(s + 1, buf ^ 1);                    // nobody reads that buffer during this step
+    auto step = [&](auto bufc, int s) {
+        constexpr int buf = decltype(bufc)::value;
+        if (s + 1 < last) fetch(s + 1, buf ^ 1);            // nobody reads that buffer during this step
         __builtin_amdgcn_sched_barrier(0);
         const int key0 = key_of(s), limit = s < nsink ? range.sink_end : range.hi, end = min(key0 + AK, limit);
         // a wavefront none of whose queries sees a key of this step has nothing to do
-        const bool sees = s < nsink ? w0 <= w1 : (w0 <= w1 && key0 <= w1 && (end - 1 > w0 - p.window || key0 < p.sinks));
+        const bool sees = w0 <= w1 && (s < nsink || (key0 <= w1 && (end - 1 > w0 - p.window || key0 < p.sinks)));
         if (sees) {
             v16f sc[KB];
-            const float* ks = Ks[buf];
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) {
-                sc[kb] = (v16f)(0.0f);
-                mix_rows_product<DW, NG>(sc[kb], ks + kb * 32 * DW, qf, r, h);
+                sc[kb] = from;
+                mix_rows_product<DW, NG>(sc[kb], Ks[buf] + kb * 32 * DW, qf, r, h);
             }
-            // every query of the wavefront sees every key of the step: no test per score
-            const bool whole = key0 + AK <= limit && key0 + AK - 1 <= w0 && (s < nsink || key0 > w1 - p.window) && q0 + wave * 32 + 32 <= len.ql;
-            if (!whole) {
+            // keys behind a query (or behind the last key), and before its window: tested only where some query has them
+            if (key0 + AK - 1 > w0 || key0 + AK > limit || q0 + wave * 32 + 32 > len.ql) {
+                const int top = min(pos, limit - 1) - key0 - 4 * h;
 #pragma unroll
                 for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-                    for (int v = 0; v < 16; v++) {
-                        const int j = key0 + 32 * kb + mix_row(v, h);
-                        if (!(j < limit && window_sees(p, pos, j))) sc[kb][v] = NEG;
-                    }
+                    for (int v = 0; v < 16; v++)
+                        if (32 * kb + mix_row(v, 0) > top) sc[kb][v] = NEG;
+            }
+            if (s >= nsink && key0 <= w1 - p.window) {
+                const int low = pos - p.window - key0 - 4 * h, sink = p.sinks - key0 - 4 * h;
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++)
+                        if (32 * kb + mix_row(v, 0) <= low && 32 * kb + mix_row(v, 0) >= sink) sc[kb][v] = NEG;
             }
             float mt = sc[0][0];
 #pragma unroll
             for (int kb = 0; kb < KB; kb++)
 #pragma unroll
                 for (int v = (kb == 0); v < 16; v++) mt = fmaxf(mt, sc[kb][v]);
-            mt = fmaxf(mt, mix_xhalf(mt));
-            if (__builtin_amdgcn_ballot_w64(mt > m + (float)LAG) != 0) {
-                const float m_new = fmaxf(m, mt);
-                const float alpha = m == NEG ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
-                m = m_new;
+            const MixHalves both = mix_halves(mt);
+            mt = fmaxf(both.a, both.b);
+            if (__builtin_amdgcn_ballot_w64(mt > raise) != 0) {
+                const bool begun = raise != LOWEST;
+                const float up = begun ? fmaxf(mt, 0.0f) : (mt == NEG ? 0.0f : mt);
+                const float alpha = begun ? __builtin_amdgcn_exp2f(-up) : 0.0f;
+                if (mt > raise) raise = (float)LAG;
                 l *= alpha;
+                from -= up;
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++) sc[kb] -= up;
 #pragma unroll
                 for (int b = 0; b < DC; b++)
 #pragma unroll
                     for (int v = 0; v < 16; v++) o[b][v] *= alpha;
             }
-            const float ref = fmaxf(m, LOWEST);             // a query that has seen nothing yet: exp2(-inf) below, not -inf + inf
             float sum = 0.0f;
 #pragma unroll
             for (int kb = 0; kb < KB; kb++)
 #pragma unroll
                 for (int v = 0; v < 16; v++) {
-                    sc[kb][v] = __builtin_amdgcn_exp2f(sc[kb][v] - ref);
+                    sc[kb][v] = __builtin_amdgcn_exp2f(sc[kb][v]);
                     sum += sc[kb][v];
                 }
             l += sum;
@@ -143,10 +153,15 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p
         }
         mix_wait();
         __syncthreads();
-        buf ^= 1;
+    };
+    for (int s = first; s < last; s += 2) {                 // the buffer is a constant in each copy of the step
+        step(std::integral_constant<int, 0>{}, s);
+        if (s + 1 < last) step(std::integral_constant<int, 1>{}, s + 1);
     }
 
-    l += mix_xhalf(l);
+    const MixHalves sums = mix_halves(l);
+    l = sums.a + sums.b;
+    const float m = raise == LOWEST ? NEG : -from[0];
     if (i >= p.QL) return;
     if (p.parts == 1) {
         mix_store_row<DC>(Yb + (size_t)i * p.y.l, o, l == 0.0f ? 0.0f : 1.0f / l, p.dv4, h);

@@ -51,7 +51,7 @@ __global__ __launch_bounds__(NTHREADS) void window_delta(const WindowGrad p) {
 
 // ---------------------------------------------------------------- dQ
 template <int DB, int DC>
-__global__ __launch_bounds__(NTHREADS, DB > 2 ? 1 : 2) void window_grad_q(const WindowGrad a) {
+__global__ __launch_bounds__(NTHREADS, 2) void window_grad_q(const WindowGrad a) {
     constexpr int DW = DB * 32, NG = DC * 4;
     const WindowParams& p = a.w;
     __shared__ __attribute__((aligned(16))) float Ks[2][32 * DW];
@@ -74,6 +74,7 @@ __global__ __launch_bounds__(NTHREADS, DB > 2 ? 1 : 2) void window_grad_q(const 
 #pragma unroll
     for (int g = 0; g < NG; g++) qf[g] *= p.c;
     const float lse = live ? p.Lse[stat] * MIX_LOG2E : 0.0f, D = live ? a.D[stat] : 0.0f;
+    const v16f from = (v16f)(-lse);                         // where the score products start: P = exp2 of the result
 
     const float* Kb = p.K + job.n * p.k.n + job.kvh * p.k.h;
     const float* Vb = p.V + job.n * p.v.n + job.kvh * p.v.h;
@@ -92,38 +93,42 @@ __global__ __launch_bounds__(NTHREADS, DB > 2 ? 1 : 2) void window_grad_q(const 
     v16f o[DC];
 #pragma unroll
     for (int b = 0; b < DC; b++) o[b] = (v16f)(0.0f);
-    if (steps > 0) {
-        fetch(0, 0);
-        mix_wait();
-    }
+    if (steps > 0) fetch(0, 0);
+    mix_wait();
     __syncthreads();
-    int buf = 0;
-    for (int s = 0; s < steps; s++) {
-        const bool more = s + 1 < steps;
-        if (more) fetch(s + 1, buf ^ 1);
+    auto step = [&](auto bufc, int s) {
+        constexpr int buf = decltype(bufc)::value;
+        if (s + 1 < steps) fetch(s + 1, buf ^ 1);
         __builtin_amdgcn_sched_barrier(0);
         const int key0 = key_of(s), limit = s < nsink ? range.sink_end : range.hi, end = min(key0 + 32, limit);
-        const bool sees = s < nsink ? w0 <= w1 : (w0 <= w1 && key0 <= w1 && (end - 1 > w0 - p.window || key0 < p.sinks));
+        const bool sees = w0 <= w1 && (s < nsink || (key0 <= w1 && (end - 1 > w0 - p.window || key0 < p.sinks)));
         if (sees) {
-            v16f sc = (v16f)(0.0f), dp = (v16f)(0.0f);
+            v16f sc = from, dp = (v16f)(0.0f);
             mix_rows_product<DW, NG>(sc, Ks[buf], qf, r, h);
             mix_rows_product<DW, NG>(dp, Vs[buf], gf, r, h);
 #pragma unroll
-            for (int v = 0; v < 16; v++) sc[v] = __builtin_amdgcn_exp2f(sc[v] - lse) * (dp[v] - D);
-            // every query of the wavefront sees every key of the step: no test per score
-            const bool whole = key0 + 32 <= limit && key0 + 31 <= w0 && (s < nsink || key0 > w1 - p.window) && q0 + wave * 32 + 32 <= len.ql;
-            if (!whole) {
+            for (int v = 0; v < 16; v++) sc[v] = __builtin_amdgcn_exp2f(sc[v]) * (dp[v] - D);
+            // keys behind a query (or behind the last key), and before its window: tested only where some query has them
+            if (key0 + 31 > w0 || key0 + 32 > limit || q0 + wave * 32 + 32 > len.ql) {
+                const int top = min(pos, limit - 1) - key0 - 4 * h;
 #pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    const int j = key0 + mix_row(v, h);
-                    if (!(j < limit && window_sees(p, pos, j))) sc[v] = 0.0f;
-                }
+                for (int v = 0; v < 16; v++)
+                    if (mix_row(v, 0) > top) sc[v] = 0.0f;
+            }
+            if (s >= nsink && key0 <= w1 - p.window) {
+                const int low = pos - p.window - key0 - 4 * h, sink = p.sinks - key0 - 4 * h;
+#pragma unroll
+                for (int v = 0; v < 16; v++)
+                    if (mix_row(v, 0) <= low && mix_row(v, 0) >= sink) sc[v] = 0.0f;
             }
             mix_columns_product<DW, DC, true>(o, Ks[buf], sc, cols, r, h);
         }
         mix_wait();
         __syncthreads();
-        buf ^= 1;
+    };
+    for (int s = 0; s < steps; s += 2) {
+        step(std::integral_constant<int, 0>{}, s);
+        if (s + 1 < steps) step(std::integral_constant<int, 1>{}, s + 1);
     }
     if (i < p.QL) mix_store_row<DC>(a.dQ + job.n * p.q.n + job.hd * p.q.h + (size_t)i * p.q.l, o, a.scale, p.dk4, h);
 }
@@ -192,12 +197,12 @@ __global__ __launch_bounds__(NTHREADS, DB > 2 ? 1 : 2) void window_grad_kv(const
         g = mix_uniform(first / per_head);
         i0 = lo + (first - g * per_head) * 32;
         fetch(g, i0, 0);
-        mix_wait();
-        store(0);
     }
+    mix_wait();
+    store(0);
     __syncthreads();
-    int buf = 0;
-    for (int s = first; s < last; s++) {
+    auto step = [&](auto bufc, int s) {
+        constexpr int buf = decltype(bufc)::value;
         const bool more = s + 1 < last;
         const bool turn = i0 + 32 >= hi;
         const int next_g = turn ? g + 1 : g, next_i0 = turn ? lo : i0 + 32;
@@ -218,15 +223,19 @@ __global__ __launch_bounds__(NTHREADS, DB > 2 ? 1 : 2) void window_grad_kv(const
                     dp[4 * q + w] = dp[4 * q + w] - D[w];
                 }
             }
-            // every query of the step sees every key of the wavefront: no test per score
-            const bool whole = u0 + 32 <= len.vl && i0 + 32 <= hi && p0 >= u0 + 31 && p1 < u0 + p.window;
-            if (!whole) {
+            // queries before a key, those whose window has passed it, and rows behind the last: tested only where there are any.
+            // Both factors are cleared: dP may be anything where nothing is seen.
+            if (p0 < u1 || i0 + 32 > hi || u0 + 32 > len.vl) {
+                const int low = (live ? key : 0x3fffffff) - p0 - 4 * h, top = hi - 1 - i0 - 4 * h;
 #pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    const int i = i0 + mix_row(v, h);
-                    // both: dP may be anything where nothing is seen
-                    if (!(live && i < hi && window_sees(p, i + off, key))) sc[v] = dp[v] = 0.0f;
-                }
+                for (int v = 0; v < 16; v++)
+                    if (mix_row(v, 0) < low || mix_row(v, 0) > top) sc[v] = dp[v] = 0.0f;
+            }
+            if (p1 >= u0 + p.window) {
+                const int top = key < p.sinks ? 0x3fffffff : key + p.window - 1 - p0 - 4 * h;
+#pragma unroll
+                for (int v = 0; v < 16; v++)
+                    if (mix_row(v, 0) > top) sc[v] = dp[v] = 0.0f;
             }
 #pragma unroll
             for (int v = 0; v < 16; v++) dp[v] *= sc[v];
@@ -236,9 +245,12 @@ __global__ __launch_bounds__(NTHREADS, DB > 2 ? 1 : 2) void window_grad_kv(const
         mix_wait();
         if (more) store(buf ^ 1);
         __syncthreads();
-        buf ^= 1;
         g = next_g;
         i0 = next_i0;
+    };
+    for (int s = first; s < last; s += 2) {
+        step(std::integral_constant<int, 0>{}, s);
+        if (s + 1 < last) step(std::integral_constant<int, 1>{}, s + 1);
     }
     if (key >= p.VL) return;
     if (parts == 1) {

@@ -37,7 +37,7 @@ struct DecayParams {
     const float* state;        // the state before each chunk, [image, head, chunk]; null: none at all
     int empty_first;           // the state at the sequence's beginning (back: at its end) is zero
     long long state_nh, state_c;   // its strides
-    int tiles;
+    int tiles, nh;
 };
 
 __device__ __forceinline__ float decay_log2(const float* g, int hd) {
@@ -56,10 +56,12 @@ __global__ __launch_bounds__(NTHREADS, 2) void decay_mix(const DecayParams p) {
     __shared__ __attribute__((aligned(16))) float Zs[2][32 * DW];
     const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
     const int lid = xcd_contiguous_id(blockIdx.x, gridDim.x);
-    const int nh = mix_uniform(lid / p.tiles), tile = lid - nh * p.tiles;
+    const int tile = mix_uniform(lid / p.nh), nh = lid - tile * p.nh;
     const int n = mix_uniform(nh / p.head), hd = nh - n * p.head;
     const int len = mix_uniform(decay_len(p.lens, n, p.L));
-    const int q0 = tile * TQ, i = q0 + wave * 32 + r;
+    // Inside a chunk the later (back: the earlier) 32 tokens have the most to do.  The workgroups that share a compute unit
+    // give them to different wavefronts, so that no SIMD has all the work.
+    const int q0 = tile * TQ, w0 = q0 + 32 * ((blockIdx.x >> 8) & 1 ? 3 - wave : wave), i = w0 + r;
     const int chunk = mix_uniform(q0 / p.C), c0 = chunk * p.C, c1 = min(c0 + p.C, len);
     const float g2 = decay_log2(p.g, hd);
     const float* xb = p.x + n * p.lx.n + hd * p.lx.h;
@@ -128,41 +130,42 @@ __global__ __launch_bounds__(NTHREADS, 2) void decay_mix(const DecayParams p) {
         yt.fetch(yb + (size_t)j0 * p.ly.l, to - j0, p.ly.l, ylds + into * TILE);
         zt.fetch(zb + (size_t)j0 * p.lz.l, to - j0, p.lz.l, zlds + into * TILE);
     };
-    if (from < to) {
-        fetch(from, 0);
-        mix_wait();
-    }
-    __syncthreads();
-    int buf = 0;
-    const int w0 = q0 + wave * 32;
-    // e^(g distance) for 32 tokens that lie at least 32 away, but for a factor that is the same for all: both powers >= 0
-    float near[16];
+    // e^(g distance) inside the wavefront's own 32 tokens, and for 32 tokens that lie at least 32 away but for a factor that
+    // is the same for all of them: every power here is >= 0
+    float own[16], near[16];
 #pragma unroll
-    for (int v = 0; v < 16; v++) near[v] = decay_pow(g2, p.back ? 31 + mix_row(v, h) - r : 31 + r - mix_row(v, h));
-    for (int j0 = from; j0 < to; j0 += 32) {
-        const bool more = j0 + 32 < to;
-        if (more) fetch(j0 + 32, buf ^ 1);
+    for (int v = 0; v < 16; v++) {
+        const int far = p.back ? mix_row(v, h) - r : r - mix_row(v, h);
+        own[v] = far < 0 ? 0.0f : decay_pow(g2, far) * p.near_scale;
+        near[v] = decay_pow(g2, 31 + far) * p.near_scale;
+    }
+    if (from < to) fetch(from, 0);
+    mix_wait();
+    __syncthreads();
+    auto step = [&](auto bufc, int j0) {
+        constexpr int buf = decltype(bufc)::value;
+        if (j0 + 32 < to) fetch(j0 + 32, buf ^ 1);
         __builtin_amdgcn_sched_barrier(0);
-        if (p.back ? j0 + 31 >= w0 : j0 <= w0 + 31) {
+        const int away = p.back ? j0 - w0 : w0 - j0;        // a multiple of 32
+        if (away >= 0) {
             v16f s = (v16f)(0.0f);
             mix_rows_product<DW, NG>(s, Ys[buf], xf, r, h);
-            const int away = p.back ? j0 - w0 : w0 - j0;       // of the step's 32 tokens from the wavefront's
-            if (away >= 32) {
-                const float f = decay_pow(g2, away - 31) * p.near_scale;
+            if (away > 0) {
+                const float f = decay_pow(g2, away - 31);
 #pragma unroll
                 for (int v = 0; v < 16; v++) s[v] *= near[v] * f;
             } else {
 #pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    const int j = j0 + mix_row(v, h), far = p.back ? j - i : i - j;
-                    s[v] = far < 0 ? 0.0f : s[v] * (decay_pow(g2, far) * p.near_scale);
-                }
+                for (int v = 0; v < 16; v++) s[v] *= own[v];
             }
             mix_columns_product<DW, DC, false>(o, Zs[buf], s, zcols, r, h);
         }
         mix_wait();
         __syncthreads();
-        buf ^= 1;
+    };
+    for (int j0 = from; j0 < to; j0 += 64) {
+        step(std::integral_constant<int, 0>{}, j0);
+        if (j0 + 32 < to) step(std::integral_constant<int, 1>{}, j0 + 32);
     }
     if (i < p.L) mix_store_row<DC>(p.out + n * p.lo.n + hd * p.lo.h + (size_t)i * p.lo.l, o, 1.0f, p.zd, h);
 }
@@ -176,6 +179,7 @@ struct DecayStates {
     int head, L, ad, bd, C, chunks, back;
     float scale;
     float* U;                 // [image, head, chunk][ad][bd]
+    int nh;
 };
 
 template <int DB, int DC>
@@ -187,7 +191,8 @@ __global__ __launch_bounds__(NTHREADS, 2) void decay_states(const DecayStates p)
     __shared__ __attribute__((aligned(16))) float Bs[2][32 * DW];
     __shared__ __attribute__((aligned(16))) float Ws[MAX_CHUNK];      // a token's power
     const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
-    const int nh = mix_uniform(blockIdx.x / p.chunks), chunk = blockIdx.x - nh * p.chunks;
+    const int lid = xcd_contiguous_id(blockIdx.x, gridDim.x);
+    const int chunk = mix_uniform(lid / p.nh), nh = lid - chunk * p.nh;
     const int n = mix_uniform(nh / p.head), hd = nh - n * p.head;
     const int c0 = chunk * p.C, cnt = min(p.C, mix_uniform(decay_len(p.lens, n, p.L)) - c0);
     if (cnt <= 0) return;                                // decay_scan does not read it
@@ -241,7 +246,7 @@ __global__ __launch_bounds__(NTHREADS, 2) void decay_states(const DecayStates p)
         buf ^= 1;
     }
     if (!works) return;
-    float* U = p.U + (size_t)blockIdx.x * p.ad * p.bd;
+    float* U = p.U + ((size_t)nh * p.chunks + chunk) * p.ad * p.bd;
 #pragma unroll
     for (int a = 0; a < TB; a++)
 #pragma unroll
@@ -373,7 +378,7 @@ bool decay_arguments_ok(int N, int head, int L, int dK4, int dV4) {
 
 hipError_t launch_states(hipStream_t s, const float* A, MixLayout la, int ad, const float* B, MixLayout lb, int bd, const float* g,
                          const int* lens, int N, int head, int L, int C, int back, float scale, float* U) {
-    DecayStates p = {A, B, la, lb, g, lens, head, L, ad, bd, C, (L + C - 1) / C, back, scale, U};
+    DecayStates p = {A, B, la, lb, g, lens, head, L, ad, bd, C, (L + C - 1) / C, back, scale, U, N * head};
     const dim3 grid((unsigned)((long long)N * head * p.chunks)), block(NTHREADS);
     switch (((ad > bd ? ad : bd) + 31) / 32) {
         case 1: hipLaunchKernelGGL((decay_states<1, 1>), grid, block, 0, s, p); break;
@@ -447,7 +452,7 @@ int dragon_Cuda_linear_attention_forward(const int64_t* streams, int32_t length,
     }
     const int C = decay_chunk(dK4, dV4), chunks = (L + C - 1) / C;
     DecayParams p = {Q, K, V, Y, lk, lk, lv, lv, g, lens, head, L, dK4, dV4, C, chunks, 0, scale, scale, first, first == nullptr,
-                     (long long)state, 0, (L + TQ - 1) / TQ};
+                     (long long)state, 0, (L + TQ - 1) / TQ, N * head};
     if (chunks > 1 || last != nullptr) {
         hipError_t e = launch_states(s, K, lk, dK4, V, lv, dV4, g, lens, N, head, L, C, 0, 1.0f, U);
         if (e == hipSuccess) e = launch_scan(s, U, first, last, g, lens, N, head, L, C, 0, (int)state);
@@ -501,7 +506,7 @@ int dragon_Cuda_linear_attention_backward(const int64_t* streams, int32_t length
     }
     if (e != hipSuccess) return e;
     DecayParams p = {G, V, K, gQ, lv, lv, lk, lk, g, lens, head, L, dV4, dK4, C, chunks, 0, scale, scale,
-                     many ? S : first, first == nullptr, many ? chunks * state : state, many ? state : 0, (L + TQ - 1) / TQ};
+                     many ? S : first, first == nullptr, many ? chunks * state : state, many ? state : 0, (L + TQ - 1) / TQ, N * head};
     e = launch_mix<true>(s, p, N);
     p.back = 1; p.far_scale = 1.0f;
     p.state = later ? R : dlast; p.empty_first = dlast == nullptr;

@@ -19,7 +19,12 @@ namespace {
 constexpr float MIX_LOG2E = 1.44269504088896340736f;
 constexpr float MIX_LN2 = 0.69314718055994530942f;
 
-__device__ __forceinline__ float mix_xhalf(float x) { return __shfl_xor(x, 32, 64); }
+// the values that lane r of either half holds, in both: {of half 0, of half 1}
+struct MixHalves { float a, b; };
+__device__ __forceinline__ MixHalves mix_halves(float x) {
+    const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+    return {__builtin_bit_cast(float, (unsigned)y[0]), __builtin_bit_cast(float, (unsigned)y[1])};
+}
 
 // the sequence row that result register v of lane half h stands for
 __device__ __forceinline__ constexpr int mix_row(int v, int h) { return 8 * (v / 4) + 4 * h + (v % 4); }
@@ -65,6 +70,19 @@ struct MixTile {
     }
 };
 
+// The order in which a product's LDS reads and matrix instructions are issued: READS reads first, then always one read behind
+// MFMAS matrix instructions.  Left alone the compiler reads an operand just before it is needed and the matrix pipe waits
+// for LDS between any two uses.
+template <int READS, int TOTAL, int MFMAS>
+__device__ __forceinline__ void mix_order() {
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    static_for<TOTAL - READS>([&](auto) {
+        __builtin_amdgcn_sched_group_barrier(0x8, MFMAS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    });
+    __builtin_amdgcn_sched_group_barrier(0x8, READS * MFMAS, 0);
+}
+
 // result[row of the tile][column] += tile . cols^T over the head dimension: cols[g] holds d = 8g + 4h .. +3 of the lane's
 // column; the tile is swizzled
 template <int DW, int NG>
@@ -78,6 +96,7 @@ __device__ __forceinline__ void mix_rows_product(v16f& s, const float* tile, con
         s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, cols[g].z, s, 0, 0, 0);
         s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, cols[g].w, s, 0, 0, 0);
     }
+    mix_order<2, NG, 4>();
 }
 
 // Where lane (r, h) finds float 32b + r of tile row mix_row(v, h).  With the swizzle the place is a lane's part that depends
@@ -108,6 +127,7 @@ __device__ __forceinline__ void mix_columns_product(v16f (&o)[DC], const float* 
 #pragma unroll
         for (int b = 0; b < DC; b++) o[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(cols.read(tile, v, b, r, h), p[v], o[b], 0, 0, 0);
     }
+    mix_order<4, 16 * DC / 2, 2>();                       // the compiler reads two values at a time
 }
 
 // a lane's column of a result, times f: float 32b + 8g + 4h .. +3 of the row at `row`
