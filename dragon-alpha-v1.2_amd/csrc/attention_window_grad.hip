@@ -6,9 +6,13 @@
 // walks over the queries that see them, head by head of the group.  That is seven products of which five are necessary:
 // the score and the dY.V^T products happen in both.  Bound by the FP32 matrix pipe.
 //
-// A key tile with sinks is seen by all queries behind it, any other by window + 128 of them: the sinks' tile is cut along the
-// queries (as every tile is where there are few), each part leaves its sums in the caller's buffer and
-// window_grad_join adds them in order.
+// Both run eight wavefronts, two per 32 queries (or keys) and on one SIMD.  The first forms S and P, hands P over through LDS
+// and, in window_grad_kv, adds up dV = P^T.dY; the second forms dY.V^T, takes P and adds up dK = dS^T.Q or dQ = dS.K.  Each
+// then keeps one operand and one accumulator in registers instead of two.  (One wavefront for everything took 512 registers,
+// ran alone on its SIMD and left the matrix pipe idle for half of the time: dK and dV at 32 x 8192 x 128 under a window of
+// 1024 in 3.3 ms.)  One barrier a step, between the products: behind it P is there, the next step's tiles have landed, and
+// those of the step before are free, so three buffers.
+//
 #include "token_mixer.h"
 #include "attention_window.h"
 #include "runtime_internal.h"
@@ -24,298 +28,459 @@ constexpr int GK = 128;    // keys per workgroup of window_grad_kv
 struct WindowGrad {
     WindowParams w;          // Y, Lse: what the forward pass left
     const float* dY; float* dQ; float* dK; float* dV;
-    float* D;                // [N, head, QL]
+    float* stats;            // [2][N, head, QL]: minus lse in units of log2, minus D -- what the products start from
+    long long rows;          // N * head * QL
     float scale;
-    int ktiles, sink_tiles, sink_parts, parts;
-    float* sink_sums; float* sums;     // [N, kv_head, keys][parts][dk4 + dv4]
+    int ktiles, workers;     // key tiles of a key / value head; workgroups of window_grad_kv
+    int per_step;            // queries of a step of window_grad_kv
+    long long* before;       // [N * ktiles + 1]: the steps of all key tiles before this one, of one key / value head
+    float* pieces;           // [2 * workers][128][dk4 + dv4]
 };
 
-// ---------------------------------------------------------------- D[i] = <dY[i], Y[i]>
-__global__ __launch_bounds__(NTHREADS) void window_delta(const WindowGrad p) {
+// ---------------------------------------------------------------- what the products start from, and the work to deal
+// the queries that see a key of tile `tile`: [lo, hi)
+struct WindowQueries { int lo, hi; };
+__device__ __forceinline__ WindowQueries window_queries(const WindowParams& p, int tile, WindowLens len) {
+    const int k0 = tile * GK, k1 = min(k0 + GK, len.vl), off = len.vl - len.ql;
+    WindowQueries x;
+    x.lo = max(k0 - off, 0);
+    x.hi = k0 < k1 ? (k0 < p.sinks ? len.ql : min(len.ql, k1 - 1 + p.window - off)) : 0;
+    return x;
+}
+// steps of `per` queries of one query head
+__device__ __forceinline__ int window_steps(WindowQueries x, int per) { return (max(x.hi - x.lo, 0) + per - 1) / per; }
+
+__global__ __launch_bounds__(NTHREADS) void window_delta(const WindowGrad a) {
+    const WindowParams& p = a.w;
+    if (blockIdx.x == gridDim.x - 1) {       // the running sum of the tiles' steps
+        __shared__ long long sum[NTHREADS];
+        const int t = threadIdx.x, group = p.head / p.kv_head;
+        const long long tiles = (long long)p.N * a.ktiles;
+        long long base = 0;
+        for (long long x0 = 0; x0 < tiles; x0 += NTHREADS) {
+            const long long x = x0 + t;
+            long long own = 0;
+            if (x < tiles) {
+                const int n = (int)(x / a.ktiles);
+                const WindowLens len = {p.QLens ? min(max(p.QLens[n], 0), p.QL) : p.QL, p.VLens ? min(max(p.VLens[n], 0), p.VL) : p.VL};
+                own = (long long)window_steps(window_queries(p, (int)(x - (long long)n * a.ktiles), len), a.per_step) * group;
+            }
+            sum[t] = own;
+            __syncthreads();
+            for (int d = 1; d < NTHREADS; d <<= 1) {
+                const long long add = t >= d ? sum[t - d] : 0;
+                __syncthreads();
+                sum[t] += add;
+                __syncthreads();
+            }
+            if (x < tiles) a.before[x] = base + sum[t] - own;
+            base += sum[NTHREADS - 1];
+            __syncthreads();
+        }
+        if (t == 0) a.before[tiles] = base;
+        return;
+    }
     const long long row = (long long)blockIdx.x * (NTHREADS / 32) + (threadIdx.x >> 5);
-    if (row >= (long long)p.w.N * p.w.head * p.w.QL) return;
-    const long long nh = row / p.w.QL;
-    const int n = (int)(nh / p.w.head), hd = (int)(nh - (long long)n * p.w.head), i = (int)(row - nh * p.w.QL);
+    if (row >= a.rows) return;
+    const long long nh = row / p.QL;
+    const int n = (int)(nh / p.head), hd = (int)(nh - (long long)n * p.head), i = (int)(row - nh * p.QL);
     const int d = 4 * (threadIdx.x & 31);
     float sum = 0.0f;
-    const int ql = p.w.QLens ? min(p.w.QLens[n], p.w.QL) : p.w.QL;
-    if (i < ql && d < p.w.dv4) {
-        const size_t at = n * p.w.y.n + hd * p.w.y.h + (size_t)i * p.w.y.l + d;
-        const v4f a = *(const v4f*)(p.dY + at), b = *(const v4f*)(p.w.Y + at);
-        sum = (a.x * b.x + a.y * b.y) + (a.z * b.z + a.w * b.w);
+    const int ql = p.QLens ? min(p.QLens[n], p.QL) : p.QL;
+    if (i < ql && d < p.dv4) {
+        const size_t at = n * p.y.n + hd * p.y.h + (size_t)i * p.y.l + d;
+        const v4f g = *(const v4f*)(a.dY + at), y = *(const v4f*)(p.Y + at);
+        sum = (g.x * y.x + g.y * y.y) + (g.z * y.z + g.w * y.w);
     }
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor(sum, x, 64);
-    if ((threadIdx.x & 31) == 0) p.D[row] = sum;
+    if ((threadIdx.x & 31) == 0) {
+        a.stats[row] = i < ql ? -p.Lse[row] * MIX_LOG2E : 0.0f;
+        a.stats[a.rows + row] = -sum;
+    }
+}
+
+constexpr int GT = 512;
+
+// P handed from one wavefront to the other: 16 bytes per lane and result group
+__device__ __forceinline__ void give(float* at, const v16f& e) {
+#pragma unroll
+    for (int q = 0; q < 4; q++) *(v4f*)(at + q * 256) = (v4f){e[4 * q], e[4 * q + 1], e[4 * q + 2], e[4 * q + 3]};
+}
+__device__ __forceinline__ void take(const float* at, v16f& e) {
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const v4f P = *(const v4f*)(at + q * 256);
+#pragma unroll
+        for (int w = 0; w < 4; w++) e[4 * q + w] *= P[w];
+    }
 }
 
 // ---------------------------------------------------------------- dQ
-template <int DB, int DC>
-__global__ __launch_bounds__(NTHREADS, 2) void window_grad_q(const WindowGrad a) {
-    constexpr int DW = DB * 32, NG = DC * 4;
+template <int DB, int DC, int KB>
+__global__ __launch_bounds__(GT, 2) void window_grad_q(const WindowGrad a) {
+    constexpr int DW = DB * 32, NG = DC * 4, AK = KB * 32, TILE = AK * DW;
     const WindowParams& p = a.w;
-    __shared__ __attribute__((aligned(16))) float Ks[2][32 * DW];
-    __shared__ __attribute__((aligned(16))) float Vs[2][32 * DW];
+    __shared__ __attribute__((aligned(16))) float Ks[3 * TILE];
+    __shared__ __attribute__((aligned(16))) float Vs[3 * TILE];
+    __shared__ __attribute__((aligned(16))) float Ps[2][4][KB * 64 * 16];  // [step][32 queries][keys / 8][lane]
     const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
+    const int block = wave & 3;
+    const bool second = wave >= 4;
     const WindowJob job = window_job(p, blockIdx.x);
     const WindowLens len = window_lens(p, job.n);
-    const int q0 = job.qt * GQ, i = q0 + wave * 32 + r;
+    const int q0 = job.qt * GQ, i = q0 + block * 32 + r;
     const size_t stat = ((size_t)job.n * p.head + job.hd) * p.QL + min(i, p.QL - 1);
     const int qn = min(q0 + GQ, len.ql), off = len.vl - len.ql;
     const WindowRange range = window_range(p, q0 + off, qn - 1 + off, q0 < qn, len.vl);
-    const int nsink = (range.sink_end + 31) / 32, steps = nsink + (max(range.hi - range.low, 0) + 31) / 32;
+    const int nsink = (range.sink_end + AK - 1) / AK, steps = nsink + (max(range.hi - range.low, 0) + AK - 1) / AK;
     const bool live = i < len.ql;
     const int pos = live ? i + off : -1;
-    const int w0 = q0 + wave * 32 + off, w1 = min(q0 + wave * 32 + 32, len.ql) - 1 + off;
+    const int w0 = q0 + block * 32 + off, w1 = min(q0 + block * 32 + 32, len.ql) - 1 + off;
 
-    v4f qf[NG], gf[NG];
-    mix_load_cols<NG>(qf, p.Q + job.n * p.q.n + job.hd * p.q.h + (size_t)min(i, p.QL - 1) * p.q.l, live, p.dk4, h);
-    mix_load_cols<NG>(gf, a.dY + job.n * p.y.n + job.hd * p.y.h + (size_t)min(i, p.QL - 1) * p.y.l, live, p.dv4, h);
+    v4f own[NG];                                                        // Q (times scale, in units of log2) or dY
+    if (second) {
+        mix_load_cols<NG>(own, a.dY + job.n * p.y.n + job.hd * p.y.h + (size_t)min(i, p.QL - 1) * p.y.l, live, p.dv4, h);
+    } else {
+        mix_load_cols<NG>(own, p.Q + job.n * p.q.n + job.hd * p.q.h + (size_t)min(i, p.QL - 1) * p.q.l, live, p.dk4, h);
 #pragma unroll
-    for (int g = 0; g < NG; g++) qf[g] *= p.c;
-    const float lse = live ? p.Lse[stat] * MIX_LOG2E : 0.0f, D = live ? a.D[stat] : 0.0f;
-    const v16f from = (v16f)(-lse);                         // where the score products start: P = exp2 of the result
+        for (int g = 0; g < NG; g++) own[g] *= p.c;
+    }
+    const v16f from = (v16f)(live ? a.stats[(second ? a.rows : 0) + stat] : 0.0f);
 
     const float* Kb = p.K + job.n * p.k.n + job.kvh * p.k.h;
     const float* Vb = p.V + job.n * p.v.n + job.kvh * p.v.h;
-    MixTile<DW, 32, true> kt, vt;
+    MixTile<DW, AK, true, GT> kt, vt;
     MixColumns<DW, true> cols;
     cols.init(r, h);
     kt.init(t, p.k.l, p.dk4);
     vt.init(t, p.v.l, p.dv4);
-    auto key_of = [&](int s) { return s < nsink ? s * 32 : range.low + (s - nsink) * 32; };
-    const unsigned klds = mix_lds(Ks[0]) + wave * 1024, vlds = mix_lds(Vs[0]) + wave * 1024;
+    const unsigned klds = mix_lds(Ks) + wave * 1024, vlds = mix_lds(Vs) + wave * 1024;
+    const bool mover = wave * 64 < AK * (DW / 4);                       // a small tile does not need all the threads
+    const float* const X = second ? Vs : Ks;
+    auto key_of = [&](int s) { return s < nsink ? s * AK : range.low + (s - nsink) * AK; };
     auto fetch = [&](int s, int into) {
         const int key0 = key_of(s), left = (s < nsink ? range.sink_end : range.hi) - key0;
-        kt.fetch(Kb + (size_t)key0 * p.k.l, left, p.k.l, klds + into * (32 * DW * 4));
-        vt.fetch(Vb + (size_t)key0 * p.v.l, left, p.v.l, vlds + into * (32 * DW * 4));
+        if (mover) {
+            kt.fetch(Kb + (size_t)key0 * p.k.l, left, p.k.l, klds + into * (TILE * 4));
+            vt.fetch(Vb + (size_t)key0 * p.v.l, left, p.v.l, vlds + into * (TILE * 4));
+        }
     };
     v16f o[DC];
 #pragma unroll
     for (int b = 0; b < DC; b++) o[b] = (v16f)(0.0f);
     if (steps > 0) fetch(0, 0);
     mix_wait();
+    if (steps > 1) fetch(1, 1);
     __syncthreads();
-    auto step = [&](auto bufc, int s) {
-        constexpr int buf = decltype(bufc)::value;
-        if (s + 1 < steps) fetch(s + 1, buf ^ 1);
-        __builtin_amdgcn_sched_barrier(0);
-        const int key0 = key_of(s), limit = s < nsink ? range.sink_end : range.hi, end = min(key0 + 32, limit);
+    int buf = 0;
+    for (int s = 0; s < steps; s++) {
+        const int key0 = key_of(s), limit = s < nsink ? range.sink_end : range.hi, end = min(key0 + AK, limit);
         const bool sees = w0 <= w1 && (s < nsink || (key0 <= w1 && (end - 1 > w0 - p.window || key0 < p.sinks)));
+        float* exchange = &Ps[s & 1][block][4 * lane];
+        v16f e[KB];
         if (sees) {
-            v16f sc = from, dp = (v16f)(0.0f);
-            mix_rows_product<DW, NG>(sc, Ks[buf], qf, r, h);
-            mix_rows_product<DW, NG>(dp, Vs[buf], gf, r, h);
 #pragma unroll
-            for (int v = 0; v < 16; v++) sc[v] = __builtin_amdgcn_exp2f(sc[v]) * (dp[v] - D);
-            // keys behind a query (or behind the last key), and before its window: tested only where some query has them
-            if (key0 + 31 > w0 || key0 + 32 > limit || q0 + wave * 32 + 32 > len.ql) {
+            for (int kb = 0; kb < KB; kb++) {
+                e[kb] = from;
+                mix_rows_product<DW, NG>(e[kb], X + buf * TILE + kb * 32 * DW, own, r, h);
+            }
+            if (!second) {
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) e[kb][v] = __builtin_amdgcn_exp2f(e[kb][v]);
+            }
+            // keys behind a query (or behind the last key), and before its window: tested only where some query has them.
+            // Both factors are cleared: dY.V^T may be anything where nothing is seen.
+            if (key0 + AK - 1 > w0 || key0 + AK > limit || q0 + block * 32 + 32 > len.ql) {
                 const int top = min(pos, limit - 1) - key0 - 4 * h;
 #pragma unroll
-                for (int v = 0; v < 16; v++)
-                    if (mix_row(v, 0) > top) sc[v] = 0.0f;
+                for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++)
+                        if (32 * kb + mix_row(v, 0) > top) e[kb][v] = 0.0f;
             }
             if (s >= nsink && key0 <= w1 - p.window) {
                 const int low = pos - p.window - key0 - 4 * h, sink = p.sinks - key0 - 4 * h;
 #pragma unroll
-                for (int v = 0; v < 16; v++)
-                    if (mix_row(v, 0) <= low && mix_row(v, 0) >= sink) sc[v] = 0.0f;
+                for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++)
+                        if (32 * kb + mix_row(v, 0) <= low && 32 * kb + mix_row(v, 0) >= sink) e[kb][v] = 0.0f;
             }
-            mix_columns_product<DW, DC, true>(o, Ks[buf], sc, cols, r, h);
+            if (!second) {
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++) give(exchange + kb * 1024, e[kb]);
+            }
         }
         mix_wait();
         __syncthreads();
-    };
-    for (int s = 0; s < steps; s += 2) {
-        step(std::integral_constant<int, 0>{}, s);
-        if (s + 1 < steps) step(std::integral_constant<int, 1>{}, s + 1);
+        const int b1 = buf == 2 ? 0 : buf + 1, b2 = b1 == 2 ? 0 : b1 + 1;
+        if (s + 2 < steps) fetch(s + 2, b2);
+        __builtin_amdgcn_sched_barrier(0);
+        if (sees && second) {
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) {
+                take(exchange + kb * 1024, e[kb]);
+                mix_columns_product<DW, DC, true>(o, Ks + buf * TILE + kb * 32 * DW, e[kb], cols, r, h);
+            }
+        }
+        buf = b1;
     }
-    if (i < p.QL) mix_store_row<DC>(a.dQ + job.n * p.q.n + job.hd * p.q.h + (size_t)i * p.q.l, o, a.scale, p.dk4, h);
+    if (second && i < p.QL) mix_store_row<DC>(a.dQ + job.n * p.q.n + job.hd * p.q.h + (size_t)i * p.q.l, o, a.scale, p.dk4, h);
 }
 
 // ---------------------------------------------------------------- dK, dV
-template <int DB, int DC>
-__global__ __launch_bounds__(NTHREADS, DB > 2 ? 1 : 2) void window_grad_kv(const WindowGrad a) {
-    constexpr int DW = DB * 32, NG = DC * 4;
+// A key tile is seen by window + 128 queries of every head of the group, one with sinks by all behind it, the last ones
+// under no window by few: the tiles differ by whatever the sequence is long.  So the steps of all tiles are counted through
+// (before) and dealt to the workgroups in equal runs.  Where a run begins or ends inside a tile the workgroup leaves its sums
+// as a piece and window_grad_join adds the tile's pieces in order.
+struct GradDeal { long long total; long long workers; };
+__device__ __forceinline__ GradDeal grad_deal(const WindowGrad& a) {
+    GradDeal x;
+    x.total = a.before[(long long)a.w.N * a.ktiles] * a.w.kv_head;
+    x.workers = min((long long)a.workers, max(x.total / 4, 1LL));     // at least 4 steps each
+    return x;
+}
+// a tile in the count: its steps for one key / value head, where the heads' steps begin
+struct GradTile { long long at; int steps; };
+__device__ __forceinline__ GradTile grad_tile(const WindowGrad& a, long long tile) {
+    GradTile x;
+    x.at = a.before[tile] * a.w.kv_head;
+    x.steps = (int)(a.before[tile + 1] - a.before[tile]);
+    return x;
+}
+// the tile (over all sequences) that step `pos` of the count belongs to: the last one that begins at or before it
+__device__ __forceinline__ long long grad_find(const WindowGrad& a, long long pos) {
+    long long lo = 0, hi = (long long)a.w.N * a.ktiles;
+    while (hi - lo > 1) {
+        const long long mid = (lo + hi) >> 1;
+        if (a.before[mid] * a.w.kv_head <= pos) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+// where worker w's run begins; a boundary up to two steps away from a tile's moves there, which saves two pieces
+__device__ __forceinline__ long long grad_begin(const WindowGrad& a, const GradDeal& d, long long w) {
+    if (w <= 0) return 0;
+    if (w >= d.workers) return d.total;
+    const long long pos = d.total / d.workers * w + (d.total % d.workers) * w / d.workers;
+    const GradTile tile = grad_tile(a, grad_find(a, pos));
+    if (tile.steps == 0) return pos;
+    const int in = (int)((pos - tile.at) % tile.steps), snap = (int)min(2LL, d.total / d.workers / 4);
+    return in <= snap ? pos - in : tile.steps - in <= snap ? pos + tile.steps - in : pos;
+}
+// the worker whose run holds step pos
+__device__ __forceinline__ long long grad_worker(const WindowGrad& a, const GradDeal& d, long long pos) {
+    long long w = min(pos / max(d.total / d.workers, 1LL), d.workers - 1);
+    while (w + 1 < d.workers && grad_begin(a, d, w + 1) <= pos) w++;
+    while (w > 0 && grad_begin(a, d, w) > pos) w--;
+    return w;
+}
+
+template <int DB, int DC, int QB>
+__global__ __launch_bounds__(GT, 2) void window_grad_kv(const WindowGrad a) {
+    constexpr int DW = DB * 32, NG = DC * 4, AQ = QB * 32, TILE = AQ * DW;
     const WindowParams& p = a.w;
-    __shared__ __attribute__((aligned(16))) float Qs[2][32 * DW];
-    __shared__ __attribute__((aligned(16))) float Gs[2][32 * DW];
-    __shared__ __attribute__((aligned(16))) float Ls[2][32], Ds[2][32];
+    __shared__ __attribute__((aligned(16))) float Qs[3 * TILE];
+    __shared__ __attribute__((aligned(16))) float Gs[3 * TILE];
+    __shared__ __attribute__((aligned(16))) float Ps[2][4][QB * 64 * 16];  // [step][32 keys][queries / 8][lane]
     const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
+    const int block = wave & 3;
+    const bool second = wave >= 4;
+    const int group = p.head / p.kv_head;
 
-    // key tiles in order (the first are seen by the most queries), the sinks' in sink_parts each
-    const int nkv = p.N * p.kv_head, group = p.head / p.kv_head;
-    const int x = mix_uniform(blockIdx.x / nkv), kv = blockIdx.x - x * nkv;
-    const bool sink_tile = x < a.sink_tiles * a.sink_parts;
-    const int parts = sink_tile ? a.sink_parts : a.parts;
-    const int y = sink_tile ? x : x - a.sink_tiles * a.sink_parts;
-    const int tile = mix_uniform(y / parts), part = y - tile * parts;
-    const int n = mix_uniform(kv / p.kv_head), kvh = kv - n * p.kv_head;
-    const int k0 = (sink_tile ? tile : a.sink_tiles + tile) * GK;
-    const WindowLens len = window_lens(p, n);
-    const int off = len.vl - len.ql;
-    const int key = k0 + wave * 32 + r, k1 = min(k0 + GK, len.vl);
-    const bool live = key < len.vl;
-    const int u0 = k0 + wave * 32, u1 = min(u0 + 32, len.vl) - 1;      // the wavefront's keys
+    const GradDeal deal = grad_deal(a);
+    auto uniform = [](long long x) { return (long long)(((unsigned long long)(unsigned)mix_uniform((int)(x >> 32)) << 32) | (unsigned)mix_uniform((int)x)); };
+    if (blockIdx.x >= deal.workers) return;
+    long long pos = uniform(grad_begin(a, deal, blockIdx.x));
+    const long long stop = uniform(grad_begin(a, deal, blockIdx.x + 1));
 
-    // the queries that see a key of the tile: [lo, hi)
-    const int lo = max(k0 - off, 0);
-    const int hi = k0 < k1 ? (k0 < p.sinks ? len.ql : min(len.ql, k1 - 1 + p.window - off)) : 0;
-    const int per_head = (max(hi - lo, 0) + 31) / 32, total = per_head * group;
-    const int first = mix_uniform((int)((long long)total * part / parts)), last = mix_uniform((int)((long long)total * (part + 1) / parts));
-
-    v4f kf[NG], vf[NG];
-    mix_load_cols<NG>(kf, p.K + n * p.k.n + kvh * p.k.h + (size_t)min(key, p.VL - 1) * p.k.l, live, p.dk4, h);
-    mix_load_cols<NG>(vf, p.V + n * p.v.n + kvh * p.v.h + (size_t)min(key, p.VL - 1) * p.v.l, live, p.dv4, h);
-#pragma unroll
-    for (int g = 0; g < NG; g++) kf[g] *= p.c;
-
-    MixTile<DW, 32, true> qt, gt;
+    MixTile<DW, AQ, true, GT> qt, gt;
     MixColumns<DW, true> cols;
     cols.init(r, h);
     qt.init(t, p.q.l, p.dk4);
     gt.init(t, p.y.l, p.dv4);
-    float stat_reg = 0.0f;
-    const unsigned qlds = mix_lds(Qs[0]) + wave * 1024, glds = mix_lds(Gs[0]) + wave * 1024;
-    // the step after (head g0 of the group, query tile i0) is (g0, i0 + 32) or the next head's first
-    auto fetch = [&](int g, int i0, int into) {
-        const int hd = kvh * group + g;
-        qt.fetch(p.Q + n * p.q.n + hd * p.q.h + (size_t)i0 * p.q.l, hi - i0, p.q.l, qlds + into * (32 * DW * 4));
-        gt.fetch(a.dY + n * p.y.n + hd * p.y.h + (size_t)i0 * p.y.l, hi - i0, p.y.l, glds + into * (32 * DW * 4));
-        const size_t row = ((size_t)n * p.head + hd) * p.QL + i0 + (t & 31);
-        if (t < 64) stat_reg = i0 + (t & 31) < hi ? (t < 32 ? p.Lse[row] * MIX_LOG2E : a.D[row]) : 0.0f;
-    };
-    auto store = [&](int into) {
-        if (t < 32) Ls[into][t] = stat_reg;
-        else if (t < 64) Ds[into][t - 32] = stat_reg;
-    };
-    v16f dk[DC], dv[DC];
+    const unsigned qlds = mix_lds(Qs) + wave * 1024, glds = mix_lds(Gs) + wave * 1024;
+    const bool mover = wave * 64 < AQ * (DW / 4);                       // a small tile does not need all the threads
+    const float* const X = second ? Gs : Qs;                            // the tile of the first product, of the second
+    const float* const Z = second ? Qs : Gs;
+    const float* const stats = a.stats + (second ? a.rows : 0);
+
+    long long at = pos < stop ? uniform(grad_find(a, pos)) : 0;         // the tile over all sequences
+    while (pos < stop) {
+        GradTile cur = grad_tile(a, at);
+        while (pos >= cur.at + (long long)cur.steps * p.kv_head) cur = grad_tile(a, ++at);     // also over tiles without steps
+        at = uniform(at);
+        const int all = mix_uniform(cur.steps), kvh = mix_uniform((int)((pos - cur.at) / cur.steps));
+        const int first = mix_uniform((int)(pos - cur.at - (long long)kvh * all));
+        const int last = mix_uniform((int)min((long long)all, first + (stop - pos)));
+        pos += last - first;
+        const int n = mix_uniform((int)(at / a.ktiles)), tile = mix_uniform((int)(at - (long long)n * a.ktiles));
+        const WindowLens len = window_lens(p, n);
+        const WindowQueries qs = window_queries(p, tile, len);
+        const int lo = qs.lo, hi = qs.hi, per_head = window_steps(qs, AQ), off = len.vl - len.ql;
+        const int u0 = tile * GK + block * 32, u1 = min(u0 + 32, len.vl) - 1;      // the wavefront's keys
+        const int key = u0 + r;
+        const bool live = key < len.vl;
+
+        v4f own[NG];                                                    // K (times scale, in units of log2) or V
+        if (second) {
+            mix_load_cols<NG>(own, p.V + n * p.v.n + kvh * p.v.h + (size_t)min(key, p.VL - 1) * p.v.l, live, p.dv4, h);
+        } else {
+            mix_load_cols<NG>(own, p.K + n * p.k.n + kvh * p.k.h + (size_t)min(key, p.VL - 1) * p.k.l, live, p.dk4, h);
 #pragma unroll
-    for (int b = 0; b < DC; b++) { dk[b] = (v16f)(0.0f); dv[b] = (v16f)(0.0f); }
-    int g = 0, i0 = lo;
-    if (first < last) {
-        g = mix_uniform(first / per_head);
-        i0 = lo + (first - g * per_head) * 32;
-        fetch(g, i0, 0);
-    }
-    mix_wait();
-    store(0);
-    __syncthreads();
-    auto step = [&](auto bufc, int s) {
-        constexpr int buf = decltype(bufc)::value;
-        const bool more = s + 1 < last;
-        const bool turn = i0 + 32 >= hi;
-        const int next_g = turn ? g + 1 : g, next_i0 = turn ? lo : i0 + 32;
-        if (more) fetch(next_g, next_i0, buf ^ 1);
-        __builtin_amdgcn_sched_barrier(0);
-        const int p0 = i0 + off, p1 = min(i0 + 32, hi) - 1 + off;      // the step's positions
-        const bool sees = u0 <= u1 && p1 >= u0 && (p0 < u1 + p.window || u0 < p.sinks);
-        if (sees) {
-            v16f sc = (v16f)(0.0f), dp = (v16f)(0.0f);
-            mix_rows_product<DW, NG>(sc, Qs[buf], kf, r, h);
-            mix_rows_product<DW, NG>(dp, Gs[buf], vf, r, h);
+            for (int g = 0; g < NG; g++) own[g] *= p.c;
+        }
+        // the statistics of a step's queries, as the products' start: rows 8q + 4h .. +3 (zeros beyond the last of the head)
+        v16f start[QB];
+        auto begin = [&](int g, int i0) {
+            const float* row = stats + ((size_t)n * p.head + kvh * group + g) * p.QL + i0;
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)row, 0, min(p.QL - i0, AQ) * 4, RSRC_FLAGS);
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const v4f lse = *(const v4f*)&Ls[buf][8 * q + 4 * h], D = *(const v4f*)&Ds[buf][8 * q + 4 * h];
+            for (int q = 0; q < 4 * QB; q++) {
+                const v4f x = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rs, (8 * q + 4 * h) * 4, 0, 0));
 #pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    sc[4 * q + w] = __builtin_amdgcn_exp2f(sc[4 * q + w] - lse[w]);
-                    dp[4 * q + w] = dp[4 * q + w] - D[w];
+                for (int w = 0; w < 4; w++) start[q / 4][4 * (q % 4) + w] = x[w];
+            }
+        };
+        auto fetch = [&](int g, int i0, int into) {
+            const int hd = kvh * group + g;
+            if (mover) {
+                qt.fetch(p.Q + n * p.q.n + hd * p.q.h + (size_t)i0 * p.q.l, hi - i0, p.q.l, qlds + into * (TILE * 4));
+                gt.fetch(a.dY + n * p.y.n + hd * p.y.h + (size_t)i0 * p.y.l, hi - i0, p.y.l, glds + into * (TILE * 4));
+            }
+        };
+        v16f acc[DC];
+#pragma unroll
+        for (int b = 0; b < DC; b++) acc[b] = (v16f)(0.0f);
+
+        int g = mix_uniform(first / per_head), i0 = lo + (first - g * per_head) * AQ;   // the step's queries
+        auto next = [&](int& hd, int& i) {
+            i += AQ;
+            if (i >= hi) { i = lo; hd++; }
+        };
+        int fg = g, fi0 = i0, i0_next;                                  // the next to fetch; the next step's
+        fetch(fg, fi0, 0);
+        begin(g, i0);
+        next(fg, fi0);
+        mix_wait();
+        if (first + 1 < last) {
+            fetch(fg, fi0, 1);
+            next(fg, fi0);
+        }
+        __syncthreads();
+        int buf = 0;
+        for (int s = first; s < last; s++) {
+            const int p0 = i0 + off, p1 = min(i0 + AQ, hi) - 1 + off;  // the step's positions
+            const bool sees = u0 <= u1 && p1 >= u0 && (p0 < u1 + p.window || u0 < p.sinks);
+            float* exchange = &Ps[s & 1][block][4 * lane];
+            v16f e[QB];
+#pragma unroll
+            for (int qb = 0; qb < QB; qb++) e[qb] = start[qb];
+            next(g, i0_next = i0);
+            if (s + 1 < last) begin(g, i0_next);                       // there when this wavefront waits for its transfers
+            if (sees) {
+#pragma unroll
+                for (int qb = 0; qb < QB; qb++) mix_rows_product<DW, NG>(e[qb], X + buf * TILE + qb * 32 * DW, own, r, h);
+                if (!second) {
+#pragma unroll
+                    for (int qb = 0; qb < QB; qb++)
+#pragma unroll
+                        for (int v = 0; v < 16; v++) e[qb][v] = __builtin_amdgcn_exp2f(e[qb][v]);
+                }
+                // queries before a key, those whose window has passed it, and rows behind the last: tested only where there are
+                // any.  Both factors are cleared: dY.V^T may be anything where nothing is seen.
+                if (p0 < u1 || i0 + AQ > hi || u0 + 32 > len.vl) {
+                    const int low = (live ? key : 0x3fffffff) - p0 - 4 * h, top = hi - 1 - i0 - 4 * h;
+#pragma unroll
+                    for (int qb = 0; qb < QB; qb++)
+#pragma unroll
+                        for (int v = 0; v < 16; v++)
+                            if (32 * qb + mix_row(v, 0) < low || 32 * qb + mix_row(v, 0) > top) e[qb][v] = 0.0f;
+                }
+                if (p1 >= u0 + p.window) {
+                    const int top = key < p.sinks ? 0x3fffffff : key + p.window - 1 - p0 - 4 * h;
+#pragma unroll
+                    for (int qb = 0; qb < QB; qb++)
+#pragma unroll
+                        for (int v = 0; v < 16; v++)
+                            if (32 * qb + mix_row(v, 0) > top) e[qb][v] = 0.0f;
+                }
+                if (!second) {
+#pragma unroll
+                    for (int qb = 0; qb < QB; qb++) give(exchange + qb * 1024, e[qb]);
                 }
             }
-            // queries before a key, those whose window has passed it, and rows behind the last: tested only where there are any.
-            // Both factors are cleared: dP may be anything where nothing is seen.
-            if (p0 < u1 || i0 + 32 > hi || u0 + 32 > len.vl) {
-                const int low = (live ? key : 0x3fffffff) - p0 - 4 * h, top = hi - 1 - i0 - 4 * h;
-#pragma unroll
-                for (int v = 0; v < 16; v++)
-                    if (mix_row(v, 0) < low || mix_row(v, 0) > top) sc[v] = dp[v] = 0.0f;
+            mix_wait();
+            __syncthreads();
+            const int b1 = buf == 2 ? 0 : buf + 1, b2 = b1 == 2 ? 0 : b1 + 1;
+            if (s + 2 < last) {
+                fetch(fg, fi0, b2);
+                next(fg, fi0);
             }
-            if (p1 >= u0 + p.window) {
-                const int top = key < p.sinks ? 0x3fffffff : key + p.window - 1 - p0 - 4 * h;
+            __builtin_amdgcn_sched_barrier(0);
+            if (sees) {
 #pragma unroll
-                for (int v = 0; v < 16; v++)
-                    if (mix_row(v, 0) > top) sc[v] = dp[v] = 0.0f;
+                for (int qb = 0; qb < QB; qb++) {
+                    if (second) take(exchange + qb * 1024, e[qb]);
+                    mix_columns_product<DW, DC, true>(acc, Z + buf * TILE + qb * 32 * DW, e[qb], cols, r, h);
+                }
             }
-#pragma unroll
-            for (int v = 0; v < 16; v++) dp[v] *= sc[v];
-            mix_columns_product<DW, DC, true>(dv, Gs[buf], sc, cols, r, h);
-            mix_columns_product<DW, DC, true>(dk, Qs[buf], dp, cols, r, h);
+            buf = b1;
+            i0 = i0_next;
         }
-        mix_wait();
-        if (more) store(buf ^ 1);
-        __syncthreads();
-        g = next_g;
-        i0 = next_i0;
-    };
-    for (int s = first; s < last; s += 2) {
-        step(std::integral_constant<int, 0>{}, s);
-        if (s + 1 < last) step(std::integral_constant<int, 1>{}, s + 1);
-    }
-    if (key >= p.VL) return;
-    if (parts == 1) {
-        mix_store_row<DC>(a.dK + n * p.k.n + kvh * p.k.h + (size_t)key * p.k.l, dk, a.scale, p.dk4, h);
-        mix_store_row<DC>(a.dV + n * p.v.n + kvh * p.v.h + (size_t)key * p.v.l, dv, 1.0f, p.dv4, h);
-    } else {
-        const int sink_rows = a.sink_tiles * GK;
-        const size_t row = sink_tile ? (size_t)kv * sink_rows + key : (size_t)kv * (p.VL - sink_rows) + key - sink_rows;
-        float* at = (sink_tile ? a.sink_sums : a.sums) + (row * parts + part) * (p.dk4 + p.dv4);
-        mix_store_row<DC>(at, dk, a.scale, p.dk4, h);
-        mix_store_row<DC>(at + p.dk4, dv, 1.0f, p.dv4, h);
+        float* out;
+        if (first == 0 && last == all) {
+            out = second ? a.dK + n * p.k.n + kvh * p.k.h + (size_t)key * p.k.l : a.dV + n * p.v.n + kvh * p.v.h + (size_t)key * p.v.l;
+        } else {        // a piece that does not begin the tile is this run's first, one that does its last
+            out = a.pieces + ((2 * (size_t)blockIdx.x + (first == 0)) * GK + block * 32 + r) * (p.dk4 + p.dv4) + (second ? 0 : p.dk4);
+        }
+        if (key < p.VL) mix_store_row<DC>(out, acc, second ? a.scale : 1.0f, second ? p.dk4 : p.dv4, h);
+        __syncthreads();                                                // the next piece's first tile lands in buffer 0
     }
 }
 
-// the parts of the keys [key0, key0 + rows) of every key / value head, in order
-__global__ __launch_bounds__(NTHREADS) void window_grad_join(const WindowGrad a, const float* sums, int key0, int rows, int stride, int parts) {
+// four workgroups per tile and key / value head: the tile's pieces in order; zeros where no query sees it
+__global__ __launch_bounds__(NTHREADS) void window_grad_join(const WindowGrad a) {
     const WindowParams& p = a.w;
+    const long long at = blockIdx.x / p.kv_head;
+    const int kvh = (int)(blockIdx.x - at * p.kv_head), n = (int)(at / a.ktiles), k0 = (int)(at - (long long)n * a.ktiles) * GK;
+    const GradDeal deal = grad_deal(a);
+    const GradTile tile = grad_tile(a, at);
+    const long long begin = tile.at + (long long)kvh * tile.steps, end = begin + tile.steps;
+    long long w0 = 0, w1 = 0;
+    if (tile.steps > 0) {
+        w0 = grad_worker(a, deal, begin);
+        w1 = grad_worker(a, deal, end - 1);
+        if (w0 == w1) return;                                           // written whole
+    }
     const int width = p.dk4 + p.dv4, per = width / 4;
-    const long long x = (long long)blockIdx.x * NTHREADS + threadIdx.x;
-    const long long row = x / per;
-    if (row >= (long long)p.N * p.kv_head * rows) return;
-    const int d = 4 * (int)(x - row * per);
-    const int kv = (int)(row / rows), key = (int)(row - (long long)kv * rows);
-    const float* at = sums + ((size_t)kv * stride + key) * parts * width + d;
-    v4f s = *(const v4f*)at;
-    for (int k = 1; k < parts; k++) s += *(const v4f*)(at + (size_t)k * width);
-    const int n = kv / p.kv_head, kvh = kv - n * p.kv_head;
-    if (d < p.dk4) *(v4f*)(a.dK + n * p.k.n + kvh * p.k.h + (size_t)(key0 + key) * p.k.l + d) = s;
-    else *(v4f*)(a.dV + n * p.v.n + kvh * p.v.h + (size_t)(key0 + key) * p.v.l + d - p.dk4) = s;
+#pragma unroll 4
+    for (int x = threadIdx.x; x < GK / 4 * per; x += NTHREADS) {
+        const int in = x / per, row = blockIdx.y * (GK / 4) + in, d = 4 * (x - in * per), key = k0 + row;
+        if (key >= p.VL) break;
+        v4f s = (v4f)(0.0f);
+        if (tile.steps > 0) {
+            s = *(const v4f*)(a.pieces + ((2 * (size_t)w0 + 1) * GK + row) * width + d);
+            for (long long w = w0 + 1; w <= w1; w++) s += *(const v4f*)(a.pieces + (2 * (size_t)w * GK + row) * width + d);
+        }
+        if (d < p.dk4) *(v4f*)(a.dK + n * p.k.n + kvh * p.k.h + (size_t)key * p.k.l + d) = s;
+        else *(v4f*)(a.dV + n * p.v.n + kvh * p.v.h + (size_t)key * p.v.l + d - p.dk4) = s;
+    }
 }
 
 // ---------------------------------------------------------------- host side
-struct WindowGradPlan { int ktiles, sink_tiles, sink_parts, parts; };
-
-WindowGradPlan window_grad_plan(int N, int head, int kv_head, int QL, int VL, int window, int sinks) {
-    WindowGradPlan x;
-    const long long group = head / kv_head;
-    x.ktiles = (VL + GK - 1) / GK;
-    const long long all = ((QL + 31LL) / 32) * group;          // steps of a tile that every query sees
-    const long long reach = window == 0 || window >= VL ? QL : (long long)window + GK < QL ? window + GK : QL;
-    const long long steps = ((reach + 31) / 32) * group;
-    const long long base = (long long)N * kv_head * x.ktiles;
-    long long parts = base >= 256 ? 1 : (512 + base - 1) / base;
-    if (parts > steps / 8) parts = steps / 8;
-    x.parts = (int)(parts < 1 ? 1 : parts > 16 ? 16 : parts);
-    x.sink_tiles = x.sink_parts = 0;
-    if (window != 0 && window < VL && sinks > 0) {
-        const long long least = steps / x.parts > 8 ? steps / x.parts : 8;
-        const long long sp = (all + least - 1) / least;
-        x.sink_parts = (int)(sp < 1 ? 1 : sp > 64 ? 64 : sp);
-        if (x.sink_parts > x.parts) x.sink_tiles = (int)(((long long)(sinks < VL ? sinks : VL) + GK - 1) / GK);
-        if (x.sink_tiles > x.ktiles) x.sink_tiles = x.ktiles;
-        if (x.sink_tiles == 0) x.sink_parts = 0;
-    }
-    return x;
-}
-
-// floats of D, of the sinks' tiles' parts, of the others'
-struct WindowGradBuffer { long long d, sink, rest; };
-WindowGradBuffer window_grad_buffer(const WindowGradPlan& x, int N, int head, int kv_head, int QL, int VL, int width) {
+// The caller's buffer, in floats: the statistics, the running sum (64-bit), the pieces.
+struct WindowGradBuffer { int ktiles, workers; long long stats, before, pieces; };
+WindowGradBuffer window_grad_buffer(int N, int head, int QL, int VL, int dk4, int dv4) {
     WindowGradBuffer b;
-    const long long sink_rows = (long long)x.sink_tiles * GK < VL ? (long long)x.sink_tiles * GK : VL;
-    b.d = ((long long)N * head * QL + 3) / 4 * 4;
-    b.sink = x.sink_tiles > 0 ? (long long)N * kv_head * x.sink_tiles * GK * x.sink_parts * width : 0;
-    b.rest = x.parts > 1 ? (long long)N * kv_head * (VL - sink_rows) * x.parts * width : 0;
+    b.ktiles = (VL + GK - 1) / GK;
+    b.workers = 256;                                                  // one for each compute unit: their LDS holds no two
+    b.stats = (2LL * N * head * QL + 3) / 4 * 4;
+    b.before = (((long long)N * b.ktiles + 1) * 2 + 3) / 4 * 4;
+    b.pieces = 2LL * b.workers * GK * (dk4 + dv4);
     return b;
 }
 
@@ -329,8 +494,8 @@ extern "C" {
 int64_t dragon_Cuda_attention_window_backward_bufsize(int32_t N, int32_t head, int32_t kv_head, int32_t QL, int32_t VL, int32_t dK4,
                                                       int32_t dV4, int32_t window, int32_t sinks) {
     if (!window_arguments_ok(N, head, kv_head, QL, VL, dK4, dV4, window, sinks)) return -1;
-    const WindowGradBuffer b = window_grad_buffer(window_grad_plan(N, head, kv_head, QL, VL, window, sinks), N, head, kv_head, QL, VL, dK4 + dV4);
-    return (b.d + b.sink + b.rest) * 4;
+    const WindowGradBuffer b = window_grad_buffer(N, head, QL, VL, dK4, dV4);
+    return (b.stats + b.before + b.pieces) * 4;
 }
 
 int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length, int64_t dQ, int64_t dK, int64_t dV, int64_t dY,
@@ -345,9 +510,8 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
         return hipErrorInvalidValue;
     if (!window_arguments_ok(N, head, kv_head, QL, VL, dK4, dV4, window, sinks) || !(scale - scale == 0.0f))
         return hipErrorInvalidValue;
-    const WindowGradPlan plan = window_grad_plan(N, head, kv_head, QL, VL, window, sinks);
-    const WindowGradBuffer b = window_grad_buffer(plan, N, head, kv_head, QL, VL, dK4 + dV4);
-    const long long need = (b.d + b.sink + b.rest) * 4;
+    const WindowGradBuffer b = window_grad_buffer(N, head, QL, VL, dK4, dV4);
+    const long long need = (b.stats + b.before + b.pieces) * 4;
     if (dBuf == 0 || !mix_aligned16(dBuf) || buf_size < need) return hipErrorInvalidValue;
 
     WindowGrad a;
@@ -364,48 +528,43 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
     p.qtiles = (QL + GQ - 1) / GQ; p.parts = 1; p.part = nullptr;
     a.dY = (const float*)(intptr_t)dDeltaY;
     a.dQ = (float*)(intptr_t)dDeltaQ; a.dK = (float*)(intptr_t)dDeltaK; a.dV = (float*)(intptr_t)dDeltaV;
-    a.D = (float*)(intptr_t)dBuf;
+    a.stats = (float*)(intptr_t)dBuf;
+    a.rows = (long long)N * head * QL;
     a.scale = scale;
-    a.ktiles = plan.ktiles; a.sink_tiles = plan.sink_tiles; a.sink_parts = plan.sink_parts; a.parts = plan.parts;
-    a.sink_sums = a.D + b.d; a.sums = a.sink_sums + b.sink;
+    a.ktiles = b.ktiles; a.workers = b.workers;
+    a.per_step = (dK4 > dV4 ? dK4 : dV4) > 64 ? 32 : 64;
+    a.before = (long long*)(a.stats + b.stats);
+    a.pieces = a.stats + b.stats + b.before;
     split_ledger_touch(a.dQ, (size_t)N * head * QL * dK4 * 4);
     split_ledger_touch(a.dK, (size_t)N * kv_head * VL * dK4 * 4);
     split_ledger_touch(a.dV, (size_t)N * kv_head * VL * dV4 * 4);
-    split_ledger_touch(a.D, (size_t)need);
+    split_ledger_touch(a.stats, (size_t)need);
 
     hipStream_t s = (hipStream_t)(intptr_t)streams[0];
     const dim3 block(NTHREADS);
-    const long long rows = (long long)N * head * QL;
-    hipLaunchKernelGGL(window_delta, dim3((unsigned)((rows + NTHREADS / 32 - 1) / (NTHREADS / 32))), block, 0, s, a);
+    hipLaunchKernelGGL(window_delta, dim3((unsigned)((a.rows + NTHREADS / 32 - 1) / (NTHREADS / 32) + 1)), block, 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const dim3 gq((unsigned)((long long)N * head * p.qtiles));
-    const dim3 gk((unsigned)((long long)N * kv_head * (plan.sink_tiles * plan.sink_parts + (plan.ktiles - plan.sink_tiles) * plan.parts)));
+    const dim3 gq((unsigned)((long long)N * head * p.qtiles)), gk((unsigned)b.workers);
     const int dmax = dK4 > dV4 ? dK4 : dV4;
-#define GRAD_CASE(DB_, DC_)                                                           \
+#define GRAD_CASE(DB_, DC_, B_)                                                        \
     do {                                                                              \
-        hipLaunchKernelGGL((window_grad_kv<DB_, DC_>), gk, block, 0, s, a);           \
+        hipLaunchKernelGGL((window_grad_kv<DB_, DC_, B_>), gk, dim3(GT), 0, s, a);        \
         e = hipGetLastError();                                                        \
         if (e != hipSuccess) return e;                                                \
-        hipLaunchKernelGGL((window_grad_q<DB_, DC_>), gq, block, 0, s, a);            \
+        hipLaunchKernelGGL((window_grad_q<DB_, DC_, B_>), gq, dim3(GT), 0, s, a);         \
         e = hipGetLastError();                                                        \
         if (e != hipSuccess) return e;                                                \
     } while (0)
     switch ((dmax + 31) / 32) {
-        case 1: GRAD_CASE(1, 1); break;
-        case 2: GRAD_CASE(2, 2); break;
-        case 3: GRAD_CASE(4, 3); break;
-        default: GRAD_CASE(4, 4); break;
+        case 1: GRAD_CASE(1, 1, 2); break;
+        case 2: GRAD_CASE(2, 2, 2); break;
+        case 3: GRAD_CASE(4, 3, 1); break;
+        default: GRAD_CASE(4, 4, 1); break;
     }
 #undef GRAD_CASE
-    const int sink_rows = plan.sink_tiles * GK < VL ? plan.sink_tiles * GK : VL;
-    auto join = [&](const float* sums, int key0, int n_rows, int stride, int parts) {
-        const long long items = (long long)N * kv_head * n_rows * ((dK4 + dV4) / 4);
-        hipLaunchKernelGGL(window_grad_join, dim3((unsigned)((items + NTHREADS - 1) / NTHREADS)), block, 0, s, a, sums, key0, n_rows, stride, parts);
-        return hipGetLastError();
-    };
-    if (plan.sink_tiles > 0) e = join(a.sink_sums, 0, sink_rows, plan.sink_tiles * GK, plan.sink_parts);
-    if (e == hipSuccess && plan.parts > 1 && VL > sink_rows) e = join(a.sums, sink_rows, VL - sink_rows, VL - sink_rows, plan.parts);
+    hipLaunchKernelGGL(window_grad_join, dim3((unsigned)((long long)N * b.ktiles * kv_head), 4), block, 0, s, a);
+    e = hipGetLastError();
     return e;
 }
 

@@ -37,14 +37,14 @@ __device__ __forceinline__ unsigned mix_lds(const float* lds) {
 // this wavefront's transfers have landed
 __device__ __forceinline__ void mix_wait() { __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); }
 
-// One [ROWS][DW] tile from memory straight into LDS by the 256 threads of a workgroup: no staging registers, no vector
+// One [ROWS][DW] tile from memory straight into LDS by THREADS threads of a workgroup (whole wavefronts): no staging registers, no vector
 // instructions (which the matrix pipe would wait for).  The hardware puts lane l's 16 bytes at the wave's base + 16 * l, so
 // the swizzle moves to the global side: the lane at slot c of row r fetches chunk c ^ swizzle(r).  A lane's byte offset
 // never changes; the tile's first row goes into the descriptor's base and the rows that exist into its size, so rows beyond
 // them and chunks beyond the row's d4 floats arrive as zeros.  Everything but the offsets has to be uniform.
-template <int DW, int ROWS, bool SWIZZLE>
+template <int DW, int ROWS, bool SWIZZLE, int THREADS = NTHREADS>
 struct MixTile {
-    static constexpr int CPR = DW / 4, RPP = NTHREADS / CPR, PASSES = ROWS / RPP;
+    static constexpr int CPR = DW / 4, RPP = THREADS / CPR < ROWS ? THREADS / CPR : ROWS, PASSES = ROWS / RPP;
     static_assert(PASSES * RPP == ROWS && PASSES >= 1, "the tile divides over the workgroup");
     int off[PASSES];
     __device__ __forceinline__ void init(int t, int pitch, int d4) {
@@ -65,7 +65,7 @@ struct MixTile {
         const unsigned to = (unsigned)mix_uniform((int)lds);
         static_for<PASSES>([&](auto sc) {
             constexpr int s = decltype(sc)::value;
-            dma_f4_lean<s * NTHREADS * 16>(rsrc, to, off[s]);
+            dma_f4_lean<s * THREADS * 16>(rsrc, to, off[s]);
         });
     }
 };
@@ -73,6 +73,7 @@ struct MixTile {
 // The order in which a product's LDS reads and matrix instructions are issued: READS reads first, then always one read behind
 // MFMAS matrix instructions.  Left alone the compiler reads an operand just before it is needed and the matrix pipe waits
 // for LDS between any two uses.
+// (The barriers around a product keep other reads out of the count.)
 template <int READS, int TOTAL, int MFMAS>
 __device__ __forceinline__ void mix_order() {
     __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
@@ -81,16 +82,21 @@ __device__ __forceinline__ void mix_order() {
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     });
     __builtin_amdgcn_sched_group_barrier(0x8, READS * MFMAS, 0);
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // result[row of the tile][column] += tile . cols^T over the head dimension: cols[g] holds d = 8g + 4h .. +3 of the lane's
 // column; the tile is swizzled
 template <int DW, int NG>
 __device__ __forceinline__ void mix_rows_product(v16f& s, const float* tile, const v4f (&cols)[NG], int r, int h) {
-    const float* row = tile + r * DW;
+    // Chunk 2g + h of row r lies at (2g + h) ^ swizzle: the lane's place of chunk h, with 2g exchanged into its low four bits
+    // (a row begins at a multiple of 2^(number of its chunks) of them, so nothing else is touched).
+    const unsigned at = mix_lds(tile) + r * (DW * 4) + 16 * (h ^ kin_swizzle<DW>(r));
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int g = 0; g < NG; g++) {
-        const v4f a = *(const v4f*)(row + 4 * ((2 * g + h) ^ kin_swizzle<DW>(r)));
+        typedef const __attribute__((address_space(3))) v4f* lds_v4f;
+        const v4f a = *(lds_v4f)((at ^ (32 * (g & 7))) + 256 * (g >> 3));
         s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, cols[g].x, s, 0, 0, 0);
         s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, cols[g].y, s, 0, 0, 0);
         s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, cols[g].z, s, 0, 0, 0);
@@ -122,6 +128,7 @@ struct MixColumns {
 // out^T[d][column] += sum over the tile's rows of tile[row][d] * p[row][column]
 template <int DW, int DC, bool SWIZZLE>
 __device__ __forceinline__ void mix_columns_product(v16f (&o)[DC], const float* tile, const v16f& p, const MixColumns<DW, SWIZZLE>& cols, int r, int h) {
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int v = 0; v < 16; v++) {
 #pragma unroll
