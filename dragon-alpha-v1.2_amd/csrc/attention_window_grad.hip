@@ -32,7 +32,7 @@ struct WindowGrad {
     long long rows;          // N * head * QL
     float scale;
     int ktiles, workers;     // key tiles of a key / value head; workgroups of window_grad_kv
-    int per_step;            // queries of a step of window_grad_kv
+    int snap;                // steps that a cut through a tile costs (two beginnings and ends, a piece written and read)
     long long* before;       // [N * ktiles + 1]: the steps of all key tiles before this one, of one key / value head
     float* pieces;           // [2 * workers][128][dk4 + dv4]
 };
@@ -63,7 +63,7 @@ __global__ __launch_bounds__(NTHREADS) void window_delta(const WindowGrad a) {
             if (x < tiles) {
                 const int n = (int)(x / a.ktiles);
                 const WindowLens len = {p.QLens ? min(max(p.QLens[n], 0), p.QL) : p.QL, p.VLens ? min(max(p.VLens[n], 0), p.VL) : p.VL};
-                own = (long long)window_steps(window_queries(p, (int)(x - (long long)n * a.ktiles), len), a.per_step) * group;
+                own = (long long)window_steps(window_queries(p, (int)(x - (long long)n * a.ktiles), len), 32) * group;
             }
             sum[t] = own;
             __syncthreads();
@@ -118,7 +118,7 @@ __device__ __forceinline__ void take(const float* at, v16f& e) {
 
 // ---------------------------------------------------------------- dQ
 template <int DB, int DC, int KB>
-__global__ __launch_bounds__(GT, 2) void window_grad_q(const WindowGrad a) {
+__global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_q(const WindowGrad a) {
     constexpr int DW = DB * 32, NG = DC * 4, AK = KB * 32, TILE = AK * DW;
     const WindowParams& p = a.w;
     __shared__ __attribute__((aligned(16))) float Ks[3 * TILE];
@@ -261,14 +261,14 @@ __device__ __forceinline__ long long grad_find(const WindowGrad& a, long long po
     }
     return lo;
 }
-// where worker w's run begins; a boundary up to two steps away from a tile's moves there, which saves two pieces
+// where worker w's run begins; a boundary that is not farther from a tile's than what two pieces cost moves there
 __device__ __forceinline__ long long grad_begin(const WindowGrad& a, const GradDeal& d, long long w) {
     if (w <= 0) return 0;
     if (w >= d.workers) return d.total;
     const long long pos = d.total / d.workers * w + (d.total % d.workers) * w / d.workers;
     const GradTile tile = grad_tile(a, grad_find(a, pos));
     if (tile.steps == 0) return pos;
-    const int in = (int)((pos - tile.at) % tile.steps), snap = (int)min(2LL, d.total / d.workers / 4);
+    const int in = (int)((pos - tile.at) % tile.steps), snap = (int)min((long long)a.snap, d.total / d.workers / 2);
     return in <= snap ? pos - in : tile.steps - in <= snap ? pos + tile.steps - in : pos;
 }
 // the worker whose run holds step pos
@@ -279,37 +279,47 @@ __device__ __forceinline__ long long grad_worker(const WindowGrad& a, const Grad
     return w;
 }
 
-template <int DB, int DC, int QB>
-__global__ __launch_bounds__(GT, 2) void window_grad_kv(const WindowGrad a) {
-    constexpr int DW = DB * 32, NG = DC * 4, AQ = QB * 32, TILE = AQ * DW;
-    const WindowParams& p = a.w;
+// the kernel's arguments, as if they had just been passed
+__device__ __forceinline__ const WindowGrad& anew(const WindowGrad&) {
+    auto at = (const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    return *(const WindowGrad*)(const char*)at;
+}
+
+template <int DB, int DC>
+__global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_kv(const WindowGrad arg) {
+    constexpr int DW = DB * 32, NG = DC * 4, TILE = 32 * DW;
     __shared__ __attribute__((aligned(16))) float Qs[3 * TILE];
     __shared__ __attribute__((aligned(16))) float Gs[3 * TILE];
-    __shared__ __attribute__((aligned(16))) float Ps[2][4][QB * 64 * 16];  // [step][32 keys][queries / 8][lane]
+    __shared__ __attribute__((aligned(16))) float Ps[2][4][64 * 16];       // [step][32 keys][4 results][lane]
     const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
     const int block = wave & 3;
     const bool second = wave >= 4;
-    const int group = p.head / p.kv_head;
 
-    const GradDeal deal = grad_deal(a);
+    const GradDeal deal = grad_deal(arg);
     auto uniform = [](long long x) { return (long long)(((unsigned long long)(unsigned)mix_uniform((int)(x >> 32)) << 32) | (unsigned)mix_uniform((int)x)); };
     if (blockIdx.x >= deal.workers) return;
-    long long pos = uniform(grad_begin(a, deal, blockIdx.x));
-    const long long stop = uniform(grad_begin(a, deal, blockIdx.x + 1));
+    long long pos = uniform(grad_begin(arg, deal, blockIdx.x));
+    const long long stop = uniform(grad_begin(arg, deal, blockIdx.x + 1));
 
-    MixTile<DW, AQ, true, GT> qt, gt;
+    MixTile<DW, 32, true, GT> qt, gt;
     MixColumns<DW, true> cols;
     cols.init(r, h);
-    qt.init(t, p.q.l, p.dk4);
-    gt.init(t, p.y.l, p.dv4);
+    qt.init(t, arg.w.q.l, arg.w.dk4);
+    gt.init(t, arg.w.y.l, arg.w.dv4);
     const unsigned qlds = mix_lds(Qs) + wave * 1024, glds = mix_lds(Gs) + wave * 1024;
-    const bool mover = wave * 64 < AQ * (DW / 4);                       // a small tile does not need all the threads
+    const bool mover = wave * 64 < 32 * (DW / 4);                       // a small tile does not need all the threads
     const float* const X = second ? Gs : Qs;                            // the tile of the first product, of the second
     const float* const Z = second ? Qs : Gs;
-    const float* const stats = a.stats + (second ? a.rows : 0);
 
-    long long at = pos < stop ? uniform(grad_find(a, pos)) : 0;         // the tile over all sequences
+    long long at = pos < stop ? uniform(grad_find(arg, pos)) : 0;         // the tile over all sequences
     while (pos < stop) {
+        // The arguments are read anew for every piece: kept in scalar registers all through the kernel they do not fit there,
+        // and under that pressure the compiler gives up the order of reads and matrix instructions in the loop below.
+        const WindowGrad& a = anew(arg);
+        const WindowParams& p = a.w;
+        const int group = mix_uniform(p.head / p.kv_head);
+        const float* const stats = a.stats + (second ? a.rows : 0);
         GradTile cur = grad_tile(a, at);
         while (pos >= cur.at + (long long)cur.steps * p.kv_head) cur = grad_tile(a, ++at);     // also over tiles without steps
         at = uniform(at);
@@ -320,7 +330,7 @@ __global__ __launch_bounds__(GT, 2) void window_grad_kv(const WindowGrad a) {
         const int n = mix_uniform((int)(at / a.ktiles)), tile = mix_uniform((int)(at - (long long)n * a.ktiles));
         const WindowLens len = window_lens(p, n);
         const WindowQueries qs = window_queries(p, tile, len);
-        const int lo = qs.lo, hi = qs.hi, per_head = window_steps(qs, AQ), off = len.vl - len.ql;
+        const int lo = qs.lo, hi = qs.hi, per_head = window_steps(qs, 32), off = len.vl - len.ql;
         const int u0 = tile * GK + block * 32, u1 = min(u0 + 32, len.vl) - 1;      // the wavefront's keys
         const int key = u0 + r;
         const bool live = key < len.vl;
@@ -333,111 +343,104 @@ __global__ __launch_bounds__(GT, 2) void window_grad_kv(const WindowGrad a) {
 #pragma unroll
             for (int g = 0; g < NG; g++) own[g] *= p.c;
         }
-        // the statistics of a step's queries, as the products' start: rows 8q + 4h .. +3 (zeros beyond the last of the head)
-        v16f start[QB];
-        auto begin = [&](int g, int i0) {
-            const float* row = stats + ((size_t)n * p.head + kvh * group + g) * p.QL + i0;
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)row, 0, min(p.QL - i0, AQ) * 4, RSRC_FLAGS);
-#pragma unroll
-            for (int q = 0; q < 4 * QB; q++) {
-                const v4f x = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rs, (8 * q + 4 * h) * 4, 0, 0));
-#pragma unroll
-                for (int w = 0; w < 4; w++) start[q / 4][4 * (q % 4) + w] = x[w];
+        // Queries go by in steps of 32 rows, head by head.  Everything that is fetched for a step moves along as an address (a
+        // step on, or to the next head's first): so few scalar registers that the compiler keeps the loop's order.
+        const int g0 = mix_uniform(first / per_head);
+        int i0 = lo + (first - g0 * per_head) * 32;                     // the step's queries
+        struct Walk {
+            int i0;
+            const float* at;
+            __device__ __forceinline__ void next(int lo, int hi, int step, long long jump) {
+                i0 += 32;
+                if (i0 >= hi) { i0 = lo; at += jump; }
+                else at += step;
             }
         };
-        auto fetch = [&](int g, int i0, int into) {
-            const int hd = kvh * group + g;
+        const int hd0 = kvh * group + g0;
+        Walk wq = {i0, p.Q + n * p.q.n + hd0 * p.q.h + (size_t)i0 * p.q.l};
+        Walk wg = {i0, a.dY + n * p.y.n + hd0 * p.y.h + (size_t)i0 * p.y.l};
+        Walk ws = {i0, stats + ((size_t)n * p.head + hd0) * p.QL + i0};
+        const long long q_jump = p.q.h - (long long)(per_head - 1) * 32 * p.q.l, g_jump = p.y.h - (long long)(per_head - 1) * 32 * p.y.l;
+        const int s_jump = p.QL - (per_head - 1) * 32;
+        auto fetch = [&](int into) {
             if (mover) {
-                qt.fetch(p.Q + n * p.q.n + hd * p.q.h + (size_t)i0 * p.q.l, hi - i0, p.q.l, qlds + into * (TILE * 4));
-                gt.fetch(a.dY + n * p.y.n + hd * p.y.h + (size_t)i0 * p.y.l, hi - i0, p.y.l, glds + into * (TILE * 4));
+                qt.fetch(wq.at, hi - wq.i0, p.q.l, qlds + into * (TILE * 4));
+                gt.fetch(wg.at, hi - wq.i0, p.y.l, glds + into * (TILE * 4));
             }
+            wg.next(lo, hi, 32 * p.y.l, g_jump);
+            wq.next(lo, hi, 32 * p.q.l, q_jump);
+        };
+        // the statistics of a step's queries, as the products' start: rows 8q + 4h .. +3 (zeros beyond the last of the sequence)
+        v16f start;
+        auto begin = [&]() {
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)ws.at, 0, min(hi - ws.i0, 32) * 4, RSRC_FLAGS);
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const v4f x = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rs, (8 * q + 4 * h) * 4, 0, 0));
+#pragma unroll
+                for (int w = 0; w < 4; w++) start[4 * q + w] = x[w];
+            }
+            ws.next(lo, hi, 32, s_jump);
         };
         v16f acc[DC];
 #pragma unroll
         for (int b = 0; b < DC; b++) acc[b] = (v16f)(0.0f);
 
-        int g = mix_uniform(first / per_head), i0 = lo + (first - g * per_head) * AQ;   // the step's queries
-        auto next = [&](int& hd, int& i) {
-            i += AQ;
-            if (i >= hi) { i = lo; hd++; }
-        };
-        int fg = g, fi0 = i0, i0_next;                                  // the next to fetch; the next step's
-        fetch(fg, fi0, 0);
-        begin(g, i0);
-        next(fg, fi0);
+        fetch(0);
+        begin();
         mix_wait();
-        if (first + 1 < last) {
-            fetch(fg, fi0, 1);
-            next(fg, fi0);
-        }
+        if (first + 1 < last) fetch(1);
         __syncthreads();
         int buf = 0;
         for (int s = first; s < last; s++) {
-            const int p0 = i0 + off, p1 = min(i0 + AQ, hi) - 1 + off;  // the step's positions
+            const int p0 = i0 + off, p1 = min(i0 + 32, hi) - 1 + off;  // the step's positions
             const bool sees = u0 <= u1 && p1 >= u0 && (p0 < u1 + p.window || u0 < p.sinks);
             float* exchange = &Ps[s & 1][block][4 * lane];
-            v16f e[QB];
-#pragma unroll
-            for (int qb = 0; qb < QB; qb++) e[qb] = start[qb];
-            next(g, i0_next = i0);
-            if (s + 1 < last) begin(g, i0_next);                       // there when this wavefront waits for its transfers
+            v16f e = start;
+            if (s + 1 < last) begin();                                  // there when this wavefront waits for its transfers
             if (sees) {
-#pragma unroll
-                for (int qb = 0; qb < QB; qb++) mix_rows_product<DW, NG>(e[qb], X + buf * TILE + qb * 32 * DW, own, r, h);
+                mix_rows_product<DW, NG>(e, X + buf * TILE, own, r, h);
                 if (!second) {
 #pragma unroll
-                    for (int qb = 0; qb < QB; qb++)
-#pragma unroll
-                        for (int v = 0; v < 16; v++) e[qb][v] = __builtin_amdgcn_exp2f(e[qb][v]);
+                    for (int v = 0; v < 16; v++) e[v] = __builtin_amdgcn_exp2f(e[v]);
                 }
                 // queries before a key, those whose window has passed it, and rows behind the last: tested only where there are
                 // any.  Both factors are cleared: dY.V^T may be anything where nothing is seen.
-                if (p0 < u1 || i0 + AQ > hi || u0 + 32 > len.vl) {
+                if (p0 < u1 || i0 + 32 > hi || u0 + 32 > len.vl) {
                     const int low = (live ? key : 0x3fffffff) - p0 - 4 * h, top = hi - 1 - i0 - 4 * h;
 #pragma unroll
-                    for (int qb = 0; qb < QB; qb++)
-#pragma unroll
-                        for (int v = 0; v < 16; v++)
-                            if (32 * qb + mix_row(v, 0) < low || 32 * qb + mix_row(v, 0) > top) e[qb][v] = 0.0f;
+                    for (int v = 0; v < 16; v++)
+                        if (mix_row(v, 0) < low || mix_row(v, 0) > top) e[v] = 0.0f;
                 }
                 if (p1 >= u0 + p.window) {
                     const int top = key < p.sinks ? 0x3fffffff : key + p.window - 1 - p0 - 4 * h;
 #pragma unroll
-                    for (int qb = 0; qb < QB; qb++)
-#pragma unroll
-                        for (int v = 0; v < 16; v++)
-                            if (32 * qb + mix_row(v, 0) > top) e[qb][v] = 0.0f;
+                    for (int v = 0; v < 16; v++)
+                        if (mix_row(v, 0) > top) e[v] = 0.0f;
                 }
-                if (!second) {
-#pragma unroll
-                    for (int qb = 0; qb < QB; qb++) give(exchange + qb * 1024, e[qb]);
-                }
+                if (!second) give(exchange, e);
             }
             mix_wait();
             __syncthreads();
             const int b1 = buf == 2 ? 0 : buf + 1, b2 = b1 == 2 ? 0 : b1 + 1;
-            if (s + 2 < last) {
-                fetch(fg, fi0, b2);
-                next(fg, fi0);
-            }
+            if (s + 2 < last) fetch(b2);
             __builtin_amdgcn_sched_barrier(0);
             if (sees) {
-#pragma unroll
-                for (int qb = 0; qb < QB; qb++) {
-                    if (second) take(exchange + qb * 1024, e[qb]);
-                    mix_columns_product<DW, DC, true>(acc, Z + buf * TILE + qb * 32 * DW, e[qb], cols, r, h);
-                }
+                if (second) take(exchange, e);
+                mix_columns_product<DW, DC, true>(acc, Z + buf * TILE, e, cols, r, h);
             }
             buf = b1;
-            i0 = i0_next;
+            i0 += 32;
+            if (i0 >= hi) i0 = lo;
         }
+        const WindowGrad& b = anew(arg);
         float* out;
         if (first == 0 && last == all) {
-            out = second ? a.dK + n * p.k.n + kvh * p.k.h + (size_t)key * p.k.l : a.dV + n * p.v.n + kvh * p.v.h + (size_t)key * p.v.l;
+            out = second ? b.dK + n * b.w.k.n + kvh * b.w.k.h + (size_t)key * b.w.k.l : b.dV + n * b.w.v.n + kvh * b.w.v.h + (size_t)key * b.w.v.l;
         } else {        // a piece that does not begin the tile is this run's first, one that does its last
-            out = a.pieces + ((2 * (size_t)blockIdx.x + (first == 0)) * GK + block * 32 + r) * (p.dk4 + p.dv4) + (second ? 0 : p.dk4);
+            out = b.pieces + ((2 * (size_t)blockIdx.x + (first == 0)) * GK + block * 32 + r) * (b.w.dk4 + b.w.dv4) + (second ? 0 : b.w.dk4);
         }
-        if (key < p.VL) mix_store_row<DC>(out, acc, second ? a.scale : 1.0f, second ? p.dk4 : p.dv4, h);
+        if (key < b.w.VL) mix_store_row<DC>(out, acc, second ? b.scale : 1.0f, second ? b.w.dk4 : b.w.dv4, h);
         __syncthreads();                                                // the next piece's first tile lands in buffer 0
     }
 }
@@ -477,7 +480,7 @@ struct WindowGradBuffer { int ktiles, workers; long long stats, before, pieces; 
 WindowGradBuffer window_grad_buffer(int N, int head, int QL, int VL, int dk4, int dv4) {
     WindowGradBuffer b;
     b.ktiles = (VL + GK - 1) / GK;
-    b.workers = 256;                                                  // one for each compute unit: their LDS holds no two
+    b.workers = (dk4 > dv4 ? dk4 : dv4) > 64 ? 256 : 512;                                                  // one for each compute unit: their LDS holds no two
     b.stats = (2LL * N * head * QL + 3) / 4 * 4;
     b.before = (((long long)N * b.ktiles + 1) * 2 + 3) / 4 * 4;
     b.pieces = 2LL * b.workers * GK * (dk4 + dv4);
@@ -532,7 +535,7 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
     a.rows = (long long)N * head * QL;
     a.scale = scale;
     a.ktiles = b.ktiles; a.workers = b.workers;
-    a.per_step = (dK4 > dV4 ? dK4 : dV4) > 64 ? 32 : 64;
+    a.snap = 2;
     a.before = (long long*)(a.stats + b.stats);
     a.pieces = a.stats + b.stats + b.before;
     split_ledger_touch(a.dQ, (size_t)N * head * QL * dK4 * 4);
@@ -549,7 +552,7 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
     const int dmax = dK4 > dV4 ? dK4 : dV4;
 #define GRAD_CASE(DB_, DC_, B_)                                                        \
     do {                                                                              \
-        hipLaunchKernelGGL((window_grad_kv<DB_, DC_, B_>), gk, dim3(GT), 0, s, a);        \
+        hipLaunchKernelGGL((window_grad_kv<DB_, DC_>), gk, dim3(GT), 0, s, a);        \
         e = hipGetLastError();                                                        \
         if (e != hipSuccess) return e;                                                \
         hipLaunchKernelGGL((window_grad_q<DB_, DC_, B_>), gq, dim3(GT), 0, s, a);         \
@@ -557,8 +560,8 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
         if (e != hipSuccess) return e;                                                \
     } while (0)
     switch ((dmax + 31) / 32) {
-        case 1: GRAD_CASE(1, 1, 2); break;
-        case 2: GRAD_CASE(2, 2, 2); break;
+        case 1: GRAD_CASE(1, 1, 1); break;
+        case 2: GRAD_CASE(2, 2, 1); break;
         case 3: GRAD_CASE(4, 3, 1); break;
         default: GRAD_CASE(4, 4, 1); break;
     }

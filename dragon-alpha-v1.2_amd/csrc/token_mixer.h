@@ -140,6 +140,7 @@ __device__ __forceinline__ void mix_columns_product(v16f (&o)[DC], const float* 
 // a lane's column of a result, times f: float 32b + 8g + 4h .. +3 of the row at `row`
 template <int DC>
 __device__ __forceinline__ void mix_store_row(float* row, const v16f (&o)[DC], float f, int d4, int h) {
+    d4 = fresh(d4);     // or the tests' results, 4 * DC of them, sit in scalar registers all through the kernel
 #pragma unroll
     for (int b = 0; b < DC; b++)
 #pragma unroll
@@ -152,6 +153,7 @@ __device__ __forceinline__ void mix_store_row(float* row, const v16f (&o)[DC], f
 // the lane's column of an operand: 4 consecutive floats per group of 8, zeros where the row does not exist
 template <int NG>
 __device__ __forceinline__ void mix_load_cols(v4f (&c)[NG], const float* row, bool exists, int d4, int h) {
+    d4 = fresh(d4);
 #pragma unroll
     for (int g = 0; g < NG; g++) {
         const int d = 8 * g + 4 * h;
