@@ -156,15 +156,12 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_q(const Window
     kt.init(t, p.k.l, p.dk4);
     vt.init(t, p.v.l, p.dv4);
     const unsigned klds = mix_lds(Ks) + wave * 1024, vlds = mix_lds(Vs) + wave * 1024;
-    const bool mover = wave * 64 < AK * (DW / 4);                       // a small tile does not need all the threads
     const float* const X = second ? Vs : Ks;
     auto key_of = [&](int s) { return s < nsink ? s * AK : range.low + (s - nsink) * AK; };
     auto fetch = [&](int s, int into) {
         const int key0 = key_of(s), left = (s < nsink ? range.sink_end : range.hi) - key0;
-        if (mover) {
-            kt.fetch(Kb + (size_t)key0 * p.k.l, left, p.k.l, klds + into * (TILE * 4));
-            vt.fetch(Vb + (size_t)key0 * p.v.l, left, p.v.l, vlds + into * (TILE * 4));
-        }
+        kt.fetch(Kb + (size_t)key0 * p.k.l, left, p.k.l, klds + into * (TILE * 4), wave);
+        vt.fetch(Vb + (size_t)key0 * p.v.l, left, p.v.l, vlds + into * (TILE * 4), wave);
     };
     v16f o[DC];
 #pragma unroll
@@ -308,7 +305,6 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_kv(const Windo
     qt.init(t, arg.w.q.l, arg.w.dk4);
     gt.init(t, arg.w.y.l, arg.w.dv4);
     const unsigned qlds = mix_lds(Qs) + wave * 1024, glds = mix_lds(Gs) + wave * 1024;
-    const bool mover = wave * 64 < 32 * (DW / 4);                       // a small tile does not need all the threads
     const float* const X = second ? Gs : Qs;                            // the tile of the first product, of the second
     const float* const Z = second ? Qs : Gs;
 
@@ -363,10 +359,8 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_kv(const Windo
         const long long q_jump = p.q.h - (long long)(per_head - 1) * 32 * p.q.l, g_jump = p.y.h - (long long)(per_head - 1) * 32 * p.y.l;
         const int s_jump = p.QL - (per_head - 1) * 32;
         auto fetch = [&](int into) {
-            if (mover) {
-                qt.fetch(wq.at, hi - wq.i0, p.q.l, qlds + into * (TILE * 4));
-                gt.fetch(wg.at, hi - wq.i0, p.y.l, glds + into * (TILE * 4));
-            }
+            qt.fetch(wq.at, hi - wq.i0, p.q.l, qlds + into * (TILE * 4), wave);
+            gt.fetch(wg.at, hi - wq.i0, p.y.l, glds + into * (TILE * 4), wave);
             wg.next(lo, hi, 32 * p.y.l, g_jump);
             wq.next(lo, hi, 32 * p.q.l, q_jump);
         };

@@ -3,17 +3,18 @@
 // and its gradient.
 //
 // Few tokens (decay_steps): the recurrence itself, the state in registers; bound by reading and writing the states.
-// Many tokens: chunks of C.  With S_c the state before chunk c and t the token's place in it,
-//     Y[t] = scale * (e^{g(t+1)} Q[t] S_c  +  sum_{j <= t} e^{g(t-j)} <Q[t], K[j]> V[j])
-// in three launches: decay_states adds up each chunk's own K^T V, decay_scan runs over the chunks and leaves S_c in their
-// place, decay_mix multiplies.  The chunks are independent in the first and the last, so a single long sequence fills the
-// chip; bound by the FP32 matrix pipe, then by memory (a longer chunk: more products inside it, fewer states to move).
+// Many tokens (decay_walk): 32 at a time.  With S the state before them and t a token's place among them,
+//     Y[t] = scale * (e^{g(t+1)} Q[t] S  +  sum_{j <= t} e^{g(t-j)} <Q[t], K[j]> V[j]),    S' = e^{32g} S + sum_j e^{g(31-j)} K[j]^T V[j]
+// A workgroup walks along a sequence with the state in its registers, a wavefront for each 32 columns of V.  Where there are
+// fewer (image, head) pairs than the chip takes workgroups the sequence is cut into segments that walk at the same time:
+// decay_states forms each segment's own sum, decay_scan runs over them and leaves the state that each begins with.
+// Bound by the FP32 matrix pipe: 2.5 products of [dk, dv] size a token, and one more where there are segments.
 //
-// The gradient is the same three launches with other operands (G = gradient of Y, sums over j >= t in the last two):
-//     dQ[t] = scale sum e^{g(t-j)} <G[t], V[j]> K[j] + ...  S_c^T           the states of the forward pass again
-//     dK[t] = scale sum e^{g(j-t)} <V[t], G[j]> Q[j] + ...  R_c^T           R: the same sum from the sequence's end,
-//     dV[t] = scale sum e^{g(j-t)} <K[t], Q[j]> G[j] + ...  R_c             over Q^T G, starting with the gradient of the last state
-// so decay_mix takes its operands x, y, z by name, a direction, and the state either way round.
+// The gradient is the same walk with other operands (G = gradient of Y, sums over j >= t in the last two, from the end):
+//     dQ[t] = scale sum e^{g(t-j)} <G[t], V[j]> K[j] + ...  S^T           the states of the forward pass again
+//     dK[t] = scale sum e^{g(j-t)} <V[t], G[j]> Q[j] + ...  R^T           R: the same sum from the sequence's end,
+//     dV[t] = scale sum e^{g(j-t)} <K[t], Q[j]> G[j] + ...  R             over Q^T G, starting with the gradient of the last state
+// so decay_walk takes its operands x, y, z by name, a direction, and the beginning state either way round.
 //
 // Every power e^{g n} is computed as such (n >= 0: it cannot overflow), never as a quotient of two powers.  States, sums and
 // powers are FP32; the exponent g n is rounded once, which is an error of |g n| 2^-24 in a factor e^{g n}.
@@ -24,20 +25,17 @@
 namespace dragon {
 namespace {
 
-constexpr int TQ = 128;       // tokens per workgroup of decay_mix: 32 per wavefront
-constexpr int MAX_CHUNK = 256;
-
-struct DecayParams {
+struct DecayWalk {
     const float* x; const float* y; const float* z; float* out;   // [L, xd], [L, xd], [L, zd], [L, zd] per (image, head)
     MixLayout lx, ly, lz, lo;
     const float* g; const int* lens;
-    int head, L, xd, zd, C, chunks;
+    int head, L, xd, zd;
+    int segment, segments;     // tokens of a segment, a multiple of 32
     int back;                  // sums over j >= t instead of j <= t
-    float near_scale, far_scale;   // factors on the sum inside the chunk and on the state's share
-    const float* state;        // the state before each chunk, [image, head, chunk]; null: none at all
-    int empty_first;           // the state at the sequence's beginning (back: at its end) is zero
-    long long state_nh, state_c;   // its strides
-    int tiles, nh;
+    float near_scale, far_scale, add_scale;   // factors on the sum inside 32 tokens, on the state's share, on what enters the state
+    const float* state;        // what each segment begins with (back: at its end), [image, head, segment]; null: zeros
+    float* last;               // one segment: the state at the other end; null: nobody wants it
+    int nh;                    // image-head pairs
 };
 
 __device__ __forceinline__ float decay_log2(const float* g, int hd) {
@@ -47,138 +45,197 @@ __device__ __forceinline__ float decay_log2(const float* g, int hd) {
 __device__ __forceinline__ float decay_pow(float g2, int n) { return __builtin_amdgcn_exp2f(g2 * (float)n); }
 __device__ __forceinline__ int decay_len(const int* lens, int n, int L) { return lens ? min(max(lens[n], 0), L) : L; }
 
-// ---------------------------------------------------------------- inside the chunks, and the state's share
-// ST: the state lies [zd][xd] (its transpose is what multiplies x)
-template <int DB, int DC, bool ST>
-__global__ __launch_bounds__(NTHREADS, 2) void decay_mix(const DecayParams p) {
-    constexpr int DW = DB * 32, NG = DC * 4;
-    __shared__ __attribute__((aligned(16))) float Ys[2][32 * DW];
-    __shared__ __attribute__((aligned(16))) float Zs[2][32 * DW];
+// ---------------------------------------------------------------- along the sequence
+// Wavefront b of a workgroup owns 32 columns of the state and of the output (as result columns' rows: out^T[32][token]).
+//   scores   every wavefront a part of the head dimension; the parts are added through LDS
+//   x . S    out^T[column][token] += S^T . x^T: the state's registers are the A operand as they stand
+//   near     out^T[column][token] += z^T . scores
+//   S'       S^T... [row][column] = decayed + y^T . z, the result layout that x . S takes
+// XB: 32-wide blocks of x's width in LDS (1, 2, 4), ZB: of z's, one wavefront each.  ST: the beginning state lies [zd][xd].
+// Two workgroups share a compute unit (80 KiB of LDS each at widths of 128).  Two barriers for 32 tokens: behind the first the
+// scores and z are there and x is free, behind the second z is free and the next x and y are there; y has two buffers.
+template <int XB, int ZB, bool ST>
+__global__ __launch_bounds__(64 * ZB, 2) void decay_walk(const DecayWalk p) {
+    constexpr int XW = XB * 32, ZW = (ZB == 3 ? 4 : ZB) * 32, NG = XB * 4, SHARE = (NG + ZB - 1) / ZB;
+    __shared__ __attribute__((aligned(16))) float Xs[32 * XW];
+    __shared__ __attribute__((aligned(16))) float Ys[2][32 * XW];
+    __shared__ __attribute__((aligned(16))) float Zs[32 * ZW];
+    __shared__ __attribute__((aligned(16))) float Ps[ZB][1024];
     const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
-    const int lid = xcd_contiguous_id(blockIdx.x, gridDim.x);
-    const int tile = mix_uniform(lid / p.nh), nh = lid - tile * p.nh;
+    const int lid = xcd_contiguous_id(blockIdx.x, gridDim.x);   // one XCD works on all heads of the same tokens, which lie side by side
+    const int segment = mix_uniform(lid / p.nh), nh = lid - segment * p.nh;
     const int n = mix_uniform(nh / p.head), hd = nh - n * p.head;
     const int len = mix_uniform(decay_len(p.lens, n, p.L));
-    // Inside a chunk the later (back: the earlier) 32 tokens have the most to do.  The workgroups that share a compute unit
-    // give them to different wavefronts, so that no SIMD has all the work.
-    const int q0 = tile * TQ, w0 = q0 + 32 * ((blockIdx.x >> 8) & 1 ? 3 - wave : wave), i = w0 + r;
-    const int chunk = mix_uniform(q0 / p.C), c0 = chunk * p.C, c1 = min(c0 + p.C, len);
+    const int from = segment * p.segment, end = min(from + p.segment, p.L), to = max(min(end, len), from);
     const float g2 = decay_log2(p.g, hd);
-    const float* xb = p.x + n * p.lx.n + hd * p.lx.h;
-    const float* yb = p.y + n * p.ly.n + hd * p.ly.h;
-    const float* zb = p.z + n * p.lz.n + hd * p.lz.h;
+    const int col = 32 * wave + r;                              // this lane's column of the state
+    const float* const xb = p.x + n * p.lx.n + hd * p.lx.h;
+    const float* const yb = p.y + n * p.ly.n + hd * p.ly.h;
+    const float* const zb = p.z + n * p.lz.n + hd * p.lz.h;
+    float* const ob = p.out + n * p.lo.n + hd * p.lo.h + 32 * wave;
+    const int mine = p.zd - 32 * wave;                          // floats of a row of `out` from this wavefront's on
 
-    v4f xf[NG];
-    mix_load_cols<NG>(xf, xb + (size_t)min(i, p.L - 1) * p.lx.l, i < len, p.xd, h);
-    v16f o[DC];
-#pragma unroll
-    for (int b = 0; b < DC; b++) o[b] = (v16f)(0.0f);
-
-    MixColumns<DW, false> zcols;
-    zcols.init(r, h);
-
-    const unsigned ylds = mix_lds(Ys[0]) + wave * 1024, zlds = mix_lds(Zs[0]) + wave * 1024;
-    constexpr unsigned TILE = 32 * DW * 4;
-
-    // ---- x . S: 32 rows of the state per step ----
-    const bool first_chunk = p.back ? c1 == len : chunk == 0;
-    if (q0 < len && p.state != nullptr && !(first_chunk && p.empty_first)) {
-        const float* sb = p.state + nh * p.state_nh + chunk * p.state_c;
-        if constexpr (ST) {
-            MixTile<DW, 32, true> st;
-            st.init(t, p.xd, p.xd);
-            st.fetch(sb, p.zd, p.xd, ylds);
-            static_for<DC>([&](auto bc) {
-                constexpr int b = decltype(bc)::value;
-                mix_wait();
-                __syncthreads();
-                if (b + 1 < DC) st.fetch(sb + (size_t)(b + 1) * 32 * p.xd, p.zd - (b + 1) * 32, p.xd, ylds + ((b + 1) & 1) * TILE);
-                __builtin_amdgcn_sched_barrier(0);
-                mix_rows_product<DW, NG>(o[b], Ys[b & 1], xf, r, h);
-            });
-        } else {
-            MixTile<DW, 32, false> st;
-            st.init(t, p.zd, p.zd);
-            st.fetch(sb, p.xd, p.zd, zlds);
-            static_for<DC>([&](auto bc) {
-                constexpr int b = decltype(bc)::value;
-                mix_wait();
-                __syncthreads();
-                if (b + 1 < DC) st.fetch(sb + (size_t)(b + 1) * 32 * p.zd, p.xd - (b + 1) * 32, p.zd, zlds + ((b + 1) & 1) * TILE);
-                __builtin_amdgcn_sched_barrier(0);
-                v16f w;
-#pragma unroll
-                for (int v = 0; v < 16; v++) w[v] = xf[4 * b + v / 4][v % 4];
-                mix_columns_product<DW, DC, false>(o, Zs[b & 1], w, zcols, r, h);
-            });
-        }
-        const float f = decay_pow(g2, max(p.back ? c1 - 1 - i : i - c0 + 1, 0)) * p.far_scale;
-#pragma unroll
-        for (int b = 0; b < DC; b++)
-#pragma unroll
-            for (int v = 0; v < 16; v++) o[b][v] *= f;
-        __syncthreads();
-    }
-
-    // ---- the chunk's own tokens, 32 per step ----
-    const int from = p.back ? q0 : c0, to = q0 < len ? (p.back ? c1 : min(q0 + TQ, len)) : from;
-    MixTile<DW, 32, true> yt;
-    MixTile<DW, 32, false> zt;
+    MixTile<XW, 32, true, 64 * ZB> xt, yt;
+    MixTile<ZW, 32, false, 64 * ZB> zt;
+    MixColumns<XW, true> cols;
+    cols.init(r, h);
+    xt.init(t, p.lx.l, p.xd);
     yt.init(t, p.ly.l, p.xd);
     zt.init(t, p.lz.l, p.zd);
-    auto fetch = [&](int j0, int into) {
-        yt.fetch(yb + (size_t)j0 * p.ly.l, to - j0, p.ly.l, ylds + into * TILE);
-        zt.fetch(zb + (size_t)j0 * p.lz.l, to - j0, p.lz.l, zlds + into * TILE);
+    const unsigned xlds = mix_lds(Xs) + wave * 1024, ylds = mix_lds(Ys[0]) + wave * 1024, zlds = mix_lds(Zs) + wave * 1024;
+    auto fetch_xy = [&](int t0, int into) {
+        xt.fetch(xb + (size_t)t0 * p.lx.l, to - t0, p.lx.l, xlds, wave);
+        yt.fetch(yb + (size_t)t0 * p.ly.l, to - t0, p.ly.l, ylds + into * (32 * XW * 4), wave);
     };
-    // e^(g distance) inside the wavefront's own 32 tokens, and for 32 tokens that lie at least 32 away but for a factor that
-    // is the same for all of them: every power here is >= 0
-    float own[16], near[16];
+    auto fetch_z = [&](int t0) { zt.fetch(zb + (size_t)t0 * p.lz.l, to - t0, p.lz.l, zlds, wave); };
+
+    // ---- the state that the segment begins with: register v of block k is row 32k + mix_row(v, h), column col ----
+    v16f S[XB];
+    bool any = p.state != nullptr;                              // the state is not zero all over
+#pragma unroll
+    for (int k = 0; k < XB; k++) S[k] = (v16f)(0.0f);
+    if (any) {
+        const float* s0 = p.state + ((size_t)nh * p.segments + segment) * p.xd * p.zd;
+#pragma unroll
+        for (int k = 0; k < XB; k++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int row = 32 * k + 8 * q + 4 * h;
+                if (row < p.xd && col < p.zd) {
+                    if constexpr (ST) {
+                        const v4f s = *(const v4f*)(s0 + (size_t)col * p.xd + row);
+#pragma unroll
+                        for (int w = 0; w < 4; w++) S[k][4 * q + w] = s[w];
+                    } else {
+#pragma unroll
+                        for (int w = 0; w < 4; w++) S[k][4 * q + w] = s0[(size_t)(row + w) * p.zd + col];
+                    }
+                }
+            }
+    }
+    // powers: between tokens of the 32 (masked), of a token's entry into the state
+    float near[16], enter[16];
 #pragma unroll
     for (int v = 0; v < 16; v++) {
-        const int far = p.back ? mix_row(v, h) - r : r - mix_row(v, h);
-        own[v] = far < 0 ? 0.0f : decay_pow(g2, far) * p.near_scale;
-        near[v] = decay_pow(g2, 31 + far) * p.near_scale;
+        const int row = mix_row(v, h), far = p.back ? row - r : r - row;
+        near[v] = far < 0 ? 0.0f : decay_pow(g2, far) * p.near_scale;
+        enter[v] = decay_pow(g2, p.back ? row + 1 : 31 - row) * p.add_scale;
     }
-    if (from < to) fetch(from, 0);
+
+    const int chunks = (to - from + 31) / 32;
+    auto start = [&](int c) { return from + 32 * (p.back ? chunks - 1 - c : c); };
+    if (chunks > 0) {
+        fetch_xy(start(0), 0);
+        fetch_z(start(0));
+    }
     mix_wait();
     __syncthreads();
-    auto step = [&](auto bufc, int j0) {
-        constexpr int buf = decltype(bufc)::value;
-        if (j0 + 32 < to) fetch(j0 + 32, buf ^ 1);
-        __builtin_amdgcn_sched_barrier(0);
-        const int away = p.back ? j0 - w0 : w0 - j0;        // a multiple of 32
-        if (away >= 0) {
+    for (int c = 0; c < chunks; c++) {
+        const int t0 = start(c), count = min(32, to - t0), buf = c & 1;
+        const bool more = c + 1 < chunks;
+
+        // ---- this wavefront's part of the scores: groups of 8 of the head dimension ----
+        {
+            const unsigned at = r * (XW * 4) + 16 * (h ^ kin_swizzle<XW>(r));
+            typedef const __attribute__((address_space(3))) v4f* lds_v4f;
             v16f s = (v16f)(0.0f);
-            mix_rows_product<DW, NG>(s, Ys[buf], xf, r, h);
-            if (away > 0) {
-                const float f = decay_pow(g2, away - 31);
 #pragma unroll
-                for (int v = 0; v < 16; v++) s[v] *= near[v] * f;
-            } else {
-#pragma unroll
-                for (int v = 0; v < 16; v++) s[v] *= own[v];
+            for (int i = 0; i < SHARE; i++) {
+                const int g = wave * SHARE + i;
+                if (NG % ZB == 0 || g < NG) {
+                    const unsigned place = (at ^ (32 * (g & 7))) + 256 * (g >> 3);
+                    const v4f a = *(lds_v4f)(size_t)(mix_lds(Ys[buf]) + place), b = *(lds_v4f)(size_t)(mix_lds(Xs) + place);
+                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, b.x, s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, b.y, s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, b.z, s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, b.w, s, 0, 0, 0);
+                }
             }
-            mix_columns_product<DW, DC, false>(o, Zs[buf], s, zcols, r, h);
+#pragma unroll
+            for (int q = 0; q < 4; q++) *(v4f*)&Ps[wave][q * 256 + 4 * lane] = (v4f){s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
         }
-        mix_wait();
+        // ---- x . S ----
+        v16f o[1] = {(v16f)(0.0f)};
+        if (any) {
+            const unsigned at = mix_lds(Xs) + r * (XW * 4) + 16 * (h ^ kin_swizzle<XW>(r));
+            typedef const __attribute__((address_space(3))) v4f* lds_v4f;
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const v4f b = *(lds_v4f)(size_t)((at ^ (32 * (g & 7))) + 256 * (g >> 3));
+#pragma unroll
+                for (int w = 0; w < 4; w++) o[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(S[g / 4][4 * (g % 4) + w], b[w], o[0], 0, 0, 0);
+            }
+            mix_order<2, NG, 4>();
+            o[0] *= decay_pow(g2, p.back ? max(count - 1 - r, 0) : r + 1) * p.far_scale;
+        }
+        mix_wait();                                             // z
         __syncthreads();
-    };
-    for (int j0 = from; j0 < to; j0 += 64) {
-        step(std::integral_constant<int, 0>{}, j0);
-        if (j0 + 32 < to) step(std::integral_constant<int, 1>{}, j0 + 32);
+        if (more) fetch_xy(start(c + 1), buf ^ 1);
+        __builtin_amdgcn_sched_barrier(0);
+        // ---- the near tokens ----
+        v16f s;
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            v4f sum = *(const v4f*)&Ps[0][q * 256 + 4 * lane];
+#pragma unroll
+            for (int w = 1; w < ZB; w++) sum += *(const v4f*)&Ps[w][q * 256 + 4 * lane];
+#pragma unroll
+            for (int w = 0; w < 4; w++) s[4 * q + w] = sum[w] * near[4 * q + w];
+        }
+        float z[16];
+#pragma unroll
+        for (int v = 0; v < 16; v++) z[v] = Zs[mix_row(v, h) * ZW + col];
+#pragma unroll
+        for (int v = 0; v < 16; v++) o[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(z[v], s[v], o[0], 0, 0, 0);
+        // ---- into the state ----
+        if (more || p.last != nullptr) {
+            v16f zw;
+            if (count == 32 || p.back) {
+#pragma unroll
+                for (int v = 0; v < 16; v++) zw[v] = z[v] * enter[v];
+            } else {                                            // the sequence's last, shorter run
+#pragma unroll
+                for (int v = 0; v < 16; v++) zw[v] = z[v] * (decay_pow(g2, max(count - 1 - mix_row(v, h), 0)) * p.add_scale);
+            }
+            if (any) {
+                const float f = decay_pow(g2, count);
+#pragma unroll
+                for (int k = 0; k < XB; k++) S[k] *= f;
+            }
+            mix_columns_product<XW, XB, true>(S, Ys[buf], zw, cols, r, h);
+            any = true;
+        }
+        mix_wait();                                             // the next x and y
+        __syncthreads();
+        if (more) fetch_z(start(c + 1));
+        if (t0 + r < end) mix_store_row<1>(ob + (size_t)(t0 + r) * p.lo.l, o, 1.0f, mine, h);
     }
-    if (i < p.L) mix_store_row<DC>(p.out + n * p.lo.n + hd * p.lo.h + (size_t)i * p.lo.l, o, 1.0f, p.zd, h);
+    // ---- rows behind the sequence's end; the state at the other end ----
+    for (int t0 = from + 32 * chunks; t0 < end; t0 += 32)
+        if (t0 + r < end)
+            for (int d = 4 * h; d < min(mine, 32); d += 8) *(v4f*)(ob + (size_t)(t0 + r) * p.lo.l + d) = (v4f)(0.0f);
+    if (p.last != nullptr) {
+        float* s1 = p.last + (size_t)nh * p.xd * p.zd;
+#pragma unroll
+        for (int k = 0; k < XB; k++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) {
+                const int row = 32 * k + mix_row(v, h);
+                if (row < p.xd && col < p.zd) s1[(size_t)row * p.zd + col] = S[k][v];
+            }
+    }
 }
 
-// ---------------------------------------------------------------- a chunk's own sum
-// U[a, b] = sum_t e^{g n(t)} A[t, a] B[t, b], n(t) = tokens behind t in the chunk, or (back) t's place in it counted from 1
+// ---------------------------------------------------------------- a segment's own sum
+// U[a, b] = sum_t e^{g n(t)} A[t, a] B[t, b], n(t) = tokens behind t in the segment, or (back) t's place in it counted from 1
 struct DecayStates {
     const float* A; const float* B;
     MixLayout la, lb;
     const float* g; const int* lens;
-    int head, L, ad, bd, C, chunks, back;
+    int head, L, ad, bd, segment, segments, back;
     float scale;
-    float* U;                 // [image, head, chunk][ad][bd]
+    float* U;                 // [image, head, segment][ad][bd]
     int nh;
 };
 
@@ -189,12 +246,11 @@ __global__ __launch_bounds__(NTHREADS, 2) void decay_states(const DecayStates p)
     constexpr int TB = DC > 2 ? 2 : 1;
     __shared__ __attribute__((aligned(16))) float As[2][32 * DW];
     __shared__ __attribute__((aligned(16))) float Bs[2][32 * DW];
-    __shared__ __attribute__((aligned(16))) float Ws[MAX_CHUNK];      // a token's power
     const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
     const int lid = xcd_contiguous_id(blockIdx.x, gridDim.x);
-    const int chunk = mix_uniform(lid / p.nh), nh = lid - chunk * p.nh;
+    const int segment = mix_uniform(lid / p.nh), nh = lid - segment * p.nh;
     const int n = mix_uniform(nh / p.head), hd = nh - n * p.head;
-    const int c0 = chunk * p.C, cnt = min(p.C, mix_uniform(decay_len(p.lens, n, p.L)) - c0);
+    const int c0 = segment * p.segment, cnt = min(p.segment, mix_uniform(decay_len(p.lens, n, p.L)) - c0);
     if (cnt <= 0) return;                                // decay_scan does not read it
     const float g2 = decay_log2(p.g, hd);
     const float* ab = p.A + n * p.la.n + hd * p.la.h + (size_t)c0 * p.la.l;
@@ -214,39 +270,52 @@ __global__ __launch_bounds__(NTHREADS, 2) void decay_states(const DecayStates p)
     for (int a = 0; a < TB; a++)
 #pragma unroll
         for (int b = 0; b < TB; b++) u[a][b] = (v16f)(0.0f);
-    for (int j = t; j < MAX_CHUNK; j += NTHREADS) Ws[j] = decay_pow(g2, max(p.back ? j + 1 : cnt - 1 - j, 0)) * p.scale;
+    // a token's power: of its place among 32, times that of the 32 in the segment -- both exponents >= 0
+    float near[16];
+#pragma unroll
+    for (int v = 0; v < 16; v++) near[v] = decay_pow(g2, p.back ? mix_row(v, h) + 1 : 31 - mix_row(v, h)) * p.scale;
     fetch(0, 0);
     mix_wait();
     __syncthreads();
-    int buf = 0;
-    for (int j0 = 0; j0 < cnt; j0 += 32) {
+    auto step = [&](auto bufc, int j0) {
+        constexpr int buf = decltype(bufc)::value;
         if (j0 + 32 < cnt) fetch(j0 + 32, buf ^ 1);
         __builtin_amdgcn_sched_barrier(0);
         if (works) {
+            float power[16];
+            if (p.back || j0 + 32 <= cnt) {
+                const float f = decay_pow(g2, p.back ? j0 : cnt - 32 - j0);
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const v4f w = *(const v4f*)&Ws[j0 + 8 * q + 4 * h];
+                for (int v = 0; v < 16; v++) power[v] = near[v] * f;
+            } else {
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    const int row = mix_row(4 * q + x, h);
-                    float fa[TB], fb[TB];
-#pragma unroll
-                    for (int a = 0; a < TB; a++) fa[a] = As[buf][row * DW + (wa + a) * 32 + r];
-#pragma unroll
-                    for (int b = 0; b < TB; b++) fb[b] = Bs[buf][row * DW + (wb + b) * 32 + r] * w[x];
-#pragma unroll
-                    for (int a = 0; a < TB; a++)
-#pragma unroll
-                        for (int b = 0; b < TB; b++) u[a][b] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[a], fb[b], u[a][b], 0, 0, 0);
-                }
+                for (int v = 0; v < 16; v++) power[v] = decay_pow(g2, max(cnt - 1 - j0 - mix_row(v, h), 0)) * p.scale;
             }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int v = 0; v < 16; v++) {
+                const int row = mix_row(v, h);
+                float fa[TB], fb[TB];
+#pragma unroll
+                for (int a = 0; a < TB; a++) fa[a] = As[buf][row * DW + (wa + a) * 32 + r];
+#pragma unroll
+                for (int b = 0; b < TB; b++) fb[b] = Bs[buf][row * DW + (wb + b) * 32 + r] * power[v];
+#pragma unroll
+                for (int a = 0; a < TB; a++)
+#pragma unroll
+                    for (int b = 0; b < TB; b++) u[a][b] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[a], fb[b], u[a][b], 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
         mix_wait();
         __syncthreads();
-        buf ^= 1;
+    };
+    for (int j0 = 0; j0 < cnt; j0 += 64) {
+        step(std::integral_constant<int, 0>{}, j0);
+        if (j0 + 32 < cnt) step(std::integral_constant<int, 1>{}, j0 + 32);
     }
     if (!works) return;
-    float* U = p.U + ((size_t)nh * p.chunks + chunk) * p.ad * p.bd;
+    float* U = p.U + ((size_t)nh * p.segments + segment) * p.ad * p.bd;
 #pragma unroll
     for (int a = 0; a < TB; a++)
 #pragma unroll
@@ -260,12 +329,12 @@ __global__ __launch_bounds__(NTHREADS, 2) void decay_states(const DecayStates p)
         }
 }
 
-// ---------------------------------------------------------------- over the chunks
-// In place: U[chunk] becomes the state before the chunk (back: behind it); the one after the last goes to `last`.
+// ---------------------------------------------------------------- over the segments
+// In place: U[segment] becomes the state before the segment (back: behind it); the one after the last goes to `last`.
 struct DecayScan {
     float* U; const float* first; float* last;
     const float* g; const int* lens;
-    int head, L, C, chunks, back, size4;     // size4: float4s of a state
+    int head, L, segment, segments, back, size4;     // size4: float4s of a state
     long long nh;
 };
 __global__ __launch_bounds__(NTHREADS) void decay_scan(const DecayScan p) {
@@ -274,10 +343,10 @@ __global__ __launch_bounds__(NTHREADS) void decay_scan(const DecayScan p) {
     if (nh >= p.nh) return;
     const int e = (int)(x - nh * p.size4);
     const int n = (int)(nh / p.head), hd = (int)(nh - (long long)n * p.head);
-    const int len = decay_len(p.lens, n, p.L), used = (len + p.C - 1) / p.C;
+    const int len = decay_len(p.lens, n, p.L), used = (len + p.segment - 1) / p.segment;
     const float g2 = decay_log2(p.g, hd);
-    const float whole = decay_pow(g2, p.C), tail = decay_pow(g2, len - (used - 1) * p.C);
-    v4f* U = (v4f*)p.U + (size_t)nh * p.chunks * p.size4 + e;
+    const float whole = decay_pow(g2, p.segment), tail = decay_pow(g2, len - (used - 1) * p.segment);
+    v4f* U = (v4f*)p.U + (size_t)nh * p.segments * p.size4 + e;
     v4f s = p.first ? ((const v4f*)p.first)[nh * p.size4 + e] : (v4f)(0.0f);
     v4f next = (v4f)(0.0f);
     if (used > 0) next = U[(size_t)(p.back ? used - 1 : 0) * p.size4];
@@ -361,25 +430,44 @@ __global__ __launch_bounds__(NTHREADS) void decay_steps(const DecaySteps p) {
 // ---------------------------------------------------------------- host side
 constexpr int STEPS_MAX = 16;     // up to here the recurrence
 
-int decay_chunk(int dK4, int dV4) { return (dK4 > dV4 ? dK4 : dV4) > 64 ? 256 : 128; }
+// How a sequence is cut: into as many segments as fill the chip with workgroups, where that is faster than walking along
+// it whole -- the segments' sums cost one product more to the walk's two and a half, and two launches.
+struct DecayCut { int segment, segments; };
+DecayCut decay_cut(int N, int head, int L, int zd) {
+    const long long nh = (long long)N * head, chunks = (L + 31LL) / 32;
+    const long long slots = zd > 64 ? 512 : zd > 32 ? 1024 : 2048;    // workgroups (of zd / 32 wavefronts) that the chip holds
+    DecayCut best = {(int)(chunks * 32), 1};
+    double least = 0.0;
+    for (long long want = 1; want <= 64; want++) {
+        const long long per = (chunks + want - 1) / want, segments = (chunks + per - 1) / per;
+        if (segments != want) continue;
+        const double walk = (double)((nh * segments + slots - 1) / slots) * per;
+        const double cost = segments == 1 ? 2.5 * walk : 3.7 * walk + 12.0;
+        if (want == 1 || cost < least) {
+            least = cost;
+            best.segment = (int)(per * 32);
+            best.segments = (int)segments;
+        }
+    }
+    return best;
+}
 
-long long decay_state_bytes(int N, int head, int L, int dK4, int dV4) {
-    const int C = decay_chunk(dK4, dV4);
-    return (long long)N * head * ((L + C - 1) / C) * dK4 * dV4 * 4;
+long long decay_state_bytes(int N, int head, const DecayCut& cut, int dK4, int dV4) {
+    return cut.segments == 1 ? 0 : (long long)N * head * cut.segments * dK4 * dV4 * 4;
 }
 
 bool decay_arguments_ok(int N, int head, int L, int dK4, int dV4) {
     if (N <= 0 || head <= 0 || L <= 0 || dK4 <= 0 || dV4 <= 0 || (dK4 & 3) || (dV4 & 3) || dK4 > 128 || dV4 > 128) return false;
     const long long row = (long long)head * (dK4 > dV4 ? dK4 : dV4);
     // a tile's offsets are 32-bit bytes, positions 32-bit, a launch's workgroups 31 bits
-    return L < 0x7fffff00 && row * TQ * 4 < 0x7ffffff0LL && (long long)N * head * ((L + TQ - 1LL) / TQ) < 0x7fffffffLL &&
+    return L < 0x7fffff00 && row * 32 * 4 < 0x7ffffff0LL && (long long)N * head * 64 < 0x7fffffffLL &&
            (long long)N * head * dK4 * dV4 / 4 < 0x7fffffffLL * 128;
 }
 
 hipError_t launch_states(hipStream_t s, const float* A, MixLayout la, int ad, const float* B, MixLayout lb, int bd, const float* g,
-                         const int* lens, int N, int head, int L, int C, int back, float scale, float* U) {
-    DecayStates p = {A, B, la, lb, g, lens, head, L, ad, bd, C, (L + C - 1) / C, back, scale, U, N * head};
-    const dim3 grid((unsigned)((long long)N * head * p.chunks)), block(NTHREADS);
+                         const int* lens, int N, int head, int L, const DecayCut& cut, int back, float scale, float* U) {
+    DecayStates p = {A, B, la, lb, g, lens, head, L, ad, bd, cut.segment, cut.segments, back, scale, U, N * head};
+    const dim3 grid((unsigned)((long long)N * head * cut.segments)), block(NTHREADS);
     switch (((ad > bd ? ad : bd) + 31) / 32) {
         case 1: hipLaunchKernelGGL((decay_states<1, 1>), grid, block, 0, s, p); break;
         case 2: hipLaunchKernelGGL((decay_states<2, 2>), grid, block, 0, s, p); break;
@@ -389,22 +477,27 @@ hipError_t launch_states(hipStream_t s, const float* A, MixLayout la, int ad, co
 }
 
 hipError_t launch_scan(hipStream_t s, float* U, const float* first, float* last, const float* g, const int* lens, int N, int head,
-                       int L, int C, int back, int size) {
-    DecayScan p = {U, first, last, g, lens, head, L, C, (L + C - 1) / C, back, size / 4, (long long)N * head};
+                       int L, const DecayCut& cut, int back, int size) {
+    DecayScan p = {U, first, last, g, lens, head, L, cut.segment, cut.segments, back, size / 4, (long long)N * head};
     const long long items = p.nh * p.size4;
     hipLaunchKernelGGL(decay_scan, dim3((unsigned)((items + NTHREADS - 1) / NTHREADS)), dim3(NTHREADS), 0, s, p);
     return hipGetLastError();
 }
 
 template <bool ST>
-hipError_t launch_mix(hipStream_t s, const DecayParams& p, int N) {
-    const dim3 grid((unsigned)((long long)N * p.head * p.tiles)), block(NTHREADS);
-    switch (((p.xd > p.zd ? p.xd : p.zd) + 31) / 32) {
-        case 1: hipLaunchKernelGGL((decay_mix<1, 1, ST>), grid, block, 0, s, p); break;
-        case 2: hipLaunchKernelGGL((decay_mix<2, 2, ST>), grid, block, 0, s, p); break;
-        case 3: hipLaunchKernelGGL((decay_mix<4, 3, ST>), grid, block, 0, s, p); break;
-        default: hipLaunchKernelGGL((decay_mix<4, 4, ST>), grid, block, 0, s, p); break;
-    }
+hipError_t launch_walk(hipStream_t s, const DecayWalk& p) {
+    const dim3 grid((unsigned)((long long)p.nh * p.segments));
+    const int xb = (p.xd + 31) / 32, zb = (p.zd + 31) / 32;
+#define WALK(XB, ZB) hipLaunchKernelGGL((decay_walk<XB, ZB, ST>), grid, dim3(64 * ZB), 0, s, p)
+#define WALK_Z(XB)                                                                                     \
+    do {                                                                                               \
+        if (zb == 1) WALK(XB, 1); else if (zb == 2) WALK(XB, 2); else if (zb == 3) WALK(XB, 3); else WALK(XB, 4); \
+    } while (0)
+    if (xb == 1) WALK_Z(1);
+    else if (xb == 2) WALK_Z(2);
+    else WALK_Z(4);
+#undef WALK_Z
+#undef WALK
     return hipGetLastError();
 }
 
@@ -417,11 +510,11 @@ extern "C" {
 
 int64_t dragon_Cuda_linear_attention_bufsize(int32_t N, int32_t head, int32_t L, int32_t dK4, int32_t dV4) {
     if (!decay_arguments_ok(N, head, L, dK4, dV4)) return -1;
-    return L <= STEPS_MAX ? 0 : decay_state_bytes(N, head, L, dK4, dV4);
+    return L <= STEPS_MAX ? 0 : decay_state_bytes(N, head, decay_cut(N, head, L, dV4), dK4, dV4);
 }
 int64_t dragon_Cuda_linear_attention_backward_bufsize(int32_t N, int32_t head, int32_t L, int32_t dK4, int32_t dV4) {
     if (!decay_arguments_ok(N, head, L, dK4, dV4)) return -1;
-    return 2 * decay_state_bytes(N, head, L, dK4, dV4);
+    return 2 * decay_state_bytes(N, head, decay_cut(N, head, L, dK4 > dV4 ? dK4 : dV4), dK4, dV4);
 }
 
 int dragon_Cuda_linear_attention_forward(const int64_t* streams, int32_t length, int64_t dQ, int64_t dK, int64_t dV, int64_t dDecay,
@@ -450,16 +543,17 @@ int dragon_Cuda_linear_attention_forward(const int64_t* streams, int32_t length,
         hipLaunchKernelGGL(decay_steps, dim3((unsigned)((long long)N * head * p.slabs)), dim3(NTHREADS), 0, s, p);
         return hipGetLastError();
     }
-    const int C = decay_chunk(dK4, dV4), chunks = (L + C - 1) / C;
-    DecayParams p = {Q, K, V, Y, lk, lk, lv, lv, g, lens, head, L, dK4, dV4, C, chunks, 0, scale, scale, first, first == nullptr,
-                     (long long)state, 0, (L + TQ - 1) / TQ, N * head};
-    if (chunks > 1 || last != nullptr) {
-        hipError_t e = launch_states(s, K, lk, dK4, V, lv, dV4, g, lens, N, head, L, C, 0, 1.0f, U);
-        if (e == hipSuccess) e = launch_scan(s, U, first, last, g, lens, N, head, L, C, 0, (int)state);
+    const DecayCut cut = decay_cut(N, head, L, dV4);
+    DecayWalk p = {Q, K, V, Y, lk, lk, lv, lv, g, lens, head, L, dK4, dV4, cut.segment, cut.segments, 0, scale, scale, 1.0f,
+                   first, last, N * head};
+    if (cut.segments > 1) {
+        hipError_t e = launch_states(s, K, lk, dK4, V, lv, dV4, g, lens, N, head, L, cut, 0, 1.0f, U);
+        if (e == hipSuccess) e = launch_scan(s, U, first, last, g, lens, N, head, L, cut, 0, (int)state);
         if (e != hipSuccess) return e;
-        p.state = U; p.state_nh = (long long)chunks * state; p.state_c = (long long)state;
+        p.state = U;
+        p.last = nullptr;
     }
-    return launch_mix<false>(s, p, N);
+    return launch_walk<false>(s, p);
 }
 
 int dragon_Cuda_linear_attention_backward(const int64_t* streams, int32_t length, int64_t dQ, int64_t dK, int64_t dV, int64_t dDecay,
@@ -474,47 +568,47 @@ int dragon_Cuda_linear_attention_backward(const int64_t* streams, int32_t length
         !mix_aligned16(dDeltaState) || (dDecay & 3) || (dLens & 3))
         return hipErrorInvalidValue;
     if (!decay_arguments_ok(N, head, L, dK4, dV4) || !(scale - scale == 0.0f)) return hipErrorInvalidValue;
-    const long long need = 2 * decay_state_bytes(N, head, L, dK4, dV4);
-    if (dBuf == 0 || !mix_aligned16(dBuf) || buf_size < need) return hipErrorInvalidValue;
+    const DecayCut cut = decay_cut(N, head, L, dK4 > dV4 ? dK4 : dV4);
+    const long long need = 2 * decay_state_bytes(N, head, cut, dK4, dV4);
+    if (need > 0 && (dBuf == 0 || !mix_aligned16(dBuf) || buf_size < need)) return hipErrorInvalidValue;
     const float* Q = (const float*)(intptr_t)dQ; const float* K = (const float*)(intptr_t)dK; const float* V = (const float*)(intptr_t)dV;
     const float* G = (const float*)(intptr_t)dDeltaY; const float* g = (const float*)(intptr_t)dDecay;
     const float* first = (const float*)(intptr_t)dState; const float* dlast = (const float*)(intptr_t)dDeltaStateOut;
     float* gQ = (float*)(intptr_t)dDeltaQ; float* gK = (float*)(intptr_t)dDeltaK; float* gV = (float*)(intptr_t)dDeltaV;
     float* gfirst = (float*)(intptr_t)dDeltaState;
     const int* lens = (const int*)(intptr_t)dLens;
-    const int C = decay_chunk(dK4, dV4), chunks = (L + C - 1) / C;
     const long long state = (long long)dK4 * dV4;
-    float* S = (float*)(intptr_t)dBuf;
-    float* R = S + (size_t)N * head * chunks * state;
+    float* S = need > 0 ? (float*)(intptr_t)dBuf : nullptr;
+    float* R = need > 0 ? S + (size_t)N * head * cut.segments * state : nullptr;
     const MixLayout lk = mix_layout(head_inner, head, L, dK4), lv = mix_layout(head_inner, head, L, dV4);
     split_ledger_touch(gQ, (size_t)N * head * L * dK4 * 4);
     split_ledger_touch(gK, (size_t)N * head * L * dK4 * 4);
     split_ledger_touch(gV, (size_t)N * head * L * dV4 * 4);
     if (gfirst != nullptr) split_ledger_touch(gfirst, (size_t)N * head * state * 4);
-    split_ledger_touch(S, (size_t)need);
+    if (need > 0) split_ledger_touch(S, (size_t)need);
     hipStream_t s = (hipStream_t)(intptr_t)streams[0];
-    const bool many = chunks > 1;
+    const float* before = first;       // what the segments begin with, and end with
+    const float* behind = dlast;
     hipError_t e = hipSuccess;
-    if (many) {
-        e = launch_states(s, K, lk, dK4, V, lv, dV4, g, lens, N, head, L, C, 0, 1.0f, S);
-        if (e == hipSuccess) e = launch_scan(s, S, first, nullptr, g, lens, N, head, L, C, 0, (int)state);
+    if (cut.segments > 1) {
+        e = launch_states(s, K, lk, dK4, V, lv, dV4, g, lens, N, head, L, cut, 0, 1.0f, S);
+        if (e == hipSuccess) e = launch_scan(s, S, first, nullptr, g, lens, N, head, L, cut, 0, (int)state);
+        if (e == hipSuccess) e = launch_states(s, Q, lk, dK4, G, lv, dV4, g, lens, N, head, L, cut, 1, scale, R);
+        if (e == hipSuccess) e = launch_scan(s, R, dlast, gfirst, g, lens, N, head, L, cut, 1, (int)state);
+        if (e != hipSuccess) return e;
+        before = S;
+        behind = R;
     }
-    const bool later = many || gfirst != nullptr;
-    if (later) {
-        if (e == hipSuccess) e = launch_states(s, Q, lk, dK4, G, lv, dV4, g, lens, N, head, L, C, 1, scale, R);
-        if (e == hipSuccess) e = launch_scan(s, R, dlast, gfirst, g, lens, N, head, L, C, 1, (int)state);
-    }
-    if (e != hipSuccess) return e;
-    DecayParams p = {G, V, K, gQ, lv, lv, lk, lk, g, lens, head, L, dV4, dK4, C, chunks, 0, scale, scale,
-                     many ? S : first, first == nullptr, many ? chunks * state : state, many ? state : 0, (L + TQ - 1) / TQ, N * head};
-    e = launch_mix<true>(s, p, N);
-    p.back = 1; p.far_scale = 1.0f;
-    p.state = later ? R : dlast; p.empty_first = dlast == nullptr;
-    p.state_nh = later ? chunks * state : state; p.state_c = later ? state : 0;
+    DecayWalk p = {G, V, K, gQ, lv, lv, lk, lk, g, lens, head, L, dV4, dK4, cut.segment, cut.segments, 0, scale, scale, 1.0f,
+                   before, nullptr, N * head};
+    e = launch_walk<true>(s, p);
+    p.back = 1; p.far_scale = 1.0f; p.add_scale = scale;
+    p.state = behind;
     p.x = V; p.y = G; p.z = Q; p.out = gK;
-    if (e == hipSuccess) e = launch_mix<true>(s, p, N);
+    if (e == hipSuccess) e = launch_walk<true>(s, p);
     p.x = K; p.y = Q; p.z = G; p.out = gV; p.lx = p.ly = lk; p.lz = p.lo = lv; p.xd = dK4; p.zd = dV4;
-    if (e == hipSuccess) e = launch_mix<false>(s, p, N);
+    p.last = cut.segments == 1 ? gfirst : nullptr;
+    if (e == hipSuccess) e = launch_walk<false>(s, p);
     return e;
 }
 

@@ -44,20 +44,20 @@ __device__ __forceinline__ void mix_wait() { __builtin_amdgcn_s_waitcnt(waitcnt_
 // them and chunks beyond the row's d4 floats arrive as zeros.  Everything but the offsets has to be uniform.
 template <int DW, int ROWS, bool SWIZZLE, int THREADS = NTHREADS>
 struct MixTile {
-    static constexpr int CPR = DW / 4, RPP = THREADS / CPR < ROWS ? THREADS / CPR : ROWS, PASSES = ROWS / RPP;
-    static_assert(PASSES * RPP == ROWS && PASSES >= 1, "the tile divides over the workgroup");
+    static constexpr int CPR = DW / 4, WAVES = THREADS / 64, BLOCKS = ROWS * DW / 256;   // blocks of 1 KiB, one transfer each
+    static constexpr int PASSES = (BLOCKS + WAVES - 1) / WAVES;
+    static constexpr bool EVEN = BLOCKS % WAVES == 0;
     int off[PASSES];
     __device__ __forceinline__ void init(int t, int pitch, int d4) {
-        const int slot = t % CPR, row0 = t / CPR;
 #pragma unroll
         for (int s = 0; s < PASSES; s++) {
-            const int row = row0 + s * RPP, chunk = SWIZZLE ? (slot ^ kin_swizzle<DW>(row)) : slot;
+            const int at = s * THREADS + t, row = at / CPR, slot = at % CPR, chunk = SWIZZLE ? (slot ^ kin_swizzle<DW>(row)) : slot;
             off[s] = chunk * 4 < d4 ? (row * pitch + chunk * 4) * 4 : OOB_OFFSET;
         }
     }
-    // rows [0, left) of the tile that starts at `base` into the LDS tile whose address for this wavefront is `lds`
+    // rows [0, left) of the tile that starts at `base` into the LDS tile whose address for wavefront `wave` is `lds`
     // (mix_lds of the tile + 1024 * wavefront); left < 1: zeros
-    __device__ __forceinline__ void fetch(const float* base, int left, int pitch, unsigned lds) const {
+    __device__ __forceinline__ void fetch(const float* base, int left, int pitch, unsigned lds, int wave = 0) const {
         const int rows = left < 0 ? 0 : (left < ROWS ? left : ROWS);
         const unsigned long long b = (unsigned long long)base;
         const v4u rsrc = {(unsigned)mix_uniform((int)b), (unsigned)mix_uniform((int)(b >> 32)) & 0xffffu,
@@ -65,7 +65,7 @@ struct MixTile {
         const unsigned to = (unsigned)mix_uniform((int)lds);
         static_for<PASSES>([&](auto sc) {
             constexpr int s = decltype(sc)::value;
-            dma_f4_lean<s * THREADS * 16>(rsrc, to, off[s]);
+            if (EVEN || s * WAVES + wave < BLOCKS) dma_f4_lean<s * THREADS * 16>(rsrc, to, off[s]);
         });
     }
 };
@@ -96,7 +96,7 @@ __device__ __forceinline__ void mix_rows_product(v16f& s, const float* tile, con
 #pragma unroll
     for (int g = 0; g < NG; g++) {
         typedef const __attribute__((address_space(3))) v4f* lds_v4f;
-        const v4f a = *(lds_v4f)((at ^ (32 * (g & 7))) + 256 * (g >> 3));
+        const v4f a = *(lds_v4f)(size_t)((at ^ (32 * (g & 7))) + 256 * (g >> 3));
         s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, cols[g].x, s, 0, 0, 0);
         s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, cols[g].y, s, 0, 0, 0);
         s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, cols[g].z, s, 0, 0, 0);

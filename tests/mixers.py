@@ -203,7 +203,7 @@ def run_decay(dh, Q, K, V, g, scale, lens=None, S0=None, dY=None, dS1=None, head
         gy = dh.DeviceArray(outer(dY, head_inner))
         d1 = dh.DeviceArray(dS1) if dS1 is not None else None
         need = A.backward_bufsize(*sizes)
-        buf2 = filled(dh, need // 4)
+        buf2 = filled(dh, max(need // 4, 4))
         dq, dk_, dv_ = filled(dh, q.size), filled(dh, k.size), filled(dh, v.size)
         d0 = filled(dh, N * H * dk * dv) if want_state else None
         dh.Cuda.deviceSynchronize()
