@@ -439,7 +439,7 @@ int dragon_Cuda_attention_window_forward(const int64_t* streams, int32_t length,
         const dim3 grid((unsigned)((long long)N * head * plan.qtiles * plan.parts));
         switch ((dmax + 31) / 32) {
             case 1: hipLaunchKernelGGL((window_tiles<1, 1, 2>), grid, block, 0, s, p); break;
-            case 2: hipLaunchKernelGGL((window_tiles<2, 2, 2>), grid, block, 0, s, p); break;
+            case 2: hipLaunchKernelGGL((window_tiles<2, 2, 1>), grid, block, 0, s, p); break;
             case 3: hipLaunchKernelGGL((window_tiles<4, 3, 1>), grid, block, 0, s, p); break;
             default: hipLaunchKernelGGL((window_tiles<4, 4, 1>), grid, block, 0, s, p); break;
         }

@@ -35,16 +35,21 @@ struct WindowGrad {
     int snap;                // steps that a cut through a tile costs (two beginnings and ends, a piece written and read)
     long long* before;       // [N * ktiles + 1]: the steps of all key tiles before this one, of one key / value head
     float* pieces;           // [2 * workers][128][dk4 + dv4]
+    int2* cut;               // [N * ktiles, kv_head]: the workers of a tile's first and last piece
+    int sink_blocks;         // 16 keys each; 0: the sinks' tiles walk over all queries like the others
+    int sink_parts;          // SINK_QUERIES queries each
+    float* sinks;            // [N, kv_head][sink_blocks][sink_parts][16][dk4 + dv4]
 };
 
 // ---------------------------------------------------------------- what the products start from, and the work to deal
 // the queries that see a key of tile `tile`: [lo, hi)
 struct WindowQueries { int lo, hi; };
-__device__ __forceinline__ WindowQueries window_queries(const WindowParams& p, int tile, WindowLens len) {
+__device__ __forceinline__ WindowQueries window_queries(const WindowGrad& a, int tile, WindowLens len) {
+    const WindowParams& p = a.w;
     const int k0 = tile * GK, k1 = min(k0 + GK, len.vl), off = len.vl - len.ql;
     WindowQueries x;
     x.lo = max(k0 - off, 0);
-    x.hi = k0 < k1 ? (k0 < p.sinks ? len.ql : min(len.ql, k1 - 1 + p.window - off)) : 0;
+    x.hi = k0 < k1 ? (k0 < p.sinks && a.sink_blocks == 0 ? len.ql : min(len.ql, k1 - 1 + p.window - off)) : 0;
     return x;
 }
 // steps of `per` queries of one query head
@@ -63,7 +68,7 @@ __global__ __launch_bounds__(NTHREADS) void window_delta(const WindowGrad a) {
             if (x < tiles) {
                 const int n = (int)(x / a.ktiles);
                 const WindowLens len = {p.QLens ? min(max(p.QLens[n], 0), p.QL) : p.QL, p.VLens ? min(max(p.VLens[n], 0), p.VL) : p.VL};
-                own = (long long)window_steps(window_queries(p, (int)(x - (long long)n * a.ktiles), len), 32) * group;
+                own = (long long)window_steps(window_queries(a, (int)(x - (long long)n * a.ktiles), len), 32) * group;
             }
             sum[t] = own;
             __syncthreads();
@@ -229,8 +234,8 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_q(const Window
 }
 
 // ---------------------------------------------------------------- dK, dV
-// A key tile is seen by window + 128 queries of every head of the group, one with sinks by all behind it, the last ones
-// under no window by few: the tiles differ by whatever the sequence is long.  So the steps of all tiles are counted through
+// A key tile is seen by window + 128 queries of every head of the group, the last ones and those under no window by fewer or
+// by more (and a tile of many sinks by all behind it): the tiles differ by whatever the sequence is long.  So the steps of all tiles are counted through
 // (before) and dealt to the workgroups in equal runs.  Where a run begins or ends inside a tile the workgroup leaves its sums
 // as a piece and window_grad_join adds the tile's pieces in order.
 struct GradDeal { long long total; long long workers; };
@@ -268,14 +273,6 @@ __device__ __forceinline__ long long grad_begin(const WindowGrad& a, const GradD
     const int in = (int)((pos - tile.at) % tile.steps), snap = (int)min((long long)a.snap, d.total / d.workers / 2);
     return in <= snap ? pos - in : tile.steps - in <= snap ? pos + tile.steps - in : pos;
 }
-// the worker whose run holds step pos
-__device__ __forceinline__ long long grad_worker(const WindowGrad& a, const GradDeal& d, long long pos) {
-    long long w = min(pos / max(d.total / d.workers, 1LL), d.workers - 1);
-    while (w + 1 < d.workers && grad_begin(a, d, w + 1) <= pos) w++;
-    while (w > 0 && grad_begin(a, d, w) > pos) w--;
-    return w;
-}
-
 // the kernel's arguments, as if they had just been passed
 __device__ __forceinline__ const WindowGrad& anew(const WindowGrad&) {
     auto at = (const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr();
@@ -325,7 +322,7 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_kv(const Windo
         pos += last - first;
         const int n = mix_uniform((int)(at / a.ktiles)), tile = mix_uniform((int)(at - (long long)n * a.ktiles));
         const WindowLens len = window_lens(p, n);
-        const WindowQueries qs = window_queries(p, tile, len);
+        const WindowQueries qs = window_queries(a, tile, len);
         const int lo = qs.lo, hi = qs.hi, per_head = window_steps(qs, 32), off = len.vl - len.ql;
         const int u0 = tile * GK + block * 32, u1 = min(u0 + 32, len.vl) - 1;      // the wavefront's keys
         const int key = u0 + r;
@@ -428,6 +425,11 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_kv(const Windo
             if (i0 >= hi) i0 = lo;
         }
         const WindowGrad& b = anew(arg);
+        if (t == 0) {
+            int2* cut = b.cut + at * b.w.kv_head + kvh;
+            if (first == 0) cut->x = blockIdx.x;
+            if (last == all) cut->y = blockIdx.x;
+        }
         float* out;
         if (first == 0 && last == all) {
             out = second ? b.dK + n * b.w.k.n + kvh * b.w.k.h + (size_t)key * b.w.k.l : b.dV + n * b.w.v.n + kvh * b.w.v.h + (size_t)key * b.w.v.l;
@@ -439,45 +441,171 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_kv(const Windo
     }
 }
 
-// four workgroups per tile and key / value head: the tile's pieces in order; zeros where no query sees it
+// ---------------------------------------------------------------- dK, dV of the sinks
+// What the queries beyond a sink's window leave there: all of them, for a few keys, so the reading of Q and dY bounds it and
+// not the products.  16 keys a workgroup, SINK_QUERIES queries of every head of the group, 16 at a time per wavefront, with
+// v_mfma_f32_16x16x4_f32 and the register layouts of window_rows (queries and keys changed about): a lane reads a query's row
+// once in pieces for the scores and once as the columns of the sums.  (In tiles of 128 keys like the rest, three of four
+// wavefronts have nothing to do: at 4 sinks and 8192 queries a tenth of window_grad_kv's steps.)
+constexpr int SINK_QUERIES = 128;
+template <int DE>
+__global__ __launch_bounds__(NTHREADS, 2) void window_grad_sinks(const WindowGrad a) {
+    constexpr int NS = DE * 4;
+    const WindowParams& p = a.w;
+    __shared__ __attribute__((aligned(16))) float So[4][16][DE * 64 + 4];
+    const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), c = lane & 15, k4 = lane >> 4;
+    const int nkv = p.N * p.kv_head, group = p.head / p.kv_head;
+    const int x = mix_uniform(blockIdx.x / nkv), kv = blockIdx.x - x * nkv;
+    const int part = mix_uniform(x / a.sink_blocks), block = x - part * a.sink_blocks;
+    const int n = mix_uniform(kv / p.kv_head), kvh = kv - n * p.kv_head;
+    const WindowLens len = window_lens(p, n);
+    const int key = block * 16 + c, keys = min(p.sinks, len.vl);
+    const bool live = key < keys;
+    // behind the queries that the tile of 128 keys walks over (none of them where they all lie beyond its window: hi < 0)
+    const int lo = max(window_queries(a, block * 16 / GK, len).hi, 0) + part * SINK_QUERIES;
+    const int hi = block * 16 < keys ? min(lo + SINK_QUERIES, len.ql) : 0;
+
+    v4f kf[NS], vf[NS];
+    const float* krow = p.K + n * p.k.n + kvh * p.k.h + (size_t)min(key, p.VL - 1) * p.k.l;
+    const float* vrow = p.V + n * p.v.n + kvh * p.v.h + (size_t)min(key, p.VL - 1) * p.v.l;
+    int qa[NS], ga[NS], qc[4 * DE], gc[4 * DE];               // byte offsets inside 16 rows
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+        const int d = 16 * s + 4 * k4;
+        kf[s] = (live && d < p.dk4) ? *(const v4f*)(krow + d) * p.c : (v4f)(0.0f);
+        vf[s] = (live && d < p.dv4) ? *(const v4f*)(vrow + d) : (v4f)(0.0f);
+        qa[s] = d < p.dk4 ? (c * p.q.l + d) * 4 : OOB_OFFSET;
+        ga[s] = d < p.dv4 ? (c * p.y.l + d) * 4 : OOB_OFFSET;
+    }
+#pragma unroll
+    for (int v = 0; v < 4; v++)
+#pragma unroll
+        for (int e = 0; e < DE; e++) {
+            const int d = 64 * e + 4 * c;
+            qc[v * DE + e] = d < p.dk4 ? ((4 * k4 + v) * p.q.l + d) * 4 : OOB_OFFSET;
+            gc[v * DE + e] = d < p.dv4 ? ((4 * k4 + v) * p.y.l + d) * 4 : OOB_OFFSET;
+        }
+    v4f dk[DE][4], dv[DE][4];
+#pragma unroll
+    for (int e = 0; e < DE; e++)
+#pragma unroll
+        for (int u = 0; u < 4; u++) dk[e][u] = dv[e][u] = (v4f)(0.0f);
+    for (int g = 0; g < group; g++) {
+        const int hd = kvh * group + g;
+        const float* qb = p.Q + n * p.q.n + hd * p.q.h;
+        const float* gb = a.dY + n * p.y.n + hd * p.y.h;
+        const float* sb = a.stats + ((size_t)n * p.head + hd) * p.QL;
+        for (int i0 = lo + 16 * wave; i0 < hi; i0 += 64) {
+            const int left = min(hi - i0, 16);
+            const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc((void*)(qb + (size_t)i0 * p.q.l), 0, left * p.q.l * 4, RSRC_FLAGS);
+            const __amdgpu_buffer_rsrc_t rg = __builtin_amdgcn_make_buffer_rsrc((void*)(gb + (size_t)i0 * p.y.l), 0, left * p.y.l * 4, RSRC_FLAGS);
+            const __amdgpu_buffer_rsrc_t rl = __builtin_amdgcn_make_buffer_rsrc((void*)(sb + i0), 0, left * 4, RSRC_FLAGS);
+            const __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc((void*)(sb + a.rows + i0), 0, left * 4, RSRC_FLAGS);
+            v4f s = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rl, 16 * k4, 0, 0));
+            v4f d = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rd, 16 * k4, 0, 0));
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+                const v4f q = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rq, qa[i], 0, 0));
+                const v4f y = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rg, ga[i], 0, 0));
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    s = __builtin_amdgcn_mfma_f32_16x16x4f32(q[u], kf[i][u], s, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_f32_16x16x4f32(y[u], vf[i][u], d, 0, 0, 0);
+                }
+            }
+            // register v: query i0 + 4 * k4 + v
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                const bool on = live && 4 * k4 + v < left;
+                s[v] = on ? __builtin_amdgcn_exp2f(s[v]) : 0.0f;
+                d[v] = on ? s[v] * d[v] : 0.0f;
+            }
+#pragma unroll
+            for (int v = 0; v < 4; v++)
+#pragma unroll
+                for (int e = 0; e < DE; e++) {
+                    const v4f y = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rg, gc[v * DE + e], 0, 0));
+                    const v4f q = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rq, qc[v * DE + e], 0, 0));
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        dv[e][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(y[u], s[v], dv[e][u], 0, 0, 0);
+                        dk[e][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(q[u], d[v], dk[e][u], 0, 0, 0);
+                    }
+                }
+        }
+    }
+    // the wavefronts' sums, added through LDS; register w of block (e, u) is float 64e + 16*k4 + 4w + u of key c
+    float* out = a.sinks + (((size_t)kv * a.sink_blocks + block) * a.sink_parts + part) * 16 * (p.dk4 + p.dv4);
+    auto join = [&](const v4f (&o)[DE][4], int at, int d4, float f) {
+#pragma unroll
+        for (int e = 0; e < DE; e++)
+#pragma unroll
+            for (int w = 0; w < 4; w++)
+                *(v4f*)&So[wave][c][64 * e + 16 * k4 + 4 * w] = (v4f){o[e][0][w], o[e][1][w], o[e][2][w], o[e][3][w]};
+        __syncthreads();
+        for (int i = t; i < 4 * d4; i += NTHREADS) {
+            const int row = i / (d4 / 4), d = 4 * (i - row * (d4 / 4));
+            const v4f sum = (*(const v4f*)&So[0][row][d] + *(const v4f*)&So[1][row][d]) + (*(const v4f*)&So[2][row][d] + *(const v4f*)&So[3][row][d]);
+            *(v4f*)(out + (size_t)row * (p.dk4 + p.dv4) + at + d) = sum * f;
+        }
+        __syncthreads();
+    };
+    join(dk, 0, p.dk4, a.scale);
+    join(dv, p.dk4, p.dv4, 1.0f);
+}
+
+// ---------------------------------------------------------------- everything that a key's gradient is made of
+// Four workgroups per tile and key / value head: the tile's pieces in order, or what was written whole, or zeros where no
+// query sees it; then the sinks' parts in order.
 __global__ __launch_bounds__(NTHREADS) void window_grad_join(const WindowGrad a) {
     const WindowParams& p = a.w;
     const long long at = blockIdx.x / p.kv_head;
     const int kvh = (int)(blockIdx.x - at * p.kv_head), n = (int)(at / a.ktiles), k0 = (int)(at - (long long)n * a.ktiles) * GK;
-    const GradDeal deal = grad_deal(a);
-    const GradTile tile = grad_tile(a, at);
-    const long long begin = tile.at + (long long)kvh * tile.steps, end = begin + tile.steps;
-    long long w0 = 0, w1 = 0;
-    if (tile.steps > 0) {
-        w0 = grad_worker(a, deal, begin);
-        w1 = grad_worker(a, deal, end - 1);
-        if (w0 == w1) return;                                           // written whole
-    }
+    const bool some = a.before[at + 1] != a.before[at];
+    const int2 cut = some ? a.cut[at * p.kv_head + kvh] : make_int2(0, 0);
+    const bool whole = some && cut.x == cut.y;
+    if (whole && k0 >= a.sink_blocks * 16) return;
     const int width = p.dk4 + p.dv4, per = width / 4;
-#pragma unroll 4
     for (int x = threadIdx.x; x < GK / 4 * per; x += NTHREADS) {
         const int in = x / per, row = blockIdx.y * (GK / 4) + in, d = 4 * (x - in * per), key = k0 + row;
-        if (key >= p.VL) break;
+        if (key >= p.VL || (whole && key >= a.sink_blocks * 16)) break;
+        float* out = d < p.dk4 ? a.dK + n * p.k.n + kvh * p.k.h + (size_t)key * p.k.l + d
+                               : a.dV + n * p.v.n + kvh * p.v.h + (size_t)key * p.v.l + d - p.dk4;
         v4f s = (v4f)(0.0f);
-        if (tile.steps > 0) {
-            s = *(const v4f*)(a.pieces + ((2 * (size_t)w0 + 1) * GK + row) * width + d);
-            for (long long w = w0 + 1; w <= w1; w++) s += *(const v4f*)(a.pieces + (2 * (size_t)w * GK + row) * width + d);
+        if (whole) {
+            s = *(const v4f*)out;
+        } else if (some) {
+            s = *(const v4f*)(a.pieces + ((2 * (size_t)cut.x + 1) * GK + row) * width + d);
+#pragma unroll 4
+            for (int w = cut.x + 1; w <= cut.y; w++) s += *(const v4f*)(a.pieces + (2 * (size_t)w * GK + row) * width + d);
         }
-        if (d < p.dk4) *(v4f*)(a.dK + n * p.k.n + kvh * p.k.h + (size_t)key * p.k.l + d) = s;
-        else *(v4f*)(a.dV + n * p.v.n + kvh * p.v.h + (size_t)key * p.v.l + d - p.dk4) = s;
+        if (key < a.sink_blocks * 16) {
+            const int block = key / 16;
+            const float* parts = a.sinks + (((size_t)(n * p.kv_head + kvh) * a.sink_blocks + block) * a.sink_parts * 16 + (key - block * 16)) * width + d;
+#pragma unroll 8
+            for (int i = 0; i < a.sink_parts; i++) s += *(const v4f*)(parts + (size_t)i * 16 * width);
+        }
+        *(v4f*)out = s;
     }
 }
 
 // ---------------------------------------------------------------- host side
-// The caller's buffer, in floats: the statistics, the running sum (64-bit), the pieces.
-struct WindowGradBuffer { int ktiles, workers; long long stats, before, pieces; };
-WindowGradBuffer window_grad_buffer(int N, int head, int QL, int VL, int dk4, int dv4) {
+// The caller's buffer, in floats: the statistics, the running sum (64-bit), the pieces and whose they are, the sinks' parts.
+constexpr int SINKS_APART = 64;      // up to here window_grad_sinks takes the queries beyond the window
+struct WindowGradBuffer { int ktiles, workers, sink_blocks, sink_parts; long long stats, before, pieces, cut, sinks, all; };
+WindowGradBuffer window_grad_buffer(int N, int head, int kv_head, int QL, int VL, int dk4, int dv4, int window, int sinks) {
     WindowGradBuffer b;
     b.ktiles = (VL + GK - 1) / GK;
-    b.workers = (dk4 > dv4 ? dk4 : dv4) > 64 ? 256 : 512;                                                  // one for each compute unit: their LDS holds no two
+    b.workers = (dk4 > dv4 ? dk4 : dv4) > 64 ? 256 : 512;             // as many as the compute units hold
+    const bool apart = window != 0 && window < VL && sinks > 0 && sinks <= SINKS_APART;
+    b.sink_blocks = apart ? ((sinks < VL ? sinks : VL) + 15) / 16 : 0;
+    b.sink_parts = apart ? (QL + SINK_QUERIES - 1) / SINK_QUERIES : 0;
     b.stats = (2LL * N * head * QL + 3) / 4 * 4;
     b.before = (((long long)N * b.ktiles + 1) * 2 + 3) / 4 * 4;
     b.pieces = 2LL * b.workers * GK * (dk4 + dv4);
+    b.cut = ((long long)N * b.ktiles * kv_head * 2 + 3) / 4 * 4;
+    b.sinks = (long long)N * kv_head * b.sink_blocks * b.sink_parts * 16 * (dk4 + dv4);
+    b.all = b.stats + b.before + b.pieces + b.cut + b.sinks;
     return b;
 }
 
@@ -491,8 +619,7 @@ extern "C" {
 int64_t dragon_Cuda_attention_window_backward_bufsize(int32_t N, int32_t head, int32_t kv_head, int32_t QL, int32_t VL, int32_t dK4,
                                                       int32_t dV4, int32_t window, int32_t sinks) {
     if (!window_arguments_ok(N, head, kv_head, QL, VL, dK4, dV4, window, sinks)) return -1;
-    const WindowGradBuffer b = window_grad_buffer(N, head, QL, VL, dK4, dV4);
-    return (b.stats + b.before + b.pieces) * 4;
+    return window_grad_buffer(N, head, kv_head, QL, VL, dK4, dV4, window, sinks).all * 4;
 }
 
 int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length, int64_t dQ, int64_t dK, int64_t dV, int64_t dY,
@@ -507,8 +634,8 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
         return hipErrorInvalidValue;
     if (!window_arguments_ok(N, head, kv_head, QL, VL, dK4, dV4, window, sinks) || !(scale - scale == 0.0f))
         return hipErrorInvalidValue;
-    const WindowGradBuffer b = window_grad_buffer(N, head, QL, VL, dK4, dV4);
-    const long long need = (b.stats + b.before + b.pieces) * 4;
+    const WindowGradBuffer b = window_grad_buffer(N, head, kv_head, QL, VL, dK4, dV4, window, sinks);
+    const long long need = b.all * 4;
     if (dBuf == 0 || !mix_aligned16(dBuf) || buf_size < need) return hipErrorInvalidValue;
 
     WindowGrad a;
@@ -532,6 +659,9 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
     a.snap = 2;
     a.before = (long long*)(a.stats + b.stats);
     a.pieces = a.stats + b.stats + b.before;
+    a.cut = (int2*)(a.pieces + b.pieces);
+    a.sinks = a.pieces + b.pieces + b.cut;
+    a.sink_blocks = b.sink_blocks; a.sink_parts = b.sink_parts;
     split_ledger_touch(a.dQ, (size_t)N * head * QL * dK4 * 4);
     split_ledger_touch(a.dK, (size_t)N * kv_head * VL * dK4 * 4);
     split_ledger_touch(a.dV, (size_t)N * kv_head * VL * dV4 * 4);
@@ -560,6 +690,13 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
         default: GRAD_CASE(4, 4, 1); break;
     }
 #undef GRAD_CASE
+    if (b.sink_blocks > 0) {
+        const dim3 gs((unsigned)((long long)N * kv_head * b.sink_blocks * b.sink_parts));
+        if (dmax <= 64) hipLaunchKernelGGL(window_grad_sinks<1>, gs, block, 0, s, a);
+        else hipLaunchKernelGGL(window_grad_sinks<2>, gs, block, 0, s, a);
+        e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
     hipLaunchKernelGGL(window_grad_join, dim3((unsigned)((long long)N * b.ktiles * kv_head), 4), block, 0, s, a);
     e = hipGetLastError();
     return e;

@@ -348,14 +348,21 @@ __global__ __launch_bounds__(NTHREADS) void decay_scan(const DecayScan p) {
     const float whole = decay_pow(g2, p.segment), tail = decay_pow(g2, len - (used - 1) * p.segment);
     v4f* U = (v4f*)p.U + (size_t)nh * p.segments * p.size4 + e;
     v4f s = p.first ? ((const v4f*)p.first)[nh * p.size4 + e] : (v4f)(0.0f);
-    v4f next = (v4f)(0.0f);
-    if (used > 0) next = U[(size_t)(p.back ? used - 1 : 0) * p.size4];
-    for (int k = 0; k < used; k++) {
-        const int c = p.back ? used - 1 - k : k;
-        const v4f u = next;
-        if (k + 1 < used) next = U[(size_t)(p.back ? c - 1 : c + 1) * p.size4];
-        U[(size_t)c * p.size4] = s;
-        s = s * (c == used - 1 ? tail : whole) + u;
+    constexpr int AHEAD = 8;       // loads in flight: each would otherwise wait for the one before
+    for (int k0 = 0; k0 < used; k0 += AHEAD) {
+        v4f u[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const int k = min(k0 + i, used - 1);
+            u[i] = U[(size_t)(p.back ? used - 1 - k : k) * p.size4];
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            if (k0 + i >= used) break;
+            const int c = p.back ? used - 1 - (k0 + i) : k0 + i;
+            U[(size_t)c * p.size4] = s;
+            s = s * (c == used - 1 ? tail : whole) + u[i];
+        }
     }
     if (p.last) ((v4f*)p.last)[nh * p.size4 + e] = s;
 }
