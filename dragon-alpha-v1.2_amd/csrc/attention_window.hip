@@ -6,7 +6,7 @@
 // A row that sees nothing (also the rows behind a sequence's queries) is zeros with lse = -infinity.
 //
 // Two kernels, chosen by the number of queries:
-//   window_tiles: 128 queries of one head per workgroup, the keys they see in steps, S^T = K.Q^T and Y^T = V^T.P^T with
+//   window_tiles: 128 (query, head) rows of one key / value head per workgroup, the keys they see in steps, S^T = K.Q^T and Y^T = V^T.P^T with
 //     v_mfma_f32_32x32x2_f32 and a running maximum and sum per query (token_mixer.h has the register layouts).  The steps
 //     are the sinks below the window's reach, then the keys from the first one that some query of the tile sees: no other
 //     key is read.  Bound by the FP32 matrix pipe.
@@ -17,12 +17,13 @@
 #include "token_mixer.h"
 #include "attention_window.h"
 #include "runtime_internal.h"
+#include "stream_policy.h"
 #include "../../include/dragon_hip_gemm.h"
 
 namespace dragon {
 namespace {
 
-constexpr int AQ = 128;          // queries per workgroup of the tiled kernel: 32 per wavefront
+constexpr int AQ = 128;          // rows per workgroup of the tiled kernel: 32 per wavefront
 constexpr int LAG = 8;           // the reference maximum may lag the true one by 2^LAG
 constexpr float NEG = -__builtin_inff();
 constexpr float LOWEST = -3.0e38f;   // below every score that is not -infinity
@@ -37,25 +38,23 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p
     const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
     const WindowJob job = window_job(p, blockIdx.x);
     const WindowLens len = window_lens(p, job.n);
-    const int q0 = job.qt * AQ;
-    const int i = q0 + wave * 32 + r;                       // this lane's query
-    float* Yb = p.Y + job.n * p.y.n + job.hd * p.y.h;
-    const size_t stat = ((size_t)job.n * p.head + job.hd) * p.QL;
+    const int group = p.head / p.kv_head, off = len.vl - len.ql;
+    // where a tile has fewer than 128 rows, the parts of its keys leave other wavefronts (and SIMDs) without work
+    const int row0 = job.qt * AQ, wrow = row0 + 32 * ((wave + job.part) & 3);
+    const WindowRow row = window_row(p, job, wrow + r, group, len.ql);
+    const size_t stat = ((size_t)job.n * p.head + row.hd) * p.QL + row.i;
 
-    // the keys that the tile's queries see: [0, sink_end) and [low, hi)
-    const int qn = min(q0 + AQ, len.ql);                    // the tile's queries end here
-    const int off = len.vl - len.ql;
-    const WindowRange range = window_range(p, q0 + off, qn - 1 + off, q0 < qn, len.vl);
+    // the keys that the tile's rows see: [0, sink_end) and [low, hi)
+    const WindowSpan all = window_span(row0, AQ, group, len.ql, off), span = window_span(wrow, 32, group, len.ql, off);
+    const WindowRange range = window_range(p, all.first, all.last, all.first <= all.last, len.vl);
     const int nsink = (range.sink_end + AK - 1) / AK, nwin = (max(range.hi - range.low, 0) + AK - 1) / AK;
     const int first = mix_uniform((int)((long long)(nsink + nwin) * job.part / p.parts));
     const int last = mix_uniform((int)((long long)(nsink + nwin) * (job.part + 1) / p.parts));
-
-    const bool live = i < len.ql;
-    const int pos = live ? i + off : -1;
-    const int w0 = q0 + wave * 32 + off, w1 = min(q0 + wave * 32 + 32, len.ql) - 1 + off;   // the wavefront's positions
+    const int pos = row.live ? row.i + off : -1;
+    const int w0 = span.first, w1 = span.last;              // the wavefront's positions
 
     v4f qf[NG];
-    mix_load_cols<NG>(qf, p.Q + job.n * p.q.n + job.hd * p.q.h + (size_t)min(i, p.QL - 1) * p.q.l, live, p.dk4, h);
+    mix_load_cols<NG>(qf, p.Q + job.n * p.q.n + row.hd * p.q.h + (size_t)row.i * p.q.l, row.live, p.dk4, h);
 #pragma unroll
     for (int g = 0; g < NG; g++) qf[g] *= p.c;              // scores in units of log2
 
@@ -102,7 +101,7 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p
                 mix_rows_product<DW, NG>(sc[kb], Ks[buf] + kb * 32 * DW, qf, r, h);
             }
             // keys behind a query (or behind the last key), and before its window: tested only where some query has them
-            if (key0 + AK - 1 > w0 || key0 + AK > limit || q0 + wave * 32 + 32 > len.ql) {
+            if (key0 + AK - 1 > w0 || key0 + AK > limit || !span.full) {
                 const int top = min(pos, limit - 1) - key0 - 4 * h;
 #pragma unroll
                 for (int kb = 0; kb < KB; kb++)
@@ -162,14 +161,13 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p
     const MixHalves sums = mix_halves(l);
     l = sums.a + sums.b;
     const float m = raise == LOWEST ? NEG : -from[0];
-    if (i >= p.QL) return;
+    if (!row.exists) return;
     if (p.parts == 1) {
-        mix_store_row<DC>(Yb + (size_t)i * p.y.l, o, l == 0.0f ? 0.0f : 1.0f / l, p.dv4, h);
-        if (p.Lse != nullptr && h == 0) p.Lse[stat + i] = window_lse(m, l);
+        mix_store_row<DC>(p.Y + job.n * p.y.n + row.hd * p.y.h + (size_t)row.i * p.y.l, o, l == 0.0f ? 0.0f : 1.0f / l, p.dv4, h);
+        if (p.Lse != nullptr && h == 0) p.Lse[stat] = window_lse(m, l);
     } else {
-        float* part = p.part_o(stat + i, job.part);
-        mix_store_row<DC>(part, o, 1.0f, p.dv4, h);
-        if (h == 0) p.part_ml(stat + i, job.part) = make_float2(m, l);
+        mix_store_row<DC>(p.part_o(stat, job.part), o, 1.0f, p.dv4, h);
+        if (h == 0) p.part_ml(stat, job.part) = make_float2(m, l);
     }
 }
 
@@ -179,29 +177,28 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p
 // chunk multiplies d = 16s + 4*k4 + u.  Result register v of lane (c, k4) is key 4*k4 + v, row c: the B operand of step v of
 // Y^T = V^T.P^T, whose A operand is key 4*k4 + v.  A lane loads 16 bytes of that key at 64*e + 4*c; its float u belongs to
 // the 16 outputs 64e + 4*(0..15) + u, so the four floats feed four blocks.
-template <int DE>   // head dimension in 64s
+template <int DE, bool NT>   // head dimension in 64s; keys and values read non-temporally
 __global__ __launch_bounds__(NTHREADS, 2) void window_rows(const WindowParams p) {
     constexpr int NS = DE * 4;
     __shared__ __attribute__((aligned(16))) float So[4][16][DE * 64 + 4];
     __shared__ float Sm[4][16], Sl[4][16];
 
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, k4 = lane >> 4;
-    const WindowJob job = window_row_job(p, blockIdx.x);
+    const WindowJob job = window_job(p, blockIdx.x);
     const WindowLens len = window_lens(p, job.n);
-    const int group = p.head / p.kv_head, rows = p.QL * group;
-    const int row0 = job.qt * 16, row = row0 + c;
-    const int i = row / group, hd = job.kvh * group + (row - i * group);
-    const int off = len.vl - len.ql;
-    const bool live = row < rows && i < len.ql;
-    const int pos = live ? i + off : -1;
+    const int group = p.head / p.kv_head, rows = p.QL * group, off = len.vl - len.ql;
+    const int row0 = job.qt * 16;
+    const WindowRow row = window_row(p, job, row0 + c, group, len.ql);
+    const bool live = row.live;
+    const int pos = live ? row.i + off : -1;
 
-    const int i0 = row0 / group, i1 = min((min(row0 + 16, rows) - 1) / group, len.ql - 1);
-    const WindowRange range = window_range(p, i0 + off, i1 + off, i0 <= i1, len.vl);
+    const WindowSpan all = window_span(row0, 16, group, len.ql, off);
+    const WindowRange range = window_range(p, all.first, all.last, all.first <= all.last, len.vl);
     const int nsink = (range.sink_end + 15) / 16, nwin = (max(range.hi - range.low, 0) + 15) / 16;
     const int first = mix_uniform((int)((long long)(nsink + nwin) * job.part / p.parts));
     const int last = mix_uniform((int)((long long)(nsink + nwin) * (job.part + 1) / p.parts));
 
-    const float* qrow = p.Q + job.n * p.q.n + (size_t)min(hd, p.head - 1) * p.q.h + (size_t)min(i, p.QL - 1) * p.q.l;
+    const float* qrow = p.Q + job.n * p.q.n + row.hd * p.q.h + (size_t)row.i * p.q.l;
     v4f qf[NS];
 #pragma unroll
     for (int s = 0; s < NS; s++) {
@@ -231,9 +228,9 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_rows(const WindowParams p)
         const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)(Kb + (size_t)key0 * p.k.l), 0, left * p.k.l * 4, RSRC_FLAGS);
         const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)(Vb + (size_t)key0 * p.v.l), 0, left * p.v.l * 4, RSRC_FLAGS);
 #pragma unroll
-        for (int s2 = 0; s2 < NS; s2++) kr[s2] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rk, koff[s2], 0, 0));
+        for (int s2 = 0; s2 < NS; s2++) kr[s2] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rk, koff[s2], 0, NT ? 2 : 0));
 #pragma unroll
-        for (int s2 = 0; s2 < 4 * DE; s2++) vr[s2] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rv, voff[s2], 0, 0));
+        for (int s2 = 0; s2 < 4 * DE; s2++) vr[s2] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rv, voff[s2], 0, NT ? 2 : 0));
     };
 
     v4f o[DE][4];
@@ -349,21 +346,21 @@ __global__ __launch_bounds__(NTHREADS) void window_join(const WindowParams p) {
 }
 
 // ---------------------------------------------------------------- host side
-constexpr int ROWS_MAX_QL = 16;      // up to here the row kernel: a tile of the other has 128 queries
+constexpr int ROWS_MAX = 32;         // rows of a key / value head up to which window_rows takes the call
 
 struct WindowPlan { bool rows; int qtiles, parts; };
 
 // One decision for the launch and for the size of the caller's buffer: from the sizes alone.
 WindowPlan window_plan(int N, int head, int kv_head, int QL, int VL, int window, int sinks) {
     WindowPlan x;
-    const long long group = head / kv_head;
-    x.rows = QL <= ROWS_MAX_QL;
+    const long long group = head / kv_head, rows = QL * group;
+    x.rows = rows <= ROWS_MAX;
     const long long per = x.rows ? 16 : AQ;
-    x.qtiles = (int)(x.rows ? (QL * group + 15) / 16 : (QL + AQ - 1) / AQ);
-    const long long base = (long long)N * x.qtiles * (x.rows ? kv_head : head);
-    const long long reach = window == 0 ? VL : (long long)window + sinks + (x.rows ? QL : per);
+    x.qtiles = (int)((rows + per - 1) / per);
+    const long long base = (long long)N * kv_head * x.qtiles;
+    const long long reach = window == 0 ? VL : (long long)window + sinks + (per + group - 1) / group;
     const long long steps = ((reach < VL ? reach : VL) + (x.rows ? 15 : 31)) / (x.rows ? 16 : 32);
-    const long long want = x.rows ? 1024 : 512, least = x.rows ? 8 : 4;   // workgroups on the chip; steps worth a part
+    const long long want = x.rows ? 1024 : 512, least = x.rows ? 16 : 4;   // workgroups on the chip; steps worth a part
     long long parts = base >= want / 2 ? 1 : (want + base - 1) / base;
     if (parts > steps / least) parts = steps / least;
     x.parts = (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
@@ -380,9 +377,9 @@ bool window_arguments_ok(int N, int head, int kv_head, int QL, int VL, int dk4, 
     if (N <= 0 || head <= 0 || kv_head <= 0 || head % kv_head != 0 || QL <= 0 || VL <= 0 || dk4 <= 0 || dv4 <= 0 || (dk4 & 3) ||
         (dv4 & 3) || dk4 > 128 || dv4 > 128 || window < 0 || sinks < 0)
         return false;
-    // positions are 32-bit, a tile's offsets 32-bit bytes, a launch's workgroups 31 bits
+    // positions and rows are 32-bit, a tile's offsets 32-bit bytes, a launch's workgroups 31 bits
     const long long row = (long long)head * (dk4 > dv4 ? dk4 : dv4);
-    return (long long)QL + VL < 0x3fffff00LL && row * AQ * 4 < 0x7ffffff0LL &&
+    return (long long)QL + VL < 0x3fffff00LL && row * AQ * 4 < 0x7ffffff0LL && (long long)QL * (head / kv_head) < 0x7fffff00LL &&
            (long long)N * head * ((QL + 15LL) / 16) * 64 < 0x7fffffffLL;
 }
 
@@ -431,12 +428,20 @@ int dragon_Cuda_attention_window_forward(const int64_t* streams, int32_t length,
     hipStream_t s = (hipStream_t)(intptr_t)streams[0];
     const int dmax = dK4 > dV4 ? dK4 : dV4;
     const dim3 block(NTHREADS);
+    const dim3 grid((unsigned)((long long)N * kv_head * plan.qtiles * plan.parts));
     if (plan.rows) {
-        const dim3 grid((unsigned)((long long)N * kv_head * plan.qtiles * plan.parts));
-        if (dmax <= 64) hipLaunchKernelGGL(window_rows<1>, grid, block, 0, s, p);
-        else hipLaunchKernelGGL(window_rows<2>, grid, block, 0, s, p);
+        // keys and values that are read once and do not fit the Infinity Cache pass it by (stream_policy.h has the border):
+        // 65536 keys of 8 heads of 128 in 105 us instead of 121, but 4 x 8192 in 62 instead of 59
+        const long long reach = window == 0 || window > VL ? VL : (long long)window + sinks;
+        const bool nt = plan.qtiles == 1 && (long long)N * kv_head * (reach < VL ? reach : VL) * (dK4 + dV4) * 4 >= STREAM_NT_BYTES;
+        if (dmax <= 64) {
+            if (nt) hipLaunchKernelGGL((window_rows<1, true>), grid, block, 0, s, p);
+            else hipLaunchKernelGGL((window_rows<1, false>), grid, block, 0, s, p);
+        } else {
+            if (nt) hipLaunchKernelGGL((window_rows<2, true>), grid, block, 0, s, p);
+            else hipLaunchKernelGGL((window_rows<2, false>), grid, block, 0, s, p);
+        }
     } else {
-        const dim3 grid((unsigned)((long long)N * head * plan.qtiles * plan.parts));
         switch ((dmax + 31) / 32) {
             case 1: hipLaunchKernelGGL((window_tiles<1, 1, 2>), grid, block, 0, s, p); break;
             case 2: hipLaunchKernelGGL((window_tiles<2, 2, 1>), grid, block, 0, s, p); break;

@@ -2,7 +2,7 @@
 // that see each other, D[i] = <dY[i], Y[i]> and dS = P * (dY.V^T - D):
 //     dQ = scale * dS.K      dK = scale * dS^T.Q      dV = P^T.dY        (dK and dV over all query heads that share the head)
 // P is computed again from Q, K and lse, never stored.  Two kernels, so that every sum has one owner and no result depends on
-// the order of arrival: window_grad_q owns 128 queries and walks over the keys they see, window_grad_kv owns 128 keys and
+// the order of arrival: window_grad_q owns 128 (query, head) rows and walks over the keys they see, window_grad_kv owns 128 keys and
 // walks over the queries that see them, head by head of the group.  That is seven products of which five are necessary:
 // the score and the dY.V^T products happen in both.  Bound by the FP32 matrix pipe.
 //
@@ -134,20 +134,22 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_q(const Window
     const bool second = wave >= 4;
     const WindowJob job = window_job(p, blockIdx.x);
     const WindowLens len = window_lens(p, job.n);
-    const int q0 = job.qt * GQ, i = q0 + block * 32 + r;
-    const size_t stat = ((size_t)job.n * p.head + job.hd) * p.QL + min(i, p.QL - 1);
-    const int qn = min(q0 + GQ, len.ql), off = len.vl - len.ql;
-    const WindowRange range = window_range(p, q0 + off, qn - 1 + off, q0 < qn, len.vl);
+    const int group = p.head / p.kv_head, off = len.vl - len.ql;
+    const int row0 = job.qt * GQ, wrow = row0 + block * 32;
+    const WindowRow row = window_row(p, job, wrow + r, group, len.ql);
+    const size_t stat = ((size_t)job.n * p.head + row.hd) * p.QL + row.i;
+    const WindowSpan all = window_span(row0, GQ, group, len.ql, off), span = window_span(wrow, 32, group, len.ql, off);
+    const WindowRange range = window_range(p, all.first, all.last, all.first <= all.last, len.vl);
     const int nsink = (range.sink_end + AK - 1) / AK, steps = nsink + (max(range.hi - range.low, 0) + AK - 1) / AK;
-    const bool live = i < len.ql;
-    const int pos = live ? i + off : -1;
-    const int w0 = q0 + block * 32 + off, w1 = min(q0 + block * 32 + 32, len.ql) - 1 + off;
+    const bool live = row.live;
+    const int pos = live ? row.i + off : -1;
+    const int w0 = span.first, w1 = span.last;                          // the wavefront's positions
 
     v4f own[NG];                                                        // Q (times scale, in units of log2) or dY
     if (second) {
-        mix_load_cols<NG>(own, a.dY + job.n * p.y.n + job.hd * p.y.h + (size_t)min(i, p.QL - 1) * p.y.l, live, p.dv4, h);
+        mix_load_cols<NG>(own, a.dY + job.n * p.y.n + row.hd * p.y.h + (size_t)row.i * p.y.l, live, p.dv4, h);
     } else {
-        mix_load_cols<NG>(own, p.Q + job.n * p.q.n + job.hd * p.q.h + (size_t)min(i, p.QL - 1) * p.q.l, live, p.dk4, h);
+        mix_load_cols<NG>(own, p.Q + job.n * p.q.n + row.hd * p.q.h + (size_t)row.i * p.q.l, live, p.dk4, h);
 #pragma unroll
         for (int g = 0; g < NG; g++) own[g] *= p.c;
     }
@@ -195,7 +197,7 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_q(const Window
             }
             // keys behind a query (or behind the last key), and before its window: tested only where some query has them.
             // Both factors are cleared: dY.V^T may be anything where nothing is seen.
-            if (key0 + AK - 1 > w0 || key0 + AK > limit || q0 + block * 32 + 32 > len.ql) {
+            if (key0 + AK - 1 > w0 || key0 + AK > limit || !span.full) {
                 const int top = min(pos, limit - 1) - key0 - 4 * h;
 #pragma unroll
                 for (int kb = 0; kb < KB; kb++)
@@ -230,7 +232,7 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_q(const Window
         }
         buf = b1;
     }
-    if (second && i < p.QL) mix_store_row<DC>(a.dQ + job.n * p.q.n + job.hd * p.q.h + (size_t)i * p.q.l, o, a.scale, p.dk4, h);
+    if (second && row.exists) mix_store_row<DC>(a.dQ + job.n * p.q.n + row.hd * p.q.h + (size_t)row.i * p.q.l, o, a.scale, p.dk4, h);
 }
 
 // ---------------------------------------------------------------- dK, dV
@@ -649,7 +651,7 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
     p.window = window == 0 || window > QL + VL ? QL + VL : window;
     p.sinks = sinks;
     p.c = scale * MIX_LOG2E;
-    p.qtiles = (QL + GQ - 1) / GQ; p.parts = 1; p.part = nullptr;
+    p.qtiles = (int)(((long long)QL * (head / kv_head) + GQ - 1) / GQ); p.parts = 1; p.part = nullptr;
     a.dY = (const float*)(intptr_t)dDeltaY;
     a.dQ = (float*)(intptr_t)dDeltaQ; a.dK = (float*)(intptr_t)dDeltaK; a.dV = (float*)(intptr_t)dDeltaV;
     a.stats = (float*)(intptr_t)dBuf;
@@ -672,7 +674,7 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
     hipLaunchKernelGGL(window_delta, dim3((unsigned)((a.rows + NTHREADS / 32 - 1) / (NTHREADS / 32) + 1)), block, 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const dim3 gq((unsigned)((long long)N * head * p.qtiles)), gk((unsigned)b.workers);
+    const dim3 gq((unsigned)((long long)N * kv_head * p.qtiles)), gk((unsigned)b.workers);
     const int dmax = dK4 > dV4 ? dK4 : dV4;
 #define GRAD_CASE(DB_, DC_, B_)                                                        \
     do {                                                                              \

@@ -20,6 +20,7 @@
 // powers are FP32; the exponent g n is rounded once, which is an error of |g n| 2^-24 in a factor e^{g n}.
 #include "token_mixer.h"
 #include "runtime_internal.h"
+#include "stream_policy.h"
 #include "../../include/dragon_hip_gemm.h"
 
 namespace dragon {
@@ -380,6 +381,7 @@ constexpr int STEP_COLS = 32;                 // columns of the state per workgr
 constexpr int STEP_ROWS = 128 / (NTHREADS / (STEP_COLS / 4));   // rows of the state per thread
 // A thread holds 4 columns of rows row0, row0 + 32, ... of the state; a token's output is added over the 8 row groups of a
 // wavefront by exchange and over the wavefronts through LDS.
+template <bool NT>
 __global__ __launch_bounds__(NTHREADS) void decay_steps(const DecaySteps p) {
     __shared__ __attribute__((aligned(16))) float part[2][4][STEP_COLS];
     const int t = threadIdx.x, wave = t >> 6;
@@ -394,7 +396,7 @@ __global__ __launch_bounds__(NTHREADS) void decay_steps(const DecaySteps p) {
 #pragma unroll
     for (int a = 0; a < STEP_ROWS; a++) {
         const int row = row0 + 32 * a;
-        s[a] = (mine && row < p.dk && p.first) ? *(const v4f*)(p.first + base + (size_t)row * p.dv) : (v4f)(0.0f);
+        s[a] = (mine && row < p.dk && p.first) ? stream_load4<NT>(p.first + base + (size_t)row * p.dv) : (v4f)(0.0f);
     }
     const float* q = p.Q + n * p.q.n + hd * p.q.h;
     const float* k = p.K + n * p.k.n + hd * p.k.h;
@@ -429,7 +431,7 @@ __global__ __launch_bounds__(NTHREADS) void decay_steps(const DecaySteps p) {
 #pragma unroll
         for (int a = 0; a < STEP_ROWS; a++) {
             const int row = row0 + 32 * a;
-            if (row < p.dk) *(v4f*)(p.last + base + (size_t)row * p.dv) = s[a];
+            if (row < p.dk) stream_store4<NT>(p.last + base + (size_t)row * p.dv, s[a]);
         }
     }
 }
@@ -547,7 +549,10 @@ int dragon_Cuda_linear_attention_forward(const int64_t* streams, int32_t length,
     hipStream_t s = (hipStream_t)(intptr_t)streams[0];
     if (L <= STEPS_MAX) {
         DecaySteps p = {Q, K, V, Y, lk, lk, lv, lv, g, lens, first, last, head, L, dK4, dV4, (dV4 + STEP_COLS - 1) / STEP_COLS, scale};
-        hipLaunchKernelGGL(decay_steps, dim3((unsigned)((long long)N * head * p.slabs)), dim3(NTHREADS), 0, s, p);
+        const dim3 grid((unsigned)((long long)N * head * p.slabs));
+        if (first != nullptr && last != nullptr && stream_nt(first, last, (long long)N * head * state * 4))
+            hipLaunchKernelGGL(decay_steps<true>, grid, dim3(NTHREADS), 0, s, p);
+        else hipLaunchKernelGGL(decay_steps<false>, grid, dim3(NTHREADS), 0, s, p);
         return hipGetLastError();
     }
     const DecayCut cut = decay_cut(N, head, L, dV4);
