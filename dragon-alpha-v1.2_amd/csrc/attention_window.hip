@@ -26,7 +26,7 @@ namespace {
 constexpr int AQ = 128;          // rows per workgroup of the tiled kernel: 32 per wavefront
 constexpr int LAG = 8;           // the reference maximum may lag the true one by 2^LAG
 constexpr float NEG = -__builtin_inff();
-constexpr float LOWEST = -3.0e38f;   // below every score that is not -infinity
+constexpr float LOWEST = -3.402823466e38f;   // not above any score but -infinity
 
 // ---------------------------------------------------------------- many queries
 template <int DB, int DC, int KB>
@@ -380,6 +380,7 @@ bool window_arguments_ok(int N, int head, int kv_head, int QL, int VL, int dk4, 
     // positions and rows are 32-bit, a tile's offsets 32-bit bytes, a launch's workgroups 31 bits
     const long long row = (long long)head * (dk4 > dv4 ? dk4 : dv4);
     return (long long)QL + VL < 0x3fffff00LL && row * AQ * 4 < 0x7ffffff0LL && (long long)QL * (head / kv_head) < 0x7fffff00LL &&
+           (long long)N * kv_head * ((VL + 127LL) / 128) < 0x7fffffffLL &&
            (long long)N * head * ((QL + 15LL) / 16) * 64 < 0x7fffffffLL;
 }
 

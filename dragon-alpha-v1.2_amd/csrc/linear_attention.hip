@@ -56,7 +56,7 @@ __device__ __forceinline__ int decay_len(const int* lens, int n, int L) { return
 // Two workgroups share a compute unit (80 KiB of LDS each at widths of 128).  Two barriers for 32 tokens: behind the first the
 // scores and z are there and x is free, behind the second z is free and the next x and y are there; y has two buffers.
 template <int XB, int ZB, bool ST>
-__global__ __launch_bounds__(64 * ZB, 2) void decay_walk(const DecayWalk p) {
+__global__ __launch_bounds__(64 * ZB, XB == 4 && ZB < 3 ? 1 : 2) void decay_walk(const DecayWalk p) {
     constexpr int XW = XB * 32, ZW = (ZB == 3 ? 4 : ZB) * 32, NG = XB * 4, SHARE = (NG + ZB - 1) / ZB;
     __shared__ __attribute__((aligned(16))) float Xs[32 * XW];
     __shared__ __attribute__((aligned(16))) float Ys[2][32 * XW];
@@ -487,7 +487,7 @@ bool decay_arguments_ok(int N, int head, int L, int dK4, int dV4) {
     if (N <= 0 || head <= 0 || L <= 0 || dK4 <= 0 || dV4 <= 0 || (dK4 & 3) || (dV4 & 3) || dK4 > 128 || dV4 > 128) return false;
     const long long row = (long long)head * (dK4 > dV4 ? dK4 : dV4);
     // a tile's offsets are 32-bit bytes, positions 32-bit, a launch's workgroups 31 bits
-    return L < 0x7fffff00 && row * 32 * 4 < 0x7ffffff0LL && (long long)N * head * 64 < 0x7fffffffLL &&
+    return L < 0x3fffff00 && row * 32 * 4 < 0x7ffffff0LL && (long long)N * head * 64 < 0x7fffffffLL &&
            (long long)N * head * dK4 * dV4 / 4 < 0x7fffffffLL * 128;
 }
 

@@ -17,6 +17,7 @@ i32, i64, f32 = c_int32, c_int64, c_float
 p_i64 = POINTER(c_int64)
 p_f32 = POINTER(c_float)
 p_i32 = POINTER(c_int32)
+p_void = POINTER(c_void_p)
 
 # name -> (restype, argtypes); mirrors the two public headers one to one
 _MM2D = [p_i64, i32, i64, i64, i64, i32, i32, i32]
@@ -188,6 +189,10 @@ SIGNATURES = {
     "dragon_policy_conv3D_GEMM_nstream": (i32, [i32, i32]),
     "dragon_engine_attention": (c_void_p, [c_void_p, c_void_p, c_void_p, c_void_p, i32, f32]),
     "dragon_engine_attention_masked": (c_void_p, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, i32, f32]),
+    "dragon_engine_attention_window": (i32, [c_void_p] * 4 + [i32] * 4 + [f32, p_void, p_void]),
+    "dragon_engine_attention_window_delta": (i32, [c_void_p] * 7 + [i32] * 4 + [f32, p_void]),
+    "dragon_engine_linear_attention": (i32, [c_void_p] * 6 + [i32, f32, p_void, p_void]),
+    "dragon_engine_linear_attention_delta": (i32, [c_void_p] * 8 + [i32, f32, i32, p_void]),
     "dragon_engine_linear": (c_void_p, [c_void_p, i32, f32, c_void_p, f32]),
     "dragon_engine_softmax": (c_void_p, [c_void_p, i32, c_void_p, i32, f32]),
     "dragon_engine_transpose": (c_void_p, [c_void_p, i32, c_void_p, i32, i32]),

@@ -250,6 +250,45 @@ class Engine:
             return self._wrap(lib.dragon_engine_attention_masked(self._h, hs[0], hs[1], hs[2], mask._h, head, scale))
         return self._wrap(lib.dragon_engine_attention(self._h, hs[0], hs[1], hs[2], head, scale))
 
+    # ---- token mixers of language models ----
+    def _outputs(self, call, n):
+        out = (ctypes.c_void_p * n)()
+        rc = call(out)
+        if rc:
+            _raise(rc)
+        return tuple(Tensor(self, h) if h else None for h in out)
+
+    def attention_window(self, Q, K, V, head, kv_head=None, window=0, sinks=0, scale=0.0, lse=False):
+        """Causal attention over the last `window` keys (0: all) and the first `sinks` of Q[N, QL, head*dk],
+        K[N, VL, kv_head*dk], V[N, VL, kv_head*dv]; lse=True: (Y, Lse), which the gradient takes."""
+        hs = [x._h if x is not None else None for x in (Q, K, V)]
+        y, l = (ctypes.c_void_p * 1)(), (ctypes.c_void_p * 1)()
+        rc = lib.dragon_engine_attention_window(self._h, *hs, head, kv_head or head, window, sinks, scale, y, l if lse else None)
+        if rc:
+            _raise(rc)
+        return (Tensor(self, y[0]), Tensor(self, l[0])) if lse else Tensor(self, y[0])
+
+    def attention_window_delta(self, deltaY, Y, Q, K, V, Lse, head, kv_head=None, window=0, sinks=0, scale=0.0):
+        """(deltaQ, deltaK, deltaV) of attention_window."""
+        hs = [x._h if x is not None else None for x in (deltaY, Y, Q, K, V, Lse)]
+        return self._outputs(lambda out: lib.dragon_engine_attention_window_delta(self._h, *hs, head, kv_head or head, window,
+                                                                                  sinks, scale, out), 3)
+
+    def linear_attention(self, Q, K, V, Decay, head, State=None, scale=0.0, state=False):
+        """Linear attention with a decay for each head of Q, K[N, L, head*dk], V[N, L, head*dv]; Decay[head] holds the
+        decays' logarithms; state=True: (Y, the state behind the last token)."""
+        hs = [x._h if x is not None else None for x in (Q, K, V, Decay, State)]
+        y, s = (ctypes.c_void_p * 1)(), (ctypes.c_void_p * 1)()
+        rc = lib.dragon_engine_linear_attention(self._h, *hs, head, scale, y, s if state else None)
+        if rc:
+            _raise(rc)
+        return (Tensor(self, y[0]), Tensor(self, s[0])) if state else Tensor(self, y[0])
+
+    def linear_attention_delta(self, deltaY, Q, K, V, Decay, head, State=None, deltaStateOut=None, scale=0.0, state=False):
+        """(deltaQ, deltaK, deltaV, deltaState) of linear_attention; deltaState is None unless state=True."""
+        hs = [x._h if x is not None else None for x in (deltaY, Q, K, V, Decay, State, deltaStateOut)]
+        return self._outputs(lambda out: lib.dragon_engine_linear_attention_delta(self._h, *hs, head, scale, int(state), out), 4)
+
     def transpose(self, inplace, X, dimIdx1, dimIdx2):
         h = lib.dragon_engine_transpose(self._h, int(inplace), X._h if X else None, dimIdx1, dimIdx2)
         if h and X is not None and h == X._h:

@@ -156,6 +156,18 @@ struct FreeAfter : Syncer {     // Syncer.dual(sc1, () -> core.free(old)): wait,
     }
 };
 
+struct SharedSyncer : Syncer {  // the outputs of one launch wait for the same thing, whichever is asked first
+    struct One { SyncerPtr sc; std::mutex mu; bool done = false; };
+    std::shared_ptr<One> one;
+    explicit SharedSyncer(std::shared_ptr<One> o) : one(std::move(o)) {}
+    void sync() override {
+        std::lock_guard<std::mutex> g(one->mu);
+        if (one->done) return;
+        one->sc->sync();
+        one->done = true;
+    }
+};
+
 std::mutex g_cuda_class_lock;  // the reference serialises setDevice+malloc/free on Cuda.class
 
 }  // namespace
@@ -726,6 +738,13 @@ SyncerPtr CudaFloat32EngineBase::softmax2D(int64_t Y, int64_t X, int field_lengt
     cu(dragon_Cuda_reduce_softmax2D(stream, X, Y, field_length, row_lengthv, width, stride, scale));
     return SyncerPtr(new StreamSyncer(streamPool_.get(), stream));
 }
+SyncerPtr CudaFloat32EngineBase::launch(const std::function<int(const int64_t*, int)>& call) {
+    std::vector<int64_t> s = streamPool_->getStreamArray(1);
+    last_gridZ = 1; last_stream_count = (int)s.size();
+    try { cu(call(s.data(), (int)s.size())); }
+    catch (...) { streamPool_->returnStreamArray(s); throw; }
+    return SyncerPtr(new StreamArraySyncer(streamPool_.get(), s));
+}
 SyncerPtr CudaFloat32EngineBase::attention(int64_t Y, int64_t Q, int64_t K, int64_t V, int N, int head, int QL,
                                            int VL, int dK4, int dV4, bool head_inner, float scale, int64_t Mask,
                                            int mask_pitch, bool mask_per_head) {
@@ -994,6 +1013,14 @@ SyncerPtr EngineCore::conv3D_biased(int64_t Y, int OH, int OW, int64_t X, int IH
     return base_->conv3D_biased(Y, OH, OW, X, IH, IW, W, FH, FW, pad4(N), pad4(IC), OC_4x, sh, sw, ph, pw,
                                 Bias, lengthv, OC);
 }
+SyncerPtr EngineCore::launch_buffered(int64_t bytes, const std::function<int(const int64_t*, int, int64_t)>& call) {
+    if (bytes < 0 || bytes / 4 > 0x7ffffff0LL) throw IllegalArgumentException("sizes out of range");
+    if (bytes == 0) return base_->launch([&](const int64_t* s, int n) { return call(s, n, 0); });
+    const Block b = malloc((int)((bytes + 3) / 4));
+    try {
+        return SyncerPtr(new FreeAfter(base_->launch([&](const int64_t* s, int n) { return call(s, n, b.address); }), this, b.size, b.address));
+    } catch (...) { free(b.size, b.address); throw; }
+}
 SyncerPtr EngineCore::attention(int64_t Y, int64_t Q, int64_t K, int64_t V, int N, int head, int QL, int VL,
                                 int dK, int dV, bool head_inner, float scale, int64_t Mask, int mask_width,
                                 bool mask_per_head) {
@@ -1127,6 +1154,14 @@ static void require(Tensor* t, const char* name) {
 
 void Engine::finish(Tensor* C, SyncerPtr sc) {
     if (sync_) sc->sync(); else C->setSyncer(std::move(sc));
+}
+
+void Engine::finish(const std::vector<Tensor*>& all, SyncerPtr sc) {
+    if (sync_) { sc->sync(); return; }
+    auto one = std::make_shared<SharedSyncer::One>();
+    one->sc = std::move(sc);
+    for (Tensor* t : all)
+        if (t) t->setSyncer(SyncerPtr(new SharedSyncer(one)));
 }
 
 Tensor* Engine::empty(const std::vector<int>& dim) {   // Engine.java:522-532
@@ -1627,6 +1662,155 @@ Tensor* Engine::attention(Tensor* Q, Tensor* K, Tensor* V, int head, float scale
                                    mask_per_head));
     } catch (...) { deleteTensor(Y); throw; }
     return Y;
+}
+
+namespace {
+
+// sizes of a token mixer's operands [N, L, heads * d]
+struct MixerDims { int N, QL, VL, dk, dv; };
+
+void mixer_equals(long long a, const char* an, long long b, const char* bn) {
+    if (a != b) throw IllegalArgumentException(std::string(an) + " { got " + std::to_string(a) + " } != " + bn + " { got " + std::to_string(b) + " }");
+}
+
+MixerDims mixer_dims(Tensor* Q, Tensor* K, Tensor* V, int head, int kv_head) {
+    auto s = [](long long v) { return std::to_string(v); };
+    if (Q->ndim() < 2 || K->ndim() < 2 || V->ndim() < 2) throw IllegalArgumentException("Q.ndim, K.ndim and V.ndim must >= 2");
+    if (head <= 0 || kv_head <= 0 || head % kv_head != 0)
+        throw IllegalArgumentException("head { got " + s(head) + " } must be a positive multiple of kv_head { got " + s(kv_head) + " } > 0");
+    mixer_equals(Q->dim[0], "Q.batch", K->dim[0], "K.batch");
+    mixer_equals(Q->dim[0], "Q.batch", V->dim[0], "V.batch");
+    const int qc = Q->lastDim(), kc = K->lastDim(), vc = V->lastDim();
+    if (qc % head != 0 || kc % kv_head != 0 || vc % kv_head != 0)
+        throw IllegalArgumentException("last dimensions { got " + s(qc) + ", " + s(kc) + ", " + s(vc) + " } must be multiples of the heads");
+    MixerDims d = {Q->dim[0], 0, 0, qc / head, vc / kv_head};
+    mixer_equals(qc / head, "Q.head_dim", kc / kv_head, "K.head_dim");
+    if ((head > 1 || kv_head > 1) && ((d.dk & 3) || (d.dv & 3)))
+        throw IllegalArgumentException("with several heads the head dimensions { got " + s(d.dk) + ", " + s(d.dv) + " } must be multiples of 4");
+    if (pad4(d.dk) > 128 || pad4(d.dv) > 128)
+        throw IllegalArgumentException("head dimensions { got " + s(d.dk) + ", " + s(d.dv) + " } must <= 128");
+    d.QL = Q->length / (d.N * qc);
+    d.VL = K->length / (d.N * kc);
+    mixer_equals(d.VL, "K.seq_len", V->length / (d.N * vc), "V.seq_len");
+    if ((long long)d.N * head * d.QL > 0x7ffffff0LL) throw IllegalArgumentException("N * head * seq_len must < 2^31");
+    return d;
+}
+
+void mixer_length(Tensor* t, const char* name, long long length) {
+    if (t->length != length)
+        throw IllegalArgumentException(std::string(name) + ".length { got " + std::to_string(t->length) + " } must be " + std::to_string(length));
+}
+
+std::vector<int> with_last(std::vector<int> dim, int last) {
+    dim.back() = last;
+    return dim;
+}
+
+// the work buffer's bytes as the entries are told them
+long long mixer_bytes(int64_t n) { return n < 0 ? 0 : n; }
+
+}  // namespace
+
+Tensor* Engine::attention_window(Tensor* Q, Tensor* K, Tensor* V, int head, int kv_head, int window, int sinks, float scale, Tensor** Lse) {
+    require(Q, "Q"); require(K, "K"); require(V, "V");
+    const MixerDims d = mixer_dims(Q, K, V, head, kv_head);
+    if (window < 0 || sinks < 0) throw IllegalArgumentException("window and sinks must >= 0");
+    if (scale == 0.0f) scale = 1.0f / sqrtf((float)d.dk);
+    const int dk4 = pad4(d.dk), dv4 = pad4(d.dv);
+    const int64_t need = dragon_Cuda_attention_window_bufsize(d.N, head, kv_head, d.QL, d.VL, dk4, dv4, window, sinks);
+    Tensor* Y = &empty(with_last(Q->dim, head * d.dv))->c();
+    Tensor* lse = nullptr;
+    try {
+        if (Lse) lse = &empty({d.N * head * d.QL})->c();
+        finish({Y, lse}, core_->launch_buffered(need, [&](const int64_t* s, int n, int64_t buf) {
+            return dragon_Cuda_attention_window_forward(s, n, Q->address, K->address, V->address, Y->address, lse ? lse->address : 0, 0, 0,
+                                                        buf, mixer_bytes(need), d.N, head, kv_head, d.QL, d.VL, dk4, dv4, 1, scale, window, sinks);
+        }));
+    } catch (...) { deleteTensor(Y); if (lse) deleteTensor(lse); throw; }
+    if (Lse) *Lse = lse;
+    return Y;
+}
+
+void Engine::attention_window_delta(Tensor* deltaY, Tensor* Y, Tensor* Q, Tensor* K, Tensor* V, Tensor* Lse, int head, int kv_head,
+                                    int window, int sinks, float scale, Tensor* out[3]) {
+    require(deltaY, "deltaY"); require(Y, "Y"); require(Q, "Q"); require(K, "K"); require(V, "V"); require(Lse, "Lse");
+    const MixerDims d = mixer_dims(Q, K, V, head, kv_head);
+    if (window < 0 || sinks < 0) throw IllegalArgumentException("window and sinks must >= 0");
+    mixer_equals(Y->lastDim(), "Y.lastDim", head * d.dv, "head * V.head_dim");
+    mixer_equals(deltaY->lastDim(), "deltaY.lastDim", head * d.dv, "head * V.head_dim");
+    mixer_length(Y, "Y", (long long)d.N * d.QL * head * d.dv);
+    mixer_length(deltaY, "deltaY", Y->length);
+    mixer_length(Lse, "Lse", (long long)d.N * head * d.QL);
+    if (scale == 0.0f) scale = 1.0f / sqrtf((float)d.dk);
+    const int dk4 = pad4(d.dk), dv4 = pad4(d.dv);
+    const int64_t need = dragon_Cuda_attention_window_backward_bufsize(d.N, head, kv_head, d.QL, d.VL, dk4, dv4, window, sinks);
+    Tensor* t[3] = {nullptr, nullptr, nullptr};
+    try {
+        t[0] = &empty(Q->dim)->c(); t[1] = &empty(K->dim)->c(); t[2] = &empty(V->dim)->c();
+        finish({t[0], t[1], t[2]}, core_->launch_buffered(need, [&](const int64_t* s, int n, int64_t buf) {
+            return dragon_Cuda_attention_window_backward(s, n, Q->address, K->address, V->address, Y->address, Lse->address, deltaY->address,
+                                                         t[0]->address, t[1]->address, t[2]->address, 0, 0, buf, mixer_bytes(need), d.N, head,
+                                                         kv_head, d.QL, d.VL, dk4, dv4, 1, scale, window, sinks);
+        }));
+    } catch (...) { for (Tensor* x : t) if (x) deleteTensor(x); throw; }
+    for (int i = 0; i < 3; i++) out[i] = t[i];
+}
+
+static MixerDims decay_dims(Tensor* Q, Tensor* K, Tensor* V, Tensor* Decay, Tensor* State, int head) {
+    const MixerDims d = mixer_dims(Q, K, V, head, head);
+    mixer_equals(d.QL, "Q.seq_len", d.VL, "K.seq_len");
+    if ((d.dk & 3) || (d.dv & 3)) throw IllegalArgumentException("head dimensions must be multiples of 4");   // rows of the state
+    mixer_length(Decay, "Decay", head);
+    if (State) {
+        mixer_equals(State->lastDim(), "State.lastDim", d.dv, "V.head_dim");
+        mixer_length(State, "State", (long long)d.N * head * d.dk * d.dv);
+    }
+    return d;
+}
+
+Tensor* Engine::linear_attention(Tensor* Q, Tensor* K, Tensor* V, Tensor* Decay, Tensor* State, int head, float scale, Tensor** StateOut) {
+    require(Q, "Q"); require(K, "K"); require(V, "V"); require(Decay, "Decay");
+    const MixerDims d = decay_dims(Q, K, V, Decay, State, head);
+    if (scale == 0.0f) scale = 1.0f / sqrtf((float)d.dk);
+    const int64_t need = dragon_Cuda_linear_attention_bufsize(d.N, head, d.QL, d.dk, d.dv);
+    Tensor* Y = &empty(with_last(Q->dim, head * d.dv))->c();
+    Tensor* last = nullptr;
+    try {
+        if (StateOut) last = &empty({d.N, head, d.dk, d.dv})->c();
+        finish({Y, last}, core_->launch_buffered(need, [&](const int64_t* s, int n, int64_t buf) {
+            return dragon_Cuda_linear_attention_forward(s, n, Q->address, K->address, V->address, Decay->address, State ? State->address : 0,
+                                                        Y->address, last ? last->address : 0, 0, buf, mixer_bytes(need), d.N, head, d.QL,
+                                                        d.dk, d.dv, 1, scale);
+        }));
+    } catch (...) { deleteTensor(Y); if (last) deleteTensor(last); throw; }
+    if (StateOut) *StateOut = last;
+    return Y;
+}
+
+void Engine::linear_attention_delta(Tensor* deltaY, Tensor* Q, Tensor* K, Tensor* V, Tensor* Decay, Tensor* State, Tensor* deltaStateOut,
+                                    int head, float scale, bool want_state, Tensor* out[4]) {
+    require(deltaY, "deltaY"); require(Q, "Q"); require(K, "K"); require(V, "V"); require(Decay, "Decay");
+    const MixerDims d = decay_dims(Q, K, V, Decay, State, head);
+    if (deltaStateOut) {
+        mixer_equals(deltaStateOut->lastDim(), "deltaStateOut.lastDim", d.dv, "V.head_dim");
+        mixer_length(deltaStateOut, "deltaStateOut", (long long)d.N * head * d.dk * d.dv);
+    }
+    mixer_equals(deltaY->lastDim(), "deltaY.lastDim", head * d.dv, "head * V.head_dim");
+    mixer_length(deltaY, "deltaY", (long long)d.N * d.QL * head * d.dv);
+    if (scale == 0.0f) scale = 1.0f / sqrtf((float)d.dk);
+    const int64_t need = dragon_Cuda_linear_attention_backward_bufsize(d.N, head, d.QL, d.dk, d.dv);
+    Tensor* t[4] = {nullptr, nullptr, nullptr, nullptr};
+    try {
+        t[0] = &empty(Q->dim)->c(); t[1] = &empty(K->dim)->c(); t[2] = &empty(V->dim)->c();
+        if (want_state) t[3] = &empty({d.N, head, d.dk, d.dv})->c();
+        finish({t[0], t[1], t[2], t[3]}, core_->launch_buffered(need, [&](const int64_t* s, int n, int64_t buf) {
+            return dragon_Cuda_linear_attention_backward(s, n, Q->address, K->address, V->address, Decay->address, State ? State->address : 0,
+                                                         deltaY->address, deltaStateOut ? deltaStateOut->address : 0, t[0]->address,
+                                                         t[1]->address, t[2]->address, t[3] ? t[3]->address : 0, 0, buf, mixer_bytes(need),
+                                                         d.N, head, d.QL, d.dk, d.dv, 1, scale);
+        }));
+    } catch (...) { for (Tensor* x : t) if (x) deleteTensor(x); throw; }
+    for (int i = 0; i < 4; i++) out[i] = t[i];
 }
 
 // Engine.java:4002-4013

@@ -18,6 +18,7 @@
 #pragma once
 #include <stdint.h>
 #include <map>
+#include <functional>
 #include <memory>
 #include <set>
 #include <mutex>
@@ -243,6 +244,9 @@ public:
     // issues transposes, batchMatMulT2, sdiv, softmax, batchMatMul: nn/unit/complex/block/ChannelMHA.java:66-83)
     // Mask != 0: the probabilities are multiplied by it after the softmax (the block's mask unit); rows of
     // mask_pitch floats, one [QL, mask_pitch] slice for all or one per (image, head)
+    // one launch sequence of the library on one stream of the pool; `call` gets the stream array and its length and
+    // returns the library's code
+    SyncerPtr launch(const std::function<int(const int64_t*, int)>& call);
     SyncerPtr attention(int64_t Y, int64_t Q, int64_t K, int64_t V, int N, int head, int QL, int VL, int dK4,
                         int dV4, bool head_inner, float scale, int64_t Mask = 0, int mask_pitch = 0,
                         bool mask_per_head = false);
@@ -303,6 +307,8 @@ public:
     SyncerPtr softmax2D(int64_t Y, int64_t X, int row_length, int lengthv, int width, float scale = 1.0f);
     SyncerPtr memcpy(int64_t dst, int64_t src, int length);
     // head dimensions arrive unpadded; with more than one head they must be multiples of 4 already
+    // base_->launch with a work buffer of `bytes` (0: address 0) that is freed behind it; bytes < 0: the sizes are refused
+    SyncerPtr launch_buffered(int64_t bytes, const std::function<int(const int64_t*, int, int64_t buf)>& call);
     SyncerPtr attention(int64_t Y, int64_t Q, int64_t K, int64_t V, int N, int head, int QL, int VL, int dK,
                         int dV, bool head_inner, float scale, int64_t Mask = 0, int mask_width = 0,
                         bool mask_per_head = false);
@@ -413,12 +419,28 @@ public:
     // element (ChannelMHA.java:75-76).
     Tensor* attention(Tensor* Q, Tensor* K, Tensor* V, int head, float scale = 0.0f, Tensor* mask = nullptr);
 
+    // The token mixers of language models (dragon_Cuda_attention_window_forward / _backward, dragon_Cuda_linear_attention_*
+    // in dragon_hip_gemm.h say what they compute).  Not Java methods.
+    // Q[N, QL, head*dk], K[N, VL, kv_head*dk], V[N, VL, kv_head*dv] -> Y[N, QL, head*dv]; the queries are the last ones of
+    // the sequence.  scale = 0: 1/sqrt(dk).  Lse (may be null): gets a new tensor [N*head*QL] for the gradient.
+    Tensor* attention_window(Tensor* Q, Tensor* K, Tensor* V, int head, int kv_head, int window, int sinks, float scale, Tensor** Lse);
+    // out: deltaQ, deltaK, deltaV
+    void attention_window_delta(Tensor* deltaY, Tensor* Y, Tensor* Q, Tensor* K, Tensor* V, Tensor* Lse, int head, int kv_head,
+                                int window, int sinks, float scale, Tensor* out[3]);
+    // Q, K[N, L, head*dk], V[N, L, head*dv], Decay[head] -> Y[N, L, head*dv]; State (may be null): [N, head, dk, dv];
+    // StateOut (may be null): gets the state behind the last token
+    Tensor* linear_attention(Tensor* Q, Tensor* K, Tensor* V, Tensor* Decay, Tensor* State, int head, float scale, Tensor** StateOut);
+    // out: deltaQ, deltaK, deltaV and, where want_state, the gradient of State (else null); deltaStateOut may be null
+    void linear_attention_delta(Tensor* deltaY, Tensor* Q, Tensor* K, Tensor* V, Tensor* Decay, Tensor* State, Tensor* deltaStateOut,
+                                int head, float scale, bool want_state, Tensor* out[4]);
+
     // Y = alpha*X1 + beta*X2 + gamma with the row vector X2 broadcast over the rows of X1
     Tensor* add_row(bool inplace, Tensor* X1, Tensor* X2) { return linear2_row(inplace, X1, X2, 1.0f, 1.0f, 0.0f); }
     Tensor* linear2_row(bool inplace, Tensor* X1, Tensor* X2, float alpha, float beta, float gamma);
 
 private:
     void finish(Tensor* C, SyncerPtr sc);
+    void finish(const std::vector<Tensor*>& all, SyncerPtr sc);    // several outputs of one launch
     std::unique_ptr<CudaFloat32EngineBase> base_;
     std::unique_ptr<EngineCore> core_;
     bool check_ = true, sync_ = true;

@@ -338,6 +338,47 @@ dragon_tensor* dragon_engine_attention_masked(dragon_engine* eg, dragon_tensor* 
     });
     return t ? wrap(t) : nullptr;
 }
+int dragon_engine_attention_window(dragon_engine* eg, dragon_tensor* Q, dragon_tensor* K, dragon_tensor* V, int32_t head,
+                                   int32_t kv_head, int32_t window, int32_t sinks, float scale, dragon_tensor** Y,
+                                   dragon_tensor** Lse) {
+    return guard([&] {
+        if (!eg || !Y) throw NullPointerException(eg ? "Y" : "engine");
+        Tensor* lse = nullptr;
+        Tensor* y = eg->eg.attention_window(T(Q), T(K), T(V), head, kv_head, window, sinks, scale, Lse ? &lse : nullptr);
+        *Y = wrap(y);
+        if (Lse) *Lse = wrap(lse);
+    });
+}
+int dragon_engine_attention_window_delta(dragon_engine* eg, dragon_tensor* deltaY, dragon_tensor* Y, dragon_tensor* Q,
+                                         dragon_tensor* K, dragon_tensor* V, dragon_tensor* Lse, int32_t head, int32_t kv_head,
+                                         int32_t window, int32_t sinks, float scale, dragon_tensor* out[3]) {
+    return guard([&] {
+        if (!eg || !out) throw NullPointerException(eg ? "out" : "engine");
+        Tensor* t[3];
+        eg->eg.attention_window_delta(T(deltaY), T(Y), T(Q), T(K), T(V), T(Lse), head, kv_head, window, sinks, scale, t);
+        for (int i = 0; i < 3; i++) out[i] = wrap(t[i]);
+    });
+}
+int dragon_engine_linear_attention(dragon_engine* eg, dragon_tensor* Q, dragon_tensor* K, dragon_tensor* V, dragon_tensor* Decay,
+                                   dragon_tensor* State, int32_t head, float scale, dragon_tensor** Y, dragon_tensor** StateOut) {
+    return guard([&] {
+        if (!eg || !Y) throw NullPointerException(eg ? "Y" : "engine");
+        Tensor* last = nullptr;
+        Tensor* y = eg->eg.linear_attention(T(Q), T(K), T(V), T(Decay), T(State), head, scale, StateOut ? &last : nullptr);
+        *Y = wrap(y);
+        if (StateOut) *StateOut = wrap(last);
+    });
+}
+int dragon_engine_linear_attention_delta(dragon_engine* eg, dragon_tensor* deltaY, dragon_tensor* Q, dragon_tensor* K,
+                                         dragon_tensor* V, dragon_tensor* Decay, dragon_tensor* State, dragon_tensor* deltaStateOut,
+                                         int32_t head, float scale, int32_t want_state, dragon_tensor* out[4]) {
+    return guard([&] {
+        if (!eg || !out) throw NullPointerException(eg ? "out" : "engine");
+        Tensor* t[4];
+        eg->eg.linear_attention_delta(T(deltaY), T(Q), T(K), T(V), T(Decay), T(State), T(deltaStateOut), head, scale, want_state != 0, t);
+        for (int i = 0; i < 4; i++) out[i] = t[i] ? wrap(t[i]) : nullptr;
+    });
+}
 dragon_tensor* dragon_engine_transpose(dragon_engine* eg, int32_t inplace, dragon_tensor* X,
                                        int32_t dimIdx1, int32_t dimIdx2) {
     Tensor* t = nullptr;

@@ -140,6 +140,26 @@ dragon_tensor* dragon_engine_attention(dragon_engine* eg, dragon_tensor* Q, drag
 dragon_tensor* dragon_engine_attention_masked(dragon_engine* eg, dragon_tensor* Q, dragon_tensor* K, dragon_tensor* V,
                                               dragon_tensor* Mask, int32_t head, float scale);
 
+/* The token mixers of language models; dragon_hip_gemm.h says what they compute.  Not Java methods.  All return 0 or an
+ * error code like the other int entries; on an error no output is set.
+ * Q[N, QL, head*dk], K[N, VL, kv_head*dk], V[N, VL, kv_head*dv] -> *Y[N, QL, head*dv]; scale = 0: 1/sqrt(dk); head
+ * dimensions up to 128, multiples of 4 with several heads.  Lse (NULL: not wanted) gets a tensor of N*head*QL values that
+ * the gradient takes; out: deltaQ, deltaK, deltaV. */
+int dragon_engine_attention_window(dragon_engine* eg, dragon_tensor* Q, dragon_tensor* K, dragon_tensor* V, int32_t head,
+                                   int32_t kv_head, int32_t window, int32_t sinks, float scale, dragon_tensor** Y,
+                                   dragon_tensor** Lse);
+int dragon_engine_attention_window_delta(dragon_engine* eg, dragon_tensor* deltaY, dragon_tensor* Y, dragon_tensor* Q,
+                                         dragon_tensor* K, dragon_tensor* V, dragon_tensor* Lse, int32_t head, int32_t kv_head,
+                                         int32_t window, int32_t sinks, float scale, dragon_tensor* out[3]);
+/* Q, K[N, L, head*dk], V[N, L, head*dv], Decay[head], State[N, head, dk, dv] (NULL: zeros) -> *Y[N, L, head*dv] and, where
+ * StateOut is given, the state behind the last token; head dimensions multiples of 4 up to 128.  out: deltaQ, deltaK, deltaV
+ * and the gradient of State (NULL unless want_state); deltaStateOut may be NULL. */
+int dragon_engine_linear_attention(dragon_engine* eg, dragon_tensor* Q, dragon_tensor* K, dragon_tensor* V, dragon_tensor* Decay,
+                                   dragon_tensor* State, int32_t head, float scale, dragon_tensor** Y, dragon_tensor** StateOut);
+int dragon_engine_linear_attention_delta(dragon_engine* eg, dragon_tensor* deltaY, dragon_tensor* Q, dragon_tensor* K,
+                                         dragon_tensor* V, dragon_tensor* Decay, dragon_tensor* State, dragon_tensor* deltaStateOut,
+                                         int32_t head, float scale, int32_t want_state, dragon_tensor* out[4]);
+
 /* Engine.linear(inplace, alpha, X, beta): Y = alpha*X + beta (Engine.java:4005-4013); Engine.sdiv(X, C)
  * is linear(1/C, X, 0).  inplace != 0 writes into X and returns X itself. */
 dragon_tensor* dragon_engine_linear(dragon_engine* eg, int32_t inplace, float alpha, dragon_tensor* X,

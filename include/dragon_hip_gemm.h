@@ -278,8 +278,9 @@ int dragon_Cuda_attention_forward_masked(const int64_t* streams, int32_t length,
  *     lse[i] = log sum_j exp(scale * <Q[i], K[j]>),   Y[i] = sum_j exp(scale * <Q[i], K[j]> - lse[i]) * V[j];
  * a query that sees none has Y[i] = 0, lse[i] = -infinity.  Q and Y have `head` heads, K and V kv_head, which divides head:
  * query head h reads key / value head h / (head / kv_head).  dLse: float[N, head, QL] (for the gradient) or 0.
- * Keys that no query of the call sees are never read (a decoding cache may hold anything there).  A key that some query sees
- * has to be finite in K and V: a NaN or an infinity there can reach the rows of queries that do not see it. */
+ * Keys that no query of the call sees are never read (a decoding cache may hold anything there).  A row that takes
+ * part has to be finite: a NaN or an infinity in a key or value that some query sees can reach the rows of queries that do not
+ * see it (and in the gradient one in Q or dDeltaY the gradients of keys that the query does not see). */
 int64_t dragon_Cuda_attention_window_bufsize(int32_t N, int32_t head, int32_t kv_head, int32_t QL, int32_t VL, int32_t dK4,
                                              int32_t dV4, int32_t window, int32_t sinks);
 int dragon_Cuda_attention_window_forward(const int64_t* streams, int32_t length, int64_t dQ, int64_t dK, int64_t dV, int64_t dY,

@@ -76,8 +76,8 @@ def decay_grad_args(**kw):
     return a
 
 
-BAD_DECAY_SIZES = [dict(N=0), dict(head=0), dict(L=0), dict(L=-5), dict(dK4=0), dict(dK4=30), dict(dK4=132), dict(dV4=0), dict(dV4=6),
-                   dict(dV4=132), dict(head=1 << 17), dict(N=1 << 16, head=1 << 15, L=200)]
+BAD_DECAY_SIZES = [dict(N=0), dict(head=0), dict(L=0), dict(L=-5), dict(L=1 << 30), dict(dK4=0), dict(dK4=30), dict(dK4=132), dict(dV4=0), dict(dV4=6),
+                   dict(dV4=132), dict(head=1 << 18), dict(N=1 << 16, head=1 << 15, L=200)]
 BAD_DECAY = BAD_DECAY_SIZES + [dict(dQ=0), dict(dK=0), dict(dV=0), dict(dDecay=0), dict(dQ=P + 4), dict(dK=P + 4), dict(dV=P + 8),
                                dict(dDecay=P + 2), dict(dState=P + 4), dict(dLens=P + 1), dict(scale=float("-inf")), dict(length=0),
                                dict(length=11), dict(dBuf=0), dict(dBuf=P + 4), dict(buf_size=100)]
