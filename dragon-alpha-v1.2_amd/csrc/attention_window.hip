@@ -32,8 +32,8 @@ constexpr float LOWEST = -3.402823466e38f;   // not above any score but -infinit
 template <int DB, int DC, int KB>
 __global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p) {
     constexpr int AK = KB * 32, DW = DB * 32, NG = DC * 4;
-    __shared__ __attribute__((aligned(16))) float Ks[2][AK * DW];
-    __shared__ __attribute__((aligned(16))) float Vs[2][AK * DW];
+    __shared__ __attribute__((aligned(1024))) float Ks[2][AK * DW];
+    __shared__ __attribute__((aligned(1024))) float Vs[2][AK * DW];
 
     const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
     const WindowJob job = window_job(p, blockIdx.x);
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p
                 }
             l += sum;
 #pragma unroll
-            for (int kb = 0; kb < KB; kb++) mix_columns_product<DW, DC, false>(o, Vs[buf] + kb * 32 * DW, sc[kb], vcols, r, h);
+            for (int kb = 0; kb < KB; kb++) mix_columns_product<DW, DC, false>(o, Vs[buf] + kb * 32 * DW, sc[kb], vcols);
         }
         mix_wait();
         __syncthreads();

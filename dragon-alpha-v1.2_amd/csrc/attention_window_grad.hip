@@ -126,8 +126,8 @@ template <int DB, int DC, int KB>
 __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_q(const WindowGrad a) {
     constexpr int DW = DB * 32, NG = DC * 4, AK = KB * 32, TILE = AK * DW;
     const WindowParams& p = a.w;
-    __shared__ __attribute__((aligned(16))) float Ks[3 * TILE];
-    __shared__ __attribute__((aligned(16))) float Vs[3 * TILE];
+    __shared__ __attribute__((aligned(1024))) float Ks[3 * TILE];
+    __shared__ __attribute__((aligned(1024))) float Vs[3 * TILE];
     __shared__ __attribute__((aligned(16))) float Ps[2][4][KB * 64 * 16];  // [step][32 queries][keys / 8][lane]
     const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
     const int block = wave & 3;
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_q(const Window
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) {
                 take(exchange + kb * 1024, e[kb]);
-                mix_columns_product<DW, DC, true>(o, Ks + buf * TILE + kb * 32 * DW, e[kb], cols, r, h);
+                mix_columns_product<DW, DC, true>(o, Ks + buf * TILE + kb * 32 * DW, e[kb], cols);
             }
         }
         buf = b1;
@@ -285,8 +285,8 @@ __device__ __forceinline__ const WindowGrad& anew(const WindowGrad&) {
 template <int DB, int DC>
 __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_kv(const WindowGrad arg) {
     constexpr int DW = DB * 32, NG = DC * 4, TILE = 32 * DW;
-    __shared__ __attribute__((aligned(16))) float Qs[3 * TILE];
-    __shared__ __attribute__((aligned(16))) float Gs[3 * TILE];
+    __shared__ __attribute__((aligned(1024))) float Qs[3 * TILE];
+    __shared__ __attribute__((aligned(1024))) float Gs[3 * TILE];
     __shared__ __attribute__((aligned(16))) float Ps[2][4][64 * 16];       // [step][32 keys][4 results][lane]
     const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
     const int block = wave & 3;
@@ -420,7 +420,7 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_kv(const Windo
             __builtin_amdgcn_sched_barrier(0);
             if (sees) {
                 if (second) take(exchange, e);
-                mix_columns_product<DW, DC, true>(acc, Z + buf * TILE, e, cols, r, h);
+                mix_columns_product<DW, DC, true>(acc, Z + buf * TILE, e, cols);
             }
             buf = b1;
             i0 += 32;

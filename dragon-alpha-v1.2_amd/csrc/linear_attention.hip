@@ -58,9 +58,9 @@ __device__ __forceinline__ int decay_len(const int* lens, int n, int L) { return
 template <int XB, int ZB, bool ST>
 __global__ __launch_bounds__(64 * ZB, XB == 4 && ZB < 3 ? 1 : 2) void decay_walk(const DecayWalk p) {
     constexpr int XW = XB * 32, ZW = (ZB == 3 ? 4 : ZB) * 32, NG = XB * 4, SHARE = (NG + ZB - 1) / ZB;
-    __shared__ __attribute__((aligned(16))) float Xs[32 * XW];
-    __shared__ __attribute__((aligned(16))) float Ys[2][32 * XW];
-    __shared__ __attribute__((aligned(16))) float Zs[32 * ZW];
+    __shared__ __attribute__((aligned(1024))) float Xs[32 * XW];
+    __shared__ __attribute__((aligned(1024))) float Ys[2][32 * XW];
+    __shared__ __attribute__((aligned(1024))) float Zs[32 * ZW];
     __shared__ __attribute__((aligned(16))) float Ps[ZB][1024];
     const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
     const int lid = xcd_contiguous_id(blockIdx.x, gridDim.x);   // one XCD works on all heads of the same tokens, which lie side by side
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(64 * ZB, XB == 4 && ZB < 3 ? 1 : 2) void decay_walk
 #pragma unroll
                 for (int k = 0; k < XB; k++) S[k] *= f;
             }
-            mix_columns_product<XW, XB, true>(S, Ys[buf], zw, cols, r, h);
+            mix_columns_product<XW, XB, true>(S, Ys[buf], zw, cols);
             any = true;
         }
         mix_wait();                                             // the next x and y
@@ -245,8 +245,8 @@ __global__ __launch_bounds__(NTHREADS, 2) void decay_states(const DecayStates p)
     constexpr int DW = DB * 32;
     // the wavefronts share the result: 2 x 2 of them, each TB x TB blocks of 32 x 32 (one block: the first alone)
     constexpr int TB = DC > 2 ? 2 : 1;
-    __shared__ __attribute__((aligned(16))) float As[2][32 * DW];
-    __shared__ __attribute__((aligned(16))) float Bs[2][32 * DW];
+    __shared__ __attribute__((aligned(1024))) float As[2][32 * DW];
+    __shared__ __attribute__((aligned(1024))) float Bs[2][32 * DW];
     const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
     const int lid = xcd_contiguous_id(blockIdx.x, gridDim.x);
     const int segment = mix_uniform(lid / p.nh), nh = lid - segment * p.nh;
@@ -377,25 +377,26 @@ struct DecaySteps {
     int head, L, dk, dv, slabs;
     float scale;
 };
-constexpr int STEP_COLS = 32;                 // columns of the state per workgroup
-constexpr int STEP_ROWS = 128 / (NTHREADS / (STEP_COLS / 4));   // rows of the state per thread
-// A thread holds 4 columns of rows row0, row0 + 32, ... of the state; a token's output is added over the 8 row groups of a
-// wavefront by exchange and over the wavefronts through LDS.
-template <bool NT>
+// A thread holds 4 columns of rows row0, row0 + LANES, ... of the state; a token's output is added over the row groups of a
+// wavefront by exchange and over the wavefronts through LDS.  COLS: columns of the state per workgroup -- 32, and 64 (256
+// contiguous bytes a row) for states that pass the caches by: 256 x 32 states of 128 x 128 in 190 us instead of 202, but
+// smaller batches are level or behind with it.
+template <bool NT, int COLS>
 __global__ __launch_bounds__(NTHREADS) void decay_steps(const DecaySteps p) {
-    __shared__ __attribute__((aligned(16))) float part[2][4][STEP_COLS];
+    constexpr int ACROSS = COLS / 4, LANES = NTHREADS / ACROSS, STEP_ROWS = 128 / LANES;
+    __shared__ __attribute__((aligned(16))) float part[2][4][COLS];
     const int t = threadIdx.x, wave = t >> 6;
     const int nh = blockIdx.x / p.slabs, slab = blockIdx.x - nh * p.slabs;
     const int n = nh / p.head, hd = nh - n * p.head;
     const int len = decay_len(p.lens, n, p.L);
-    const int col = slab * STEP_COLS + 4 * (t & 7), row0 = t >> 3;
+    const int col = slab * COLS + 4 * (t % ACROSS), row0 = t / ACROSS;
     const bool mine = col < p.dv;
     const float lam = decay_pow(decay_log2(p.g, hd), 1);
     const size_t base = (size_t)nh * p.dk * p.dv + col;
     v4f s[STEP_ROWS];
 #pragma unroll
     for (int a = 0; a < STEP_ROWS; a++) {
-        const int row = row0 + 32 * a;
+        const int row = row0 + LANES * a;
         s[a] = (mine && row < p.dk && p.first) ? stream_load4<NT>(p.first + base + (size_t)row * p.dv) : (v4f)(0.0f);
     }
     const float* q = p.Q + n * p.q.n + hd * p.q.h;
@@ -409,7 +410,7 @@ __global__ __launch_bounds__(NTHREADS) void decay_steps(const DecaySteps p) {
         if (mine) vn = *(const v4f*)(v + (size_t)i * p.v.l + col);
 #pragma unroll
         for (int a = 0; a < STEP_ROWS; a++) {
-            const int row = row0 + 32 * a;
+            const int row = row0 + LANES * a;
             if (row < p.dk) {
                 kn[a] = k[(size_t)i * p.k.l + row];
                 qn[a] = q[(size_t)i * p.q.l + row];
@@ -430,23 +431,23 @@ __global__ __launch_bounds__(NTHREADS) void decay_steps(const DecaySteps p) {
 #pragma unroll
         for (int a = 0; a < STEP_ROWS; a++) out += s[a] * qi[a];
 #pragma unroll
-        for (int x = 8; x < 64; x <<= 1)
+        for (int x = ACROSS; x < 64; x <<= 1)
 #pragma unroll
             for (int u = 0; u < 4; u++) out[u] += __shfl_xor(out[u], x, 64);
-        if ((t & 63) < 8) *(v4f*)&part[i & 1][wave][4 * (t & 7)] = out;
+        if ((t & 63) < ACROSS) *(v4f*)&part[i & 1][wave][4 * (t % ACROSS)] = out;
         __syncthreads();                      // one a token: the next token writes the other half
-        if (t < 8 && mine) {
+        if (t < ACROSS && mine) {
             const v4f sum = (*(const v4f*)&part[i & 1][0][4 * t] + *(const v4f*)&part[i & 1][1][4 * t]) +
                             (*(const v4f*)&part[i & 1][2][4 * t] + *(const v4f*)&part[i & 1][3][4 * t]);
             *(v4f*)(y + (size_t)i * p.y.l + col) = sum * p.scale;
         }
     }
-    if (t < 8 && mine)
+    if (t < ACROSS && mine)
         for (int i = len; i < p.L; i++) *(v4f*)(y + (size_t)i * p.y.l + col) = (v4f)(0.0f);
     if (p.last && mine) {
 #pragma unroll
         for (int a = 0; a < STEP_ROWS; a++) {
-            const int row = row0 + 32 * a;
+            const int row = row0 + LANES * a;
             if (row < p.dk) stream_store4<NT>(p.last + base + (size_t)row * p.dv, s[a]);
         }
     }
@@ -566,11 +567,12 @@ int dragon_Cuda_linear_attention_forward(const int64_t* streams, int32_t length,
     if (need > 0) split_ledger_touch(U, (size_t)need);
     hipStream_t s = (hipStream_t)(intptr_t)streams[0];
     if (L <= STEPS_MAX) {
-        DecaySteps p = {Q, K, V, Y, lk, lk, lv, lv, g, lens, first, last, head, L, dK4, dV4, (dV4 + STEP_COLS - 1) / STEP_COLS, scale};
+        const bool nt = first != nullptr && last != nullptr && stream_nt(first, last, (long long)N * head * state * 4);
+        const int cols = nt ? 64 : 32;
+        DecaySteps p = {Q, K, V, Y, lk, lk, lv, lv, g, lens, first, last, head, L, dK4, dV4, (dV4 + cols - 1) / cols, scale};
         const dim3 grid((unsigned)((long long)N * head * p.slabs));
-        if (first != nullptr && last != nullptr && stream_nt(first, last, (long long)N * head * state * 4))
-            hipLaunchKernelGGL(decay_steps<true>, grid, dim3(NTHREADS), 0, s, p);
-        else hipLaunchKernelGGL(decay_steps<false>, grid, dim3(NTHREADS), 0, s, p);
+        if (nt) hipLaunchKernelGGL((decay_steps<true, 64>), grid, dim3(NTHREADS), 0, s, p);
+        else hipLaunchKernelGGL((decay_steps<false, 32>), grid, dim3(NTHREADS), 0, s, p);
         return hipGetLastError();
     }
     const DecayCut cut = decay_cut(N, head, L, dV4);

@@ -105,34 +105,35 @@ __device__ __forceinline__ void mix_rows_product(v16f& s, const float* tile, con
     mix_order<2, NG, 4>();
 }
 
-// Where lane (r, h) finds float 32b + r of tile row mix_row(v, h).  With the swizzle the place is a lane's part that depends
-// on v % 4 only (the chunk's low three bits are exchanged with the row's) plus a constant.
+// Where lane (r, h) finds float 32b + r of tile row mix_row(v, h): one lane's part, exchanged with a constant of two bits
+// where the tile is swizzled, plus a constant.  (Tiles are aligned to 1 KiB, so an exchange stays inside a row.)
 template <int DW, bool SWIZZLE>
 struct MixColumns {
-    int at[SWIZZLE && DW > 32 ? 4 : 1];
+    int base;
     __device__ __forceinline__ void init(int r, int h) {
-        if constexpr (SWIZZLE && DW > 32) {
-#pragma unroll
-            for (int w = 0; w < 4; w++) at[w] = 4 * h * DW + 4 * ((r >> 2) ^ (4 * h) ^ w) + (r & 3);
-        } else {
-            at[0] = SWIZZLE ? (r & 3) : 4 * h * DW + r;
-        }
+        base = 16 * h * DW + (SWIZZLE ? 16 * ((r >> 2) ^ (DW > 32 ? 4 * h : 2 * h)) + 4 * (r & 3) : 4 * r);
     }
-    __device__ __forceinline__ float read(const float* tile, int v, int b, int r, int h) const {
-        if constexpr (!SWIZZLE) return tile[at[0] + (8 * (v / 4) + v % 4) * DW + 32 * b];
-        else if constexpr (DW > 32) return tile[at[v % 4] + (8 * (v / 4) + v % 4) * DW + 4 * ((8 * b) ^ (8 * ((v / 4) & 1)))];
-        else return tile[mix_row(v, h) * DW + 4 * ((8 * b + (r >> 2)) ^ kin_swizzle<DW>(mix_row(v, h))) + at[0]];
+    static constexpr int variant(int v) { return !SWIZZLE ? 0 : DW > 32 ? v % 4 : 2 * ((v / 4) & 1) + ((v % 4) >> 1); }
+    static constexpr int exchange(int c) { return !SWIZZLE ? 0 : 16 * (DW > 32 ? c : 4 * (c >> 1) + (c & 1)); }
+    static constexpr int place(int v, int b) {
+        return (8 * (v / 4) + v % 4) * DW * 4 + 16 * ((8 * b) ^ (SWIZZLE && DW > 32 ? 8 * ((v / 4) & 1) : 0));
     }
 };
 
 // out^T[d][column] += sum over the tile's rows of tile[row][d] * p[row][column]
 template <int DW, int DC, bool SWIZZLE>
-__device__ __forceinline__ void mix_columns_product(v16f (&o)[DC], const float* tile, const v16f& p, const MixColumns<DW, SWIZZLE>& cols, int r, int h) {
+__device__ __forceinline__ void mix_columns_product(v16f (&o)[DC], const float* tile, const v16f& p, const MixColumns<DW, SWIZZLE>& cols) {
+    typedef MixColumns<DW, SWIZZLE> C;
+    typedef const __attribute__((address_space(3))) float* lds_float;
+    unsigned at[4];
+#pragma unroll
+    for (int c = 0; c < 4; c++) at[c] = (mix_lds(tile) + cols.base) ^ C::exchange(c);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int v = 0; v < 16; v++) {
 #pragma unroll
-        for (int b = 0; b < DC; b++) o[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(cols.read(tile, v, b, r, h), p[v], o[b], 0, 0, 0);
+        for (int b = 0; b < DC; b++)
+            o[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(*(lds_float)(size_t)(at[C::variant(v)] + C::place(v, b)), p[v], o[b], 0, 0, 0);
     }
     mix_order<4, 16 * DC / 2, 2>();                       // the compiler reads two values at a time
 }

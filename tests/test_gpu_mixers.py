@@ -266,6 +266,35 @@ def test_offsets_beyond_32_bits(dh, gpu):
         check({"Y": y.get((1, QL, head, d)).transpose(0, 2, 1, 3)}, want, "QL %d" % QL)
 
 
+def test_states_too_large_for_the_caches(dh, gpu):
+    """Two tokens on 84 x 32 states of 128 x 128 (176 MB, in and out): the form that reads and writes them non-temporally."""
+    rng = np.random.default_rng(23)
+    N, H, L, d = 84, 32, 2, 128
+    f = lambda *s: rng.standard_normal(s, dtype=np.float32)
+    Q, K, V, S = f(N, H, L, d), f(N, H, L, d), f(N, H, L, d), f(N, H, d, d)
+    g = -np.exp2(-rng.uniform(0, 10, H)).astype(np.float32)
+    got = run_decay(dh, Q, K, V, g, 0.25, None, S)
+    for h in range(H):
+        s, lam = S[:, h].astype(np.float64), np.exp(np.float64(g[h]))
+        a = np.abs(s)
+        for t in range(L):
+            k, v, q = (x[:, h, t].astype(np.float64) for x in (K, V, Q))
+            s = lam * s + k[:, :, None] * v[:, None]
+            a = lam * a + np.abs(k)[:, :, None] * np.abs(v)[:, None]
+            y, ya = 0.25 * np.einsum("nk,nkv->nv", q, s), 0.25 * np.einsum("nk,nkv->nv", np.abs(q), a)
+            # as in decay_reference: dk + dv + L + 32 roundings and the powers'
+            weight = (2 * d + L + 32 + 4 * abs(float(g[h])) * L) * 2.0 ** -24
+            assert (np.abs(got["Y"][:, h, t] - y) <= weight * ya).all()
+        assert (np.abs(got["S1"][:, h] - s) <= weight * a).all()
+
+
+def test_a_cache_too_large_for_the_caches(dh, gpu):
+    """A single token on 45000 keys of 8 heads of 128 (369 MB): the form that reads them non-temporally."""
+    Q, K, V, _ = window_operands(np.random.default_rng(24), 1, 16, 8, 1, 45000, 128, 128)
+    got = run_window(dh, Q, K, V, 128 ** -0.5, 0, 0, head_inner=1)
+    check(got, window_reference(Q, K, V, 128 ** -0.5, 0, 0, [1], [45000]))
+
+
 def test_calls_on_two_streams_at_once(dh, gpu):
     """Each with its own work buffer: nothing is shared between calls."""
     rng = np.random.default_rng(22)
