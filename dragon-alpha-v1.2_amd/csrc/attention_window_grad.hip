@@ -28,7 +28,7 @@ constexpr int GK = 128;    // keys per workgroup of window_grad_kv
 struct WindowGrad {
     WindowParams w;          // Y, Lse: what the forward pass left
     const float* dY; float* dQ; float* dK; float* dV;
-    float* stats;            // [2][N, head, QL]: minus lse in units of log2, minus D -- what the products start from
+    float* stats;            // [2][N, head, QL]: lse and D, zeros behind the queries
     long long rows;          // N * head * QL
     float scale;
     int ktiles, workers;     // key tiles of a key / value head; workgroups of window_grad_kv
@@ -41,7 +41,7 @@ struct WindowGrad {
     float* sinks;            // [N, kv_head][sink_blocks][sink_parts][16][dk4 + dv4]
 };
 
-// ---------------------------------------------------------------- what the products start from, and the work to deal
+// ---------------------------------------------------------------- the rows' statistics, and the work to deal
 // the queries that see a key of tile `tile`: [lo, hi)
 struct WindowQueries { int lo, hi; };
 __device__ __forceinline__ WindowQueries window_queries(const WindowGrad& a, int tile, WindowLens len) {
@@ -100,12 +100,16 @@ __global__ __launch_bounds__(NTHREADS) void window_delta(const WindowGrad a) {
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor(sum, x, 64);
     if ((threadIdx.x & 31) == 0) {
-        a.stats[row] = i < ql ? -p.Lse[row] * MIX_LOG2E : 0.0f;
-        a.stats[a.rows + row] = -sum;
+        a.stats[row] = i < ql ? p.Lse[row] : 0.0f;
+        a.stats[a.rows + row] = sum;
     }
 }
 
 constexpr int GT = 512;
+
+// P of a score and its row's lse.  The difference is formed in units of e and near 0 where P counts; the scores are not
+// accumulated from -lse on, nor is lse brought to units of log2 beforehand: either costs up to |lse| 2^-24 in every P of the row.
+__device__ __forceinline__ float probability(float s, float lse) { return __builtin_amdgcn_exp2f((s - lse) * MIX_LOG2E); }
 
 // P handed from one wavefront to the other: 16 bytes per lane and result group
 __device__ __forceinline__ void give(float* at, const v16f& e) {
@@ -145,15 +149,15 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_q(const Window
     const int pos = live ? row.i + off : -1;
     const int w0 = span.first, w1 = span.last;                          // the wavefront's positions
 
-    v4f own[NG];                                                        // Q (times scale, in units of log2) or dY
+    v4f own[NG];                                                        // Q (times scale) or dY
     if (second) {
         mix_load_cols<NG>(own, a.dY + job.n * p.y.n + row.hd * p.y.h + (size_t)row.i * p.y.l, live, p.dv4, h);
     } else {
         mix_load_cols<NG>(own, p.Q + job.n * p.q.n + row.hd * p.q.h + (size_t)row.i * p.q.l, live, p.dk4, h);
 #pragma unroll
-        for (int g = 0; g < NG; g++) own[g] *= p.c;
+        for (int g = 0; g < NG; g++) own[g] *= a.scale;
     }
-    const v16f from = (v16f)(live ? a.stats[(second ? a.rows : 0) + stat] : 0.0f);
+    const float own_stat = live ? a.stats[(second ? a.rows : 0) + stat] : 0.0f;            // lse or D
 
     const float* Kb = p.K + job.n * p.k.n + job.kvh * p.k.h;
     const float* Vb = p.V + job.n * p.v.n + job.kvh * p.v.h;
@@ -186,15 +190,13 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_q(const Window
         if (sees) {
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) {
-                e[kb] = from;
+                e[kb] = (v16f)(0.0f);
                 mix_rows_product<DW, NG>(e[kb], X + buf * TILE + kb * 32 * DW, own, r, h);
             }
-            if (!second) {
 #pragma unroll
-                for (int kb = 0; kb < KB; kb++)
+            for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-                    for (int v = 0; v < 16; v++) e[kb][v] = __builtin_amdgcn_exp2f(e[kb][v]);
-            }
+                for (int v = 0; v < 16; v++) e[kb][v] = second ? e[kb][v] - own_stat : probability(e[kb][v], own_stat);
             // keys behind a query (or behind the last key), and before its window: tested only where some query has them.
             // Both factors are cleared: dY.V^T may be anything where nothing is seen.
             if (key0 + AK - 1 > w0 || key0 + AK > limit || !span.full) {
@@ -330,13 +332,13 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_kv(const Windo
         const int key = u0 + r;
         const bool live = key < len.vl;
 
-        v4f own[NG];                                                    // K (times scale, in units of log2) or V
+        v4f own[NG];                                                    // K (times scale) or V
         if (second) {
             mix_load_cols<NG>(own, p.V + n * p.v.n + kvh * p.v.h + (size_t)min(key, p.VL - 1) * p.v.l, live, p.dv4, h);
         } else {
             mix_load_cols<NG>(own, p.K + n * p.k.n + kvh * p.k.h + (size_t)min(key, p.VL - 1) * p.k.l, live, p.dk4, h);
 #pragma unroll
-            for (int g = 0; g < NG; g++) own[g] *= p.c;
+            for (int g = 0; g < NG; g++) own[g] *= a.scale;
         }
         // Queries go by in steps of 32 rows, head by head.  Everything that is fetched for a step moves along as an address (a
         // step on, or to the next head's first): so few scalar registers that the compiler keeps the loop's order.
@@ -363,15 +365,15 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_kv(const Windo
             wg.next(lo, hi, 32 * p.y.l, g_jump);
             wq.next(lo, hi, 32 * p.q.l, q_jump);
         };
-        // the statistics of a step's queries, as the products' start: rows 8q + 4h .. +3 (zeros beyond the last of the sequence)
-        v16f start;
+        // lse or D of a step's queries: rows 8q + 4h .. +3 (zeros beyond the last of the sequence)
+        v16f stat;
         auto begin = [&]() {
             const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)ws.at, 0, min(hi - ws.i0, 32) * 4, RSRC_FLAGS);
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 const v4f x = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rs, (8 * q + 4 * h) * 4, 0, 0));
 #pragma unroll
-                for (int w = 0; w < 4; w++) start[4 * q + w] = x[w];
+                for (int w = 0; w < 4; w++) stat[4 * q + w] = x[w];
             }
             ws.next(lo, hi, 32, s_jump);
         };
@@ -389,14 +391,11 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_kv(const Windo
             const int p0 = i0 + off, p1 = min(i0 + 32, hi) - 1 + off;  // the step's positions
             const bool sees = u0 <= u1 && p1 >= u0 && (p0 < u1 + p.window || u0 < p.sinks);
             float* exchange = &Ps[s & 1][block][4 * lane];
-            v16f e = start;
-            if (s + 1 < last) begin();                                  // there when this wavefront waits for its transfers
+            v16f e = (v16f)(0.0f);
             if (sees) {
                 mix_rows_product<DW, NG>(e, X + buf * TILE, own, r, h);
-                if (!second) {
 #pragma unroll
-                    for (int v = 0; v < 16; v++) e[v] = __builtin_amdgcn_exp2f(e[v]);
-                }
+                for (int v = 0; v < 16; v++) e[v] = second ? e[v] - stat[v] : probability(e[v], stat[v]);
                 // queries before a key, those whose window has passed it, and rows behind the last: tested only where there are
                 // any.  Both factors are cleared: dY.V^T may be anything where nothing is seen.
                 if (p0 < u1 || i0 + 32 > hi || u0 + 32 > len.vl) {
@@ -416,6 +415,7 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_kv(const Windo
             mix_wait();
             __syncthreads();
             const int b1 = buf == 2 ? 0 : buf + 1, b2 = b1 == 2 ? 0 : b1 + 1;
+            if (s + 1 < last) begin();                                  // needed behind the next step's first product
             if (s + 2 < last) fetch(b2);
             __builtin_amdgcn_sched_barrier(0);
             if (sees) {
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_grad_sinks(const WindowGra
 #pragma unroll
     for (int s = 0; s < NS; s++) {
         const int d = 16 * s + 4 * k4;
-        kf[s] = (live && d < p.dk4) ? *(const v4f*)(krow + d) * p.c : (v4f)(0.0f);
+        kf[s] = (live && d < p.dk4) ? *(const v4f*)(krow + d) * a.scale : (v4f)(0.0f);
         vf[s] = (live && d < p.dv4) ? *(const v4f*)(vrow + d) : (v4f)(0.0f);
         qa[s] = d < p.dk4 ? (c * p.q.l + d) * 4 : OOB_OFFSET;
         ga[s] = d < p.dv4 ? (c * p.y.l + d) * 4 : OOB_OFFSET;
@@ -503,8 +503,9 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_grad_sinks(const WindowGra
             const __amdgpu_buffer_rsrc_t rg = __builtin_amdgcn_make_buffer_rsrc((void*)(gb + (size_t)i0 * p.y.l), 0, left * p.y.l * 4, RSRC_FLAGS);
             const __amdgpu_buffer_rsrc_t rl = __builtin_amdgcn_make_buffer_rsrc((void*)(sb + i0), 0, left * 4, RSRC_FLAGS);
             const __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc((void*)(sb + a.rows + i0), 0, left * 4, RSRC_FLAGS);
-            v4f s = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rl, 16 * k4, 0, 0));
-            v4f d = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rd, 16 * k4, 0, 0));
+            const v4f lse = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rl, 16 * k4, 0, 0));
+            const v4f D = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rd, 16 * k4, 0, 0));
+            v4f s = (v4f)(0.0f), d = (v4f)(0.0f);
 #pragma unroll
             for (int i = 0; i < NS; i++) {
                 const v4f q = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(rq, qa[i], 0, 0));
@@ -519,8 +520,8 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_grad_sinks(const WindowGra
 #pragma unroll
             for (int v = 0; v < 4; v++) {
                 const bool on = live && 4 * k4 + v < left;
-                s[v] = on ? __builtin_amdgcn_exp2f(s[v]) : 0.0f;
-                d[v] = on ? s[v] * d[v] : 0.0f;
+                s[v] = on ? probability(s[v], lse[v]) : 0.0f;
+                d[v] = on ? s[v] * (d[v] - D[v]) : 0.0f;
             }
 #pragma unroll
             for (int v = 0; v < 4; v++)
