@@ -177,12 +177,13 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_q(const Window
     v16f o[DC];
 #pragma unroll
     for (int b = 0; b < DC; b++) o[b] = (v16f)(0.0f);
-    if (steps > 0) fetch(0, 0);
+    const int first = (int)((long long)steps * job.part / p.parts), last = (int)((long long)steps * (job.part + 1) / p.parts);
+    if (first < last) fetch(first, 0);
     mix_wait();
-    if (steps > 1) fetch(1, 1);
+    if (first + 1 < last) fetch(first + 1, 1);
     __syncthreads();
     int buf = 0;
-    for (int s = 0; s < steps; s++) {
+    for (int s = first; s < last; s++) {
         const int key0 = key_of(s), limit = s < nsink ? range.sink_end : range.hi, end = min(key0 + AK, limit);
         const bool sees = w0 <= w1 && (s < nsink || (key0 <= w1 && (end - 1 > w0 - p.window || key0 < p.sinks)));
         float* exchange = &Ps[s & 1][block][4 * lane];
@@ -223,7 +224,7 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_q(const Window
         mix_wait();
         __syncthreads();
         const int b1 = buf == 2 ? 0 : buf + 1, b2 = b1 == 2 ? 0 : b1 + 1;
-        if (s + 2 < steps) fetch(s + 2, b2);
+        if (s + 2 < last) fetch(s + 2, b2);
         __builtin_amdgcn_sched_barrier(0);
         if (sees && second) {
 #pragma unroll
@@ -234,7 +235,25 @@ __global__ __launch_bounds__(GT, DB > 2 ? 2 : 4) void window_grad_q(const Window
         }
         buf = b1;
     }
-    if (second && row.exists) mix_store_row<DC>(a.dQ + job.n * p.q.n + row.hd * p.q.h + (size_t)row.i * p.q.l, o, a.scale, p.dk4, h);
+    if (second && row.exists) {
+        float* const out = p.parts == 1 ? a.dQ + job.n * p.q.n + row.hd * p.q.h + (size_t)row.i * p.q.l
+                                        : p.part + (stat * p.parts + job.part) * p.dk4;
+        mix_store_row<DC>(out, o, p.parts == 1 ? a.scale : 1.0f, p.dk4, h);
+    }
+}
+// dQ from the parts that the keys were cut into, in order: 4 floats a thread
+__device__ __forceinline__ void window_grad_join_q(const WindowGrad& a, long long x) {
+    const WindowParams& p = a.w;
+    const int per = p.dk4 / 4;
+    const long long row = x / per;
+    if (row >= a.rows) return;
+    const int d = 4 * (int)(x - row * per), i = (int)(row % p.QL), hd = (int)(row / p.QL % p.head);
+    const long long n = row / p.QL / p.head;
+    const float* const part = p.part + row * p.parts * p.dk4 + d;
+    v4f s = *(const v4f*)part;
+#pragma unroll 4
+    for (int k = 1; k < p.parts; k++) s += *(const v4f*)(part + (size_t)k * p.dk4);
+    *(v4f*)(a.dQ + n * p.q.n + hd * p.q.h + (size_t)i * p.q.l + d) = s * a.scale;
 }
 
 // ---------------------------------------------------------------- dK, dV
@@ -559,10 +578,14 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_grad_sinks(const WindowGra
 
 // ---------------------------------------------------------------- everything that a key's gradient is made of
 // Four workgroups per tile and key / value head: the tile's pieces in order, or what was written whole, or zeros where no
-// query sees it; then the sinks' parts in order.
+// query sees it; then the sinks' parts in order.  The workgroups behind them join dQ where the keys were cut.
 __global__ __launch_bounds__(NTHREADS) void window_grad_join(const WindowGrad a) {
     const WindowParams& p = a.w;
     const long long at = blockIdx.x / p.kv_head;
+    if (at >= (long long)p.N * a.ktiles) {
+        window_grad_join_q(a, ((blockIdx.x - (long long)p.N * a.ktiles * p.kv_head) * 4 + blockIdx.y) * NTHREADS + threadIdx.x);
+        return;
+    }
     const int kvh = (int)(blockIdx.x - at * p.kv_head), n = (int)(at / a.ktiles), k0 = (int)(at - (long long)n * a.ktiles) * GK;
     const bool some = a.before[at + 1] != a.before[at];
     const int2 cut = some ? a.cut[at * p.kv_head + kvh] : make_int2(0, 0);
@@ -593,9 +616,20 @@ __global__ __launch_bounds__(NTHREADS) void window_grad_join(const WindowGrad a)
 }
 
 // ---------------------------------------------------------------- host side
-// The caller's buffer, in floats: the statistics, the running sum (64-bit), the pieces and whose they are, the sinks' parts.
+// Cuts of the keys of window_grad_q: where the tiles are fewer than half of the workgroups that the compute units hold, each
+// tile's keys are walked over by several, at least 4 steps each, whose sums window_grad_join adds in order.
+int window_grad_parts(int N, int head, int kv_head, int QL, int VL, int workers, int window, int sinks) {
+    const long long group = head / kv_head, base = (long long)N * kv_head * ((QL * group + GQ - 1) / GQ);
+    const long long reach = window == 0 ? VL : (long long)window + sinks + (GQ + group - 1) / group;
+    const long long steps = ((reach < VL ? reach : VL) + 31) / 32;
+    long long parts = base >= workers / 2 ? 1 : (workers + base - 1) / base;
+    if (parts > steps / 4) parts = steps / 4;
+    return (int)(parts < 1 ? 1 : parts);
+}
+// The caller's buffer, in floats: the statistics, the running sum (64-bit), the pieces and whose they are, the sinks' parts,
+// the parts of dQ.
 constexpr int SINKS_APART = 64;      // up to here window_grad_sinks takes the queries beyond the window
-struct WindowGradBuffer { int ktiles, workers, sink_blocks, sink_parts; long long stats, before, pieces, cut, sinks, all; };
+struct WindowGradBuffer { int ktiles, workers, sink_blocks, sink_parts, parts; long long stats, before, pieces, cut, sinks, all; };
 WindowGradBuffer window_grad_buffer(int N, int head, int kv_head, int QL, int VL, int dk4, int dv4, int window, int sinks) {
     WindowGradBuffer b;
     b.ktiles = (VL + GK - 1) / GK;
@@ -608,7 +642,8 @@ WindowGradBuffer window_grad_buffer(int N, int head, int kv_head, int QL, int VL
     b.pieces = 2LL * b.workers * GK * (dk4 + dv4);
     b.cut = ((long long)N * b.ktiles * kv_head * 2 + 3) / 4 * 4;
     b.sinks = (long long)N * kv_head * b.sink_blocks * b.sink_parts * 16 * (dk4 + dv4);
-    b.all = b.stats + b.before + b.pieces + b.cut + b.sinks;
+    b.parts = window_grad_parts(N, head, kv_head, QL, VL, b.workers, window, sinks);
+    b.all = b.stats + b.before + b.pieces + b.cut + b.sinks + (b.parts > 1 ? (long long)N * head * QL * b.parts * dk4 : 0);
     return b;
 }
 
@@ -652,7 +687,7 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
     p.window = window == 0 || window > QL + VL ? QL + VL : window;
     p.sinks = sinks;
     p.c = scale * MIX_LOG2E;
-    p.qtiles = (int)(((long long)QL * (head / kv_head) + GQ - 1) / GQ); p.parts = 1; p.part = nullptr;
+    p.qtiles = (int)(((long long)QL * (head / kv_head) + GQ - 1) / GQ); p.parts = b.parts;
     a.dY = (const float*)(intptr_t)dDeltaY;
     a.dQ = (float*)(intptr_t)dDeltaQ; a.dK = (float*)(intptr_t)dDeltaK; a.dV = (float*)(intptr_t)dDeltaV;
     a.stats = (float*)(intptr_t)dBuf;
@@ -664,6 +699,7 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
     a.pieces = a.stats + b.stats + b.before;
     a.cut = (int2*)(a.pieces + b.pieces);
     a.sinks = a.pieces + b.pieces + b.cut;
+    p.part = a.sinks + b.sinks;
     a.sink_blocks = b.sink_blocks; a.sink_parts = b.sink_parts;
     split_ledger_touch(a.dQ, (size_t)N * head * QL * dK4 * 4);
     split_ledger_touch(a.dK, (size_t)N * kv_head * VL * dK4 * 4);
@@ -675,7 +711,7 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
     hipLaunchKernelGGL(window_delta, dim3((unsigned)((a.rows + NTHREADS / 32 - 1) / (NTHREADS / 32) + 1)), block, 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const dim3 gq((unsigned)((long long)N * kv_head * p.qtiles)), gk((unsigned)b.workers);
+    const dim3 gq((unsigned)((long long)N * kv_head * p.qtiles * p.parts)), gk((unsigned)b.workers);
     const int dmax = dK4 > dV4 ? dK4 : dV4;
 #define GRAD_CASE(DB_, DC_, B_)                                                        \
     do {                                                                              \
@@ -700,7 +736,8 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
         e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(window_grad_join, dim3((unsigned)((long long)N * b.ktiles * kv_head), 4), block, 0, s, a);
+    const long long join_q = p.parts == 1 ? 0 : (a.rows * (dK4 / 4) + 4 * NTHREADS - 1) / (4 * NTHREADS);
+    hipLaunchKernelGGL(window_grad_join, dim3((unsigned)((long long)N * b.ktiles * kv_head + join_q), 4), block, 0, s, a);
     e = hipGetLastError();
     return e;
 }
