@@ -350,7 +350,9 @@ constexpr int ROWS_MAX = 32;         // rows of a key / value head up to which w
 
 struct WindowPlan { bool rows; int qtiles, parts; };
 
-// One decision for the launch and for the size of the caller's buffer: from the sizes alone.
+// One decision for the launch and for the size of the caller's buffer: from the sizes alone.  The keys are cut where the tiles
+// are fewer than half of the workgroups wanted; where tiles of 128 rows see everything before them, and so differ by the
+// sequence, up to all of them (256 tiles of 64 columns: 78 -> 65 us, 320 of 128: 164 -> 123; cut for twice as many: 131).
 WindowPlan window_plan(int N, int head, int kv_head, int QL, int VL, int window, int sinks) {
     WindowPlan x;
     const long long group = head / kv_head, rows = QL * group;
@@ -361,7 +363,7 @@ WindowPlan window_plan(int N, int head, int kv_head, int QL, int VL, int window,
     const long long reach = window == 0 ? VL : (long long)window + sinks + (per + group - 1) / group;
     const long long steps = ((reach < VL ? reach : VL) + (x.rows ? 15 : 31)) / (x.rows ? 16 : 32);
     const long long want = x.rows ? 1024 : 512, least = x.rows ? 16 : 4;   // workgroups on the chip; steps worth a part
-    long long parts = base >= want / 2 ? 1 : (want + base - 1) / base;
+    long long parts = base >= (x.rows || reach < VL ? want / 2 : want) ? 1 : (want + base - 1) / base;
     if (parts > steps / least) parts = steps / least;
     x.parts = (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
     return x;

@@ -616,14 +616,17 @@ __global__ __launch_bounds__(NTHREADS) void window_grad_join(const WindowGrad a)
 }
 
 // ---------------------------------------------------------------- host side
-// Cuts of the keys of window_grad_q: where the tiles are fewer than half of the workgroups that the compute units hold, each
-// tile's keys are walked over by several, at least 4 steps each, whose sums window_grad_join adds in order.
+// Cuts of the keys of window_grad_q: where the tiles are few, several workgroups walk over a tile's keys, at least 2 steps each,
+// and window_grad_join adds their sums in order (7 x 1023 queries of one head of 112: 198 -> 50 us; one head of 4096 of 64:
+// 430 -> 47).  Few is half of what the compute units hold under a window, all of it where the tiles see everything before
+// them and differ by the sequence: cut there, 256 tiles of 64 take 303 us with everything around them instead of 332, but 184
+// -> 187 under a window of 256; cut for twice as many, 192 tiles of 128 take 404 us instead of 393.
 int window_grad_parts(int N, int head, int kv_head, int QL, int VL, int workers, int window, int sinks) {
     const long long group = head / kv_head, base = (long long)N * kv_head * ((QL * group + GQ - 1) / GQ);
     const long long reach = window == 0 ? VL : (long long)window + sinks + (GQ + group - 1) / group;
     const long long steps = ((reach < VL ? reach : VL) + 31) / 32;
-    long long parts = base >= workers / 2 ? 1 : (workers + base - 1) / base;
-    if (parts > steps / 4) parts = steps / 4;
+    long long parts = base >= (reach < VL ? workers / 2 : workers) ? 1 : (workers + base - 1) / base;
+    if (parts > steps / 2) parts = steps / 2;
     return (int)(parts < 1 ? 1 : parts);
 }
 // The caller's buffer, in floats: the statistics, the running sum (64-bit), the pieces and whose they are, the sinks' parts,
