@@ -41,6 +41,7 @@ WINDOW = [
     (1, 1, 1, 300, 2500, 64, 64, 0, 0, None, None),                # keys cut into parts, tiles
     (2, 4, 2, 300, 300, 80, 80, 128, 200, None, [300, 260]),       # fewer keys than queries in one; sinks in two key tiles
     (1, 6, 1, 520, 520, 128, 64, 33, 40, None, None),
+    (12, 8, 8, 500, 500, 16, 16, 40, 2, None, None),               # many tiles: nothing is cut, in either direction
 ]
 
 
