@@ -40,8 +40,9 @@ struct DecayWalk {
 };
 
 __device__ __forceinline__ float decay_log2(const float* g, int hd) {
-    // not below -1e30: 0 * g has to be 0 where the head forgets at once (g = -infinity)
-    return fmaxf(g[hd] * MIX_LOG2E, -1.0e30f);
+    // not below -1e30: 0 * g has to be 0 where the head forgets at once (g = -infinity); NaN stays NaN
+    const float g2 = g[hd] * MIX_LOG2E;
+    return g2 < -1.0e30f ? -1.0e30f : g2;
 }
 __device__ __forceinline__ float decay_pow(float g2, int n) { return __builtin_amdgcn_exp2f(g2 * (float)n); }
 __device__ __forceinline__ int decay_len(const int* lens, int n, int L) { return lens ? min(max(lens[n], 0), L) : L; }

@@ -306,7 +306,8 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
  * [N, head, dK4, dV4], or 0 for zeros; dStateOut: S after the last, or 0 if nobody wants it.  A call with L tokens and one
  * with the next tokens and the first one's dStateOut as dState give what one call with all of them gives.  Up to 12 tokens
  * the recurrence is computed as it stands, beyond that 32 tokens at a time, the sequence cut into segments where there are few
- * heads (only these take a work buffer). */
+ * heads (only these take a work buffer).  Operands are finite: a NaN or an infinity in a token can reach the rows of up to 31
+ * tokens before it (and in the gradient behind it); a decay that is NaN makes its head's results NaN. */
 int64_t dragon_Cuda_linear_attention_bufsize(int32_t N, int32_t head, int32_t L, int32_t dK4, int32_t dV4);
 int dragon_Cuda_linear_attention_forward(const int64_t* streams, int32_t length, int64_t dQ, int64_t dK, int64_t dV,
                                          int64_t dDecay, int64_t dState, int64_t dY, int64_t dStateOut, int64_t dLens,

@@ -174,6 +174,19 @@ def test_decay_that_forgets_at_once_or_never(dh, gpu, g):
         check(got, decay_reference(Q, K, V, [g], 0.5, [L], S0, dY, dS1), "g %g, L %d" % (g, L))
 
 
+@pytest.mark.parametrize("L", (3, 100, 700))
+def test_decay_that_is_no_number(dh, gpu, L):
+    rng = np.random.default_rng(L)
+    f = lambda *s: rng.standard_normal(s).astype(np.float32)
+    Q, K, V, S0 = f(1, 3, L, 32), f(1, 3, L, 32), f(1, 3, L, 32), f(1, 3, 32, 32)
+    g = np.array([-0.1, np.nan, -0.2], np.float32)
+    got = run_decay(dh, Q, K, V, g, 0.2, None, S0)
+    assert np.isnan(got["Y"][:, 1]).all() and np.isnan(got["S1"][:, 1]).all()
+    keep = [0, 2]
+    want = decay_reference(Q[:, keep], K[:, keep], V[:, keep], g[keep], 0.2, [L], S0[:, keep])
+    check({name: got[name][:, keep] for name in ("Y", "S1")}, want)
+
+
 def test_decay_state_in_place(dh, gpu):
     rng = np.random.default_rng(12)
     for L in (1, 12, 200):
