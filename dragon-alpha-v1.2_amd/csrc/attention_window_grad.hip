@@ -12,7 +12,6 @@
 // ran alone on its SIMD and left the matrix pipe idle for half of the time: dK and dV at 32 x 8192 x 128 under a window of
 // 1024 in 3.3 ms.)  One barrier a step, between the products: behind it P is there, the next step's tiles have landed, and
 // those of the step before are free, so three buffers.
-//
 #include "token_mixer.h"
 #include "attention_window.h"
 #include "runtime_internal.h"
@@ -657,7 +656,10 @@ struct WindowGradBuffer { int ktiles, workers, sink_blocks, sink_parts, parts; l
 WindowGradBuffer window_grad_buffer(int N, int head, int kv_head, int QL, int VL, int dk4, int dv4, int window, int sinks) {
     WindowGradBuffer b;
     b.ktiles = (VL + GK - 1) / GK;
-    b.workers = (dk4 > dv4 ? dk4 : dv4) > 64 ? UNITS : 2 * UNITS;             // as many as the compute units hold
+    // as many workers as the compute units hold, or as there are tiles or runs of 4 steps
+    const long long hold = (dk4 > dv4 ? dk4 : dv4) > 64 ? UNITS : 2 * UNITS, tiles = (long long)N * b.ktiles * kv_head;
+    const long long runs = tiles * (head / kv_head) * ((QL + 31LL) / 32) / 4, most = tiles > runs ? tiles : runs;
+    b.workers = (int)(most < hold ? most : hold);
     const bool apart = window != 0 && window < VL && sinks > 0 && sinks <= SINKS_APART;
     b.sink_blocks = apart ? ((sinks < VL ? sinks : VL) + 15) / 16 : 0;
     b.sink_parts = apart ? (QL + SINK_QUERIES - 1) / SINK_QUERIES : 0;
@@ -666,7 +668,7 @@ WindowGradBuffer window_grad_buffer(int N, int head, int kv_head, int QL, int VL
     b.pieces = 2LL * b.workers * GK * (dk4 + dv4);
     b.cut = ((long long)N * b.ktiles * kv_head * 2 + 3) / 4 * 4;
     b.sinks = (long long)N * kv_head * b.sink_blocks * b.sink_parts * 16 * (dk4 + dv4);
-    b.parts = window_grad_parts(N, head, kv_head, QL, VL, b.workers, window, sinks);
+    b.parts = window_grad_parts(N, head, kv_head, QL, VL, (int)hold, window, sinks);
     b.all = b.stats + b.before + b.pieces + b.cut + b.sinks + (b.parts > 1 ? (long long)N * head * QL * b.parts * dk4 : 0);
     return b;
 }
