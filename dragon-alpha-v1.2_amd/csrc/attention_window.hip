@@ -323,22 +323,44 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_rows(const WindowParams p)
 }
 
 // ---------------------------------------------------------------- the parts of a row, added in order
-__global__ __launch_bounds__(NTHREADS) void window_join(const WindowParams p) {
-    const int per = p.dv4 / 4;
-    const long long x = (long long)blockIdx.x * NTHREADS + threadIdx.x;
-    const long long stat = x / per;
-    if (stat >= (long long)p.N * p.head * p.QL) return;
-    const int d = 4 * (int)(x - stat * per);
-    float M = NEG;
-    for (int s = 0; s < p.parts; s++) M = fmaxf(M, p.part_ml(stat, s).x);
-    float L = 0.0f;
+// `wide` threads (16 or 32) for a row's columns, `across` of such groups (a power of two up to 8) next to each other for its
+// parts: a thread adds every across-th part, LDS joins the rest.  With few rows and many parts one thread for all of them
+// would read one after the other: 64 parts of 32 rows in 22.3 us, so in 4.7.
+__global__ __launch_bounds__(NTHREADS) void window_join(const WindowParams p, int wide, int across) {
+    __shared__ __attribute__((aligned(16))) v4f Sy[NTHREADS];
+    __shared__ float2 Sml[NTHREADS / 16];
+    const int t = threadIdx.x, slot = t / wide, sub = slot & (across - 1), d = 4 * (t & (wide - 1));
+    const long long stat = (long long)blockIdx.x * (NTHREADS / wide / across) + slot / across;
+    const bool mine = stat < (long long)p.N * p.head * p.QL && d < p.dv4;
+    float M = NEG, L = 0.0f;
     v4f y = (v4f)(0.0f);
-    for (int s = 0; s < p.parts; s++) {
-        const float2 ml = p.part_ml(stat, s);
-        const float f = ml.x == NEG ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
-        L += ml.y * f;
-        y += *(const v4f*)(p.part_o(stat, s) + d) * f;
+    if (mine) {
+#pragma unroll 4
+        for (int s = sub; s < p.parts; s += across) M = fmaxf(M, p.part_ml(stat, s).x);
+#pragma unroll 4
+        for (int s = sub; s < p.parts; s += across) {
+            const float2 ml = p.part_ml(stat, s);
+            const float f = ml.x == NEG ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
+            L += ml.y * f;
+            y += *(const v4f*)(p.part_o(stat, s) + d) * f;
+        }
     }
+    if (across > 1) {
+        Sy[t] = y;
+        if (d == 0) Sml[slot] = make_float2(M, L);
+        __syncthreads();
+        if (sub != 0) return;
+        for (int s = 1; s < across; s++) M = fmaxf(M, Sml[slot + s].x);
+        L = 0.0f;
+        y = (v4f)(0.0f);
+        for (int s = 0; s < across; s++) {
+            const float2 ml = Sml[slot + s];
+            const float f = ml.x == NEG ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
+            L += ml.y * f;
+            y += Sy[t + s * wide] * f;
+        }
+    }
+    if (!mine) return;
     const long long nh = stat / p.QL;
     const int n = (int)(nh / p.head), hd = (int)(nh - (long long)n * p.head), i = (int)(stat - nh * p.QL);
     *(v4f*)(p.Y + n * p.y.n + hd * p.y.h + (size_t)i * p.y.l + d) = L == 0.0f ? (v4f)(0.0f) : y * (1.0f / L);
@@ -346,6 +368,7 @@ __global__ __launch_bounds__(NTHREADS) void window_join(const WindowParams p) {
 }
 
 // ---------------------------------------------------------------- host side
+constexpr long long JOIN_ROWS = 1024;    // rows from which a thread of window_join takes all parts (500 x 8 rows: 63 us, else 67)
 constexpr int ROWS_MAX = 32;         // rows of a key / value head up to which window_rows takes the call
 
 struct WindowPlan { bool rows; int qtiles, parts; };
@@ -353,6 +376,9 @@ struct WindowPlan { bool rows; int qtiles, parts; };
 // One decision for the launch and for the size of the caller's buffer: from the sizes alone.  The keys are cut where the tiles
 // are fewer than half of the workgroups wanted; where tiles of 128 rows see everything before them, and so differ by the
 // sequence, up to all of them (256 tiles of 64 columns: 78 -> 65 us, 320 of 128: 164 -> 123; cut for twice as many: 131).
+// A part of window_rows is worth its launch of window_join from 8 steps on, if there are 24 to cut: one token on 1024 keys of 4
+// heads of 64 in 10.0 us (cuts of 16: 11.2), but on 256 keys 7.9 whole and 9.4 cut.  More parts than compute units gain nothing
+// there (16384 keys of 8 heads of 128: 29 us, with twice as many 33).
 WindowPlan window_plan(int N, int head, int kv_head, int QL, int VL, int window, int sinks) {
     WindowPlan x;
     const long long group = head / kv_head, rows = QL * group;
@@ -362,7 +388,7 @@ WindowPlan window_plan(int N, int head, int kv_head, int QL, int VL, int window,
     const long long base = (long long)N * kv_head * x.qtiles;
     const long long reach = window == 0 ? VL : (long long)window + sinks + (per + group - 1) / group;
     const long long steps = ((reach < VL ? reach : VL) + (x.rows ? 15 : 31)) / (x.rows ? 16 : 32);
-    const long long want = x.rows ? 1024 : 512, least = x.rows ? 16 : 4;   // workgroups on the chip; steps worth a part
+    const long long want = x.rows ? 256 : 512, least = x.rows ? (steps < 24 ? 24 : 8) : 4;   // workgroups on the chip; steps worth a part
     long long parts = base >= (x.rows || reach < VL ? want / 2 : want) ? 1 : (want + base - 1) / base;
     if (parts > steps / least) parts = steps / least;
     x.parts = (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
@@ -434,7 +460,7 @@ int dragon_Cuda_attention_window_forward(const int64_t* streams, int32_t length,
     const dim3 grid((unsigned)((long long)N * kv_head * plan.qtiles * plan.parts));
     if (plan.rows) {
         // keys and values that are read once and do not fit the Infinity Cache pass it by (stream_policy.h has the border):
-        // 65536 keys of 8 heads of 128 in 105 us instead of 121, but 4 x 8192 in 62 instead of 59
+        // 65536 keys of 8 heads of 128 in 84 us instead of 96, but 16 x 2048 in 66 instead of 50
         const long long reach = window == 0 || window > VL ? VL : (long long)window + sinks;
         const bool nt = plan.qtiles == 1 && (long long)N * kv_head * (reach < VL ? reach : VL) * (dK4 + dV4) * 4 >= STREAM_NT_BYTES;
         if (dmax <= 64) {
@@ -454,8 +480,9 @@ int dragon_Cuda_attention_window_forward(const int64_t* streams, int32_t length,
     }
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && plan.parts > 1) {
-        const long long items = (long long)N * head * QL * (dV4 / 4);
-        hipLaunchKernelGGL(window_join, dim3((unsigned)((items + NTHREADS - 1) / NTHREADS)), block, 0, s, p);
+        const int across = (long long)N * head * QL >= JOIN_ROWS ? 1 : plan.parts >= 8 ? 8 : plan.parts >= 4 ? 4 : 2;
+        const int wide = dV4 <= 64 ? 16 : 32, rows = NTHREADS / wide / across;
+        hipLaunchKernelGGL(window_join, dim3((unsigned)(((long long)N * head * QL + rows - 1) / rows)), block, 0, s, p, wide, across);
         e = hipGetLastError();
     }
     return e;
