@@ -9,9 +9,11 @@
 //   window_tiles: 128 (query, head) rows of one key / value head per workgroup, the keys they see in steps, S^T = K.Q^T and Y^T = V^T.P^T with
 //     v_mfma_f32_32x32x2_f32 and a running maximum and sum per query (token_mixer.h has the register layouts).  The steps
 //     are the sinks below the window's reach, then the keys from the first one that some query of the tile sees: no other
-//     key is read.  Bound by the FP32 matrix pipe.
+//     key is read.  Bound by the FP32 matrix pipe: 16384 queries of 8 heads of 128 under a window of 2048 in 1.01 ms, 128
+//     TFLOP/s of what they see, the pipes busy for 83 % of the time (the rest: the softmax's vector instructions, the barrier).
 //   window_rows: up to 16 (query, head) rows that share a key / value head per wavefront; keys and values go from memory
-//     straight into v_mfma_f32_16x16x4_f32 operands, 16 keys at a time.  Bound by reading K and V.
+//     straight into v_mfma_f32_16x16x4_f32 operands, 16 keys at a time.  Bound by reading K and V: 64 sequences of 8 heads of
+//     128 under a window of 4096 in 281 us, 5.8 TB/s.
 // Where either leaves compute units idle the keys are cut: every part leaves its maximum, sum and un-normalised output in the
 // caller's buffer and window_join adds them in order (a second launch, so the result does not depend on who is last).
 #include "token_mixer.h"
@@ -369,13 +371,15 @@ __global__ __launch_bounds__(NTHREADS) void window_join(const WindowParams p, in
 
 // ---------------------------------------------------------------- host side
 constexpr long long JOIN_ROWS = 1024;    // rows from which a thread of window_join takes all parts (500 x 8 rows: 63 us, else 67)
-constexpr int ROWS_MAX = 32;         // rows of a key / value head up to which window_rows takes the call
+// Rows of a key / value head up to which window_rows takes the call.  64 rows on 16 x 8192 keys of 8 heads of 128 under a window
+// of 1024: 51 us (window_tiles 79), on 8 x 4096 all: 97 (136); but 72 rows on 2 x 4096: 52 (49), 96 rows: 64 (51).
+constexpr int ROWS_MAX = 64;
 
 struct WindowPlan { bool rows; int qtiles, parts; };
 
-// One decision for the launch and for the size of the caller's buffer: from the sizes alone.  The keys are cut where the tiles
-// are fewer than half of the workgroups wanted; where tiles of 128 rows see everything before them, and so differ by the
-// sequence, up to all of them (256 tiles of 64 columns: 78 -> 65 us, 320 of 128: 164 -> 123; cut for twice as many: 131).
+// One decision for the launch and for the size of the caller's buffer: from the sizes alone.  The keys are cut where there are
+// fewer workgroups than wanted; for tiles of 128 rows under a window, which differ little, fewer than half of them.  (Tiles that
+// see everything before them: 256 tiles of 64 columns 78 -> 65 us, 320 of 128: 164 -> 123; cut for twice as many: 131.)
 // A part of window_rows is worth its launch of window_join from 8 steps on, if there are 24 to cut: one token on 1024 keys of 4
 // heads of 64 in 10.0 us (cuts of 16: 11.2), but on 256 keys 7.9 whole and 9.4 cut.  More parts than compute units gain nothing
 // there (16384 keys of 8 heads of 128: 29 us, with twice as many 33).
@@ -389,7 +393,7 @@ WindowPlan window_plan(int N, int head, int kv_head, int QL, int VL, int window,
     const long long reach = window == 0 ? VL : (long long)window + sinks + (per + group - 1) / group;
     const long long steps = ((reach < VL ? reach : VL) + (x.rows ? 15 : 31)) / (x.rows ? 16 : 32);
     const long long want = x.rows ? 256 : 512, least = x.rows ? (steps < 24 ? 24 : 8) : 4;   // workgroups on the chip; steps worth a part
-    long long parts = base >= (x.rows || reach < VL ? want / 2 : want) ? 1 : (want + base - 1) / base;
+    long long parts = base >= (!x.rows && reach < VL ? want / 2 : want) ? 1 : (want + base - 1) / base;
     if (parts > steps / least) parts = steps / least;
     x.parts = (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
     return x;

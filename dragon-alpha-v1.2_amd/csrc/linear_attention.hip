@@ -2,13 +2,16 @@
 //     S_t = e^g S_{t-1} + K[t]^T V[t],     Y[t] = scale * Q[t] S_t            (g <= 0, one per head)
 // and its gradient.
 //
-// Few tokens (decay_steps): the recurrence itself, the state in registers; bound by reading and writing the states.
+// Few tokens (decay_steps): the recurrence itself, the state in registers; bound by reading and writing the states: a token of
+// 256 x 32 states of 128 x 128 in 190 us, 5.7 TB/s.
 // Many tokens (decay_walk): 32 at a time.  With S the state before them and t a token's place among them,
 //     Y[t] = scale * (e^{g(t+1)} Q[t] S  +  sum_{j <= t} e^{g(t-j)} <Q[t], K[j]> V[j]),    S' = e^{32g} S + sum_j e^{g(31-j)} K[j]^T V[j]
 // A workgroup walks along a sequence with the state in its registers, a wavefront for each 32 columns of V.  Where there are
 // fewer (image, head) pairs than the chip takes workgroups the sequence is cut into segments that walk at the same time:
 // decay_states forms each segment's own sum, decay_scan runs over them and leaves the state that each begins with.
-// Bound by the FP32 matrix pipe: 2.5 products of [dk, dv] size a token, and one more where there are segments.
+// Bound by the FP32 matrix pipe: 2.5 products of [dk, dv] size a token, and one more where there are segments.  16 heads of 128
+// and 32768 tokens: the states 155 us (111 TFLOP/s), the scan 13, the walk 400 to 420 (103), the pipes busy for 74 % of both; the
+// rest of the walk goes to vector instructions (powers, decay of the state) and to two barriers for 32 tokens.
 //
 // The gradient is the same walk with other operands (G = gradient of Y, sums over j >= t in the last two, from the end):
 //     dQ[t] = scale sum e^{g(t-j)} <G[t], V[j]> K[j] + ...  S^T           the states of the forward pass again
