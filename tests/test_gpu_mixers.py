@@ -41,6 +41,12 @@ WINDOW = [
     (1, 1, 1, 300, 2500, 64, 64, 0, 0, None, None),                # keys cut into parts, tiles
     (2, 4, 2, 300, 300, 80, 80, 128, 200, None, [300, 260]),       # fewer keys than queries in one; sinks in two key tiles
     (1, 6, 1, 520, 520, 128, 64, 33, 40, None, None),
+    (2, 64, 1, 1, 430, 64, 64, 50, 3, None, [430, 31]),            # 64 rows on one head
+    (2, 6, 2, 20, 300, 36, 100, 40, 2, [20, 7], [300, 299]),       # 60 rows, ragged
+    (1, 13, 1, 5, 1000, 128, 128, 0, 3, None, None),               # 65 rows: a tile
+    (1, 4, 2, 1, 400, 128, 128, 0, 0, None, None),                 # cut in three
+    (1, 4, 4, 300, 2500, 96, 72, 0, 0, None, None),                # cut, and many rows to join
+    (1, 2, 1, 150, 150, 32, 32, 1000, 5, None, None),              # a window beyond the sequence
     (12, 8, 8, 500, 500, 16, 16, 40, 2, None, None),               # many tiles: nothing is cut, in either direction
 ]
 
