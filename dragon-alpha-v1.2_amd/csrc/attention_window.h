@@ -13,12 +13,7 @@ struct WindowParams {
     int window, sinks;                       // window >= 1 (all keys: the host passes more than there are positions)
     float c;                                 // scale * log2(e): the exponentials are base 2
     int qtiles, parts;                       // workgroups along the rows; cuts of the keys
-    float* part;                             // parts > 1: the parts' outputs, behind them their (maximum, sum)
-
-    __device__ __forceinline__ float* part_o(size_t row, int s) const { return part + (row * parts + s) * dv4; }
-    __device__ __forceinline__ float2& part_ml(size_t row, int s) const {
-        return ((float2*)(part + (size_t)N * head * QL * parts * dv4))[row * parts + s];
-    }
+    float* part;                             // parts > 1: the parts' results (attention_window.hip, attention_window_grad.hip)
 };
 
 // (n is the same for the whole wavefront wherever this is called but in window_delta, which has lengths of its own)

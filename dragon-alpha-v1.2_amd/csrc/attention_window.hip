@@ -30,19 +30,130 @@ constexpr int LAG = 8;           // the reference maximum may lag the true one b
 constexpr float NEG = -__builtin_inff();
 constexpr float LOWEST = -3.402823466e38f;   // not above any score but -infinity
 
+// ---------------------------------------------------------------- the keys cut into parts
+// A launch has N * kv_head * qtiles * parts workgroups, from the capacities: `parts` for each tile.  Where the sequences have
+// lengths window_tiles deals them by the steps that a tile has, so that the longest part is as short as can be: pieces of 500 and
+// 250 on 9000 and 4500 keys of 16 heads of 96 in 305 us instead of 418, prompts of 1000 to 250 of 8 heads of 64 in 47 instead of
+// 65.  Every wavefront works the deal out for itself, a pair (tile, sequence) a lane; the first workgroup of a pair writes it
+// down for window_join.  (window_rows reads so little that the deal costs it more: 16.2 -> 17.8 us at 8 sequences of up to 4096.)
+constexpr int PAIRS = 512;      // at most, where there are parts (window_plan)
+struct WindowCutting {
+    int per, ak, least, want;   // rows of a tile, keys of a step, steps worth a part, workgroups on the chip
+    bool deal;                  // parts by length
+};
+constexpr WindowCutting ROWS_CUTTING = {16, 16, 8, 256, false};
+__host__ __device__ constexpr WindowCutting tile_cutting(int ak, bool deal) { return {AQ, ak, 4, 512, deal}; }
+
+// the steps of pair x = (qtiles - 1 - tile) * N + sequence: tiles at the sequences' ends first
+__device__ __forceinline__ int window_pair_steps(const WindowParams& p, const WindowCutting& c, int x) {
+    const int q = x / p.N, n = x - q * p.N, row0 = (p.qtiles - 1 - q) * c.per, group = p.head / p.kv_head;
+    const int ql = p.QLens ? min(max(p.QLens[n], 0), p.QL) : p.QL, vl = p.VLens ? min(max(p.VLens[n], 0), p.VL) : p.VL;
+    const int end = min(row0 + c.per, ql * group), off = vl - ql;
+    const WindowRange range = window_range(p, row0 / group + off, (end - 1) / group + off, end > row0, vl);
+    return (range.sink_end + c.ak - 1) / c.ak + (max(range.hi - range.low, 0) + c.ak - 1) / c.ak;
+}
+// sum over this lane and those below it
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);      // the lane 1 below, in rows of 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);      // the last lane of row 0 to row 1, of 2 to 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);      // of row 1 to rows 2 and 3
+    return x;
+}
+__device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+
+// what a part's row leaves: its output, its (maximum, sum); behind them {first slot, parts} of every pair
+__device__ __forceinline__ float* window_part_o(const WindowParams& p, const WindowCutting& c, int slot, int row) {
+    return p.part + ((size_t)slot * c.per + row) * p.dv4;
+}
+__device__ __forceinline__ float2& window_part_ml(const WindowParams& p, const WindowCutting& c, int slot, int row) {
+    return ((float2*)(p.part + (size_t)p.N * p.kv_head * p.qtiles * p.parts * c.per * p.dv4))[(size_t)slot * c.per + row];
+}
+__device__ __forceinline__ int2& window_part_deal(const WindowParams& p, const WindowCutting& c, int pair) {
+    return ((int2*)(p.part + (size_t)p.N * p.kv_head * p.qtiles * p.parts * c.per * (p.dv4 + 2)))[pair];
+}
+
+// a workgroup's tile and its part of that tile's keys; slot: where its results go.  none: a workgroup too many
+struct WindowPart { WindowJob job; int parts, slot; bool none; };
+__device__ __forceinline__ WindowPart window_part(const WindowParams& p, const WindowCutting c, int id) {
+    WindowPart x;
+    x.parts = p.parts;
+    x.slot = 0;
+    x.none = false;
+    const int pairs = p.N * p.qtiles, lane = threadIdx.x & 63;
+    if (!c.deal) {
+        x.job = window_job(p, id);
+        x.slot = (x.job.kvh * pairs + (p.qtiles - 1 - x.job.qt) * p.N + x.job.n) * p.parts + x.job.part;
+        return x;
+    }
+    const int slots = min(pairs * p.parts, c.want / p.kv_head), at = mix_uniform(id / p.kv_head);   // >= pairs (window_plan)
+    int steps[PAIRS / 64], sum = 0, most = 0;
+#pragma unroll
+    for (int k = 0; k < PAIRS / 64; k++) {
+        steps[k] = 0;
+        if (64 * k < pairs && 64 * k + lane < pairs) steps[k] = window_pair_steps(p, c, 64 * k + lane);
+        most = max(most, steps[k]);
+    }
+    // The least `longest` for which the parts fit the slots: with hi they do.  (A pair has at most one part more than its steps /
+    // longest, so all / (slots - pairs) is enough, and all / slots is needed; their sum may be beyond 32 bits.)
+    double all = 0.0;
+#pragma unroll
+    for (int k = 0; k < PAIRS / 64; k++)
+        if (64 * k < pairs) all += (double)wave_sum(steps[k] >> 12) * 4096.0 + (double)wave_sum(steps[k] & 4095);
+    auto parts_of = [](int steps, int longest) { return max((int)((unsigned)(steps + longest - 1) / (unsigned)longest), 1); };
+    int lo = max(c.least, (int)(all / slots)), hi = slots > pairs ? (int)(all / (slots - pairs)) + 1 : 0x3fffffff;
+    hi = max(hi, lo);
+    while (lo < hi) {
+        const int longest = (lo + hi) >> 1;
+        sum = 0;
+#pragma unroll
+        for (int k = 0; k < PAIRS / 64; k++)
+            if (64 * k < pairs) sum += 64 * k + lane < pairs ? parts_of(steps[k], longest) : 0;
+        if (wave_sum(sum) <= slots) hi = longest;
+        else lo = longest + 1;
+    }
+    x.none = true;
+    int base = 0;
+#pragma unroll
+    for (int k = 0; k < PAIRS / 64; k++) {
+        if (64 * k < pairs && x.none) {
+            const int own = 64 * k + lane < pairs ? parts_of(steps[k], hi) : 0, end = base + wave_scan(own);
+            const unsigned long long behind = __ballot(end > at);
+            if (behind != 0) {
+                const int l = __builtin_ctzll(behind), pair = 64 * k + l, q = mix_uniform(pair / p.N);
+                x.parts = __builtin_amdgcn_readlane(own, l);
+                const int first = __builtin_amdgcn_readlane(end, l) - x.parts;
+                x.job.part = at - first;
+                x.job.qt = p.qtiles - 1 - q;
+                x.job.n = pair - q * p.N;
+                x.job.kvh = id - at * p.kv_head;
+                x.slot = x.job.kvh * pairs * p.parts + at;
+                x.none = false;
+                if (threadIdx.x == 0 && x.job.kvh == 0 && x.job.part == 0) window_part_deal(p, c, pair) = make_int2(first, x.parts);
+            }
+            base = __builtin_amdgcn_readlane(end, 63);
+        }
+    }
+    return x;
+}
+
 // ---------------------------------------------------------------- many queries
-template <int DB, int DC, int KB>
+template <int DB, int DC, int KB, bool DEAL>
 __global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p) {
     constexpr int AK = KB * 32, DW = DB * 32, NG = DC * 4;
+    constexpr WindowCutting cutting = tile_cutting(AK, DEAL);
     __shared__ __attribute__((aligned(1024))) float Ks[2][AK * DW];
     __shared__ __attribute__((aligned(1024))) float Vs[2][AK * DW];
 
     const int t = threadIdx.x, lane = t & 63, wave = mix_uniform(t >> 6), r = lane & 31, h = lane >> 5;
-    const WindowJob job = window_job(p, blockIdx.x);
+    const WindowPart part = window_part(p, cutting, blockIdx.x);
+    if (part.none) return;
+    const WindowJob job = part.job;
     const WindowLens len = window_lens(p, job.n);
     const int group = p.head / p.kv_head, off = len.vl - len.ql;
-    // where a tile has fewer than 128 rows, the parts of its keys leave other wavefronts (and SIMDs) without work
-    const int row0 = job.qt * AQ, wrow = row0 + 32 * ((wave + job.part) & 3);
+    const int row0 = job.qt * AQ, wrow = row0 + 32 * wave;
     const WindowRow row = window_row(p, job, wrow + r, group, len.ql);
     const size_t stat = ((size_t)job.n * p.head + row.hd) * p.QL + row.i;
 
@@ -50,8 +161,8 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p
     const WindowSpan all = window_span(row0, AQ, group, len.ql, off), span = window_span(wrow, 32, group, len.ql, off);
     const WindowRange range = window_range(p, all.first, all.last, all.first <= all.last, len.vl);
     const int nsink = (range.sink_end + AK - 1) / AK, nwin = (max(range.hi - range.low, 0) + AK - 1) / AK;
-    const int first = mix_uniform((int)((long long)(nsink + nwin) * job.part / p.parts));
-    const int last = mix_uniform((int)((long long)(nsink + nwin) * (job.part + 1) / p.parts));
+    const int first = mix_uniform((int)((long long)(nsink + nwin) * job.part / part.parts));
+    const int last = mix_uniform((int)((long long)(nsink + nwin) * (job.part + 1) / part.parts));
     const int pos = row.live ? row.i + off : -1;
     const int w0 = span.first, w1 = span.last;              // the wavefront's positions
 
@@ -168,8 +279,8 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p
         mix_store_row<DC>(p.Y + job.n * p.y.n + row.hd * p.y.h + (size_t)row.i * p.y.l, o, l == 0.0f ? 0.0f : 1.0f / l, p.dv4, h);
         if (p.Lse != nullptr && h == 0) p.Lse[stat] = window_lse(m, l);
     } else {
-        mix_store_row<DC>(p.part_o(stat, job.part), o, 1.0f, p.dv4, h);
-        if (h == 0) p.part_ml(stat, job.part) = make_float2(m, l);
+        mix_store_row<DC>(window_part_o(p, cutting, part.slot, wrow + r - row0), o, 1.0f, p.dv4, h);
+        if (h == 0) window_part_ml(p, cutting, part.slot, wrow + r - row0) = make_float2(m, l);
     }
 }
 
@@ -182,11 +293,14 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_tiles(const WindowParams p
 template <int DE, bool NT>   // head dimension in 64s; keys and values read non-temporally
 __global__ __launch_bounds__(NTHREADS, 2) void window_rows(const WindowParams p) {
     constexpr int NS = DE * 4;
+    constexpr WindowCutting cutting = ROWS_CUTTING;
     __shared__ __attribute__((aligned(16))) float So[4][16][DE * 64 + 4];
     __shared__ float Sm[4][16], Sl[4][16];
 
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, k4 = lane >> 4;
-    const WindowJob job = window_job(p, blockIdx.x);
+    const WindowPart part = window_part(p, cutting, blockIdx.x);
+    if (part.none) return;
+    const WindowJob job = part.job;
     const WindowLens len = window_lens(p, job.n);
     const int group = p.head / p.kv_head, rows = p.QL * group, off = len.vl - len.ql;
     const int row0 = job.qt * 16;
@@ -197,8 +311,8 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_rows(const WindowParams p)
     const WindowSpan all = window_span(row0, 16, group, len.ql, off);
     const WindowRange range = window_range(p, all.first, all.last, all.first <= all.last, len.vl);
     const int nsink = (range.sink_end + 15) / 16, nwin = (max(range.hi - range.low, 0) + 15) / 16;
-    const int first = mix_uniform((int)((long long)(nsink + nwin) * job.part / p.parts));
-    const int last = mix_uniform((int)((long long)(nsink + nwin) * (job.part + 1) / p.parts));
+    const int first = mix_uniform((int)((long long)(nsink + nwin) * job.part / part.parts));
+    const int last = mix_uniform((int)((long long)(nsink + nwin) * (job.part + 1) / part.parts));
 
     const float* qrow = p.Q + job.n * p.q.n + row.hd * p.q.h + (size_t)row.i * p.q.l;
     v4f qf[NS];
@@ -318,8 +432,8 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_rows(const WindowParams p)
             *(v4f*)(p.Y + job.n * p.y.n + qh * p.y.h + (size_t)qi * p.y.l + d) = L == 0.0f ? (v4f)(0.0f) : y * (1.0f / L);
             if (p.Lse != nullptr && d == 0) p.Lse[stat] = window_lse(M, L);
         } else {
-            *(v4f*)(p.part_o(stat, job.part) + d) = y;
-            if (d == 0) p.part_ml(stat, job.part) = make_float2(M, L);
+            *(v4f*)(window_part_o(p, cutting, part.slot, rr) + d) = y;
+            if (d == 0) window_part_ml(p, cutting, part.slot, rr) = make_float2(M, L);
         }
     }
 }
@@ -328,23 +442,29 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_rows(const WindowParams p)
 // `wide` threads (16 or 32) for a row's columns, `across` of such groups (a power of two up to 8) next to each other for its
 // parts: a thread adds every across-th part, LDS joins the rest.  With few rows and many parts one thread for all of them
 // would read one after the other: 64 parts of 32 rows in 22.3 us, so in 4.7.
-__global__ __launch_bounds__(NTHREADS) void window_join(const WindowParams p, int wide, int across) {
+__global__ __launch_bounds__(NTHREADS) void window_join(const WindowParams p, const WindowCutting c, int wide, int across) {
     __shared__ __attribute__((aligned(16))) v4f Sy[NTHREADS];
     __shared__ float2 Sml[NTHREADS / 16];
     const int t = threadIdx.x, slot = t / wide, sub = slot & (across - 1), d = 4 * (t & (wide - 1));
     const long long stat = (long long)blockIdx.x * (NTHREADS / wide / across) + slot / across;
     const bool mine = stat < (long long)p.N * p.head * p.QL && d < p.dv4;
+    const long long nh = stat / p.QL;
+    const int n = (int)(nh / p.head), hd = (int)(nh - (long long)n * p.head), i = (int)(stat - nh * p.QL);
     float M = NEG, L = 0.0f;
     v4f y = (v4f)(0.0f);
     if (mine) {
+        const int group = p.head / p.kv_head, kvh = hd / group, row = i * group + hd - kvh * group, tile = row / c.per;
+        const int pair = (p.qtiles - 1 - tile) * p.N + n, in = row - tile * c.per;
+        const int2 deal = c.deal ? window_part_deal(p, c, pair) : make_int2(pair * p.parts, p.parts);
+        const int parts = deal.y, slot = kvh * p.N * p.qtiles * p.parts + deal.x;
 #pragma unroll 4
-        for (int s = sub; s < p.parts; s += across) M = fmaxf(M, p.part_ml(stat, s).x);
+        for (int s = sub; s < parts; s += across) M = fmaxf(M, window_part_ml(p, c, slot + s, in).x);
 #pragma unroll 4
-        for (int s = sub; s < p.parts; s += across) {
-            const float2 ml = p.part_ml(stat, s);
+        for (int s = sub; s < parts; s += across) {
+            const float2 ml = window_part_ml(p, c, slot + s, in);
             const float f = ml.x == NEG ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
             L += ml.y * f;
-            y += *(const v4f*)(p.part_o(stat, s) + d) * f;
+            y += *(const v4f*)(window_part_o(p, c, slot + s, in) + d) * f;
         }
     }
     if (across > 1) {
@@ -363,8 +483,6 @@ __global__ __launch_bounds__(NTHREADS) void window_join(const WindowParams p, in
         }
     }
     if (!mine) return;
-    const long long nh = stat / p.QL;
-    const int n = (int)(nh / p.head), hd = (int)(nh - (long long)n * p.head), i = (int)(stat - nh * p.QL);
     *(v4f*)(p.Y + n * p.y.n + hd * p.y.h + (size_t)i * p.y.l + d) = L == 0.0f ? (v4f)(0.0f) : y * (1.0f / L);
     if (p.Lse != nullptr && d == 0) p.Lse[stat] = window_lse(M, L);
 }
@@ -375,7 +493,7 @@ constexpr long long JOIN_ROWS = 1024;    // rows from which a thread of window_j
 // of 1024: 51 us (window_tiles 79), on 8 x 4096 all: 97 (136); but 72 rows on 2 x 4096: 52 (49), 96 rows: 64 (51).
 constexpr int ROWS_MAX = 64;
 
-struct WindowPlan { bool rows; int qtiles, parts; };
+struct WindowPlan { bool rows; int qtiles, parts, per; };
 
 // One decision for the launch and for the size of the caller's buffer: from the sizes alone.  The keys are cut where there are
 // fewer workgroups than wanted; for tiles of 128 rows under a window, which differ little, fewer than half of them.  (Tiles that
@@ -387,20 +505,21 @@ WindowPlan window_plan(int N, int head, int kv_head, int QL, int VL, int window,
     WindowPlan x;
     const long long group = head / kv_head, rows = QL * group;
     x.rows = rows <= ROWS_MAX;
-    const long long per = x.rows ? 16 : AQ;
+    const long long per = x.per = x.rows ? 16 : AQ;
     x.qtiles = (int)((rows + per - 1) / per);
     const long long base = (long long)N * kv_head * x.qtiles;
     const long long reach = window == 0 ? VL : (long long)window + sinks + (per + group - 1) / group;
     const long long steps = ((reach < VL ? reach : VL) + (x.rows ? 15 : 31)) / (x.rows ? 16 : 32);
-    const long long want = x.rows ? 256 : 512, least = x.rows ? (steps < 24 ? 24 : 8) : 4;   // workgroups on the chip; steps worth a part
+    const WindowCutting c = x.rows ? ROWS_CUTTING : tile_cutting(32, false);
+    const long long want = c.want, least = x.rows && steps < 24 ? 24 : c.least;
     long long parts = base >= (!x.rows && reach < VL ? want / 2 : want) ? 1 : (want + base - 1) / base;
     if (parts > steps / least) parts = steps / least;
     x.parts = (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
     return x;
 }
 
-long long window_buffer(const WindowPlan& x, int N, int head, int QL, int dv4) {
-    return x.parts == 1 ? 0 : (long long)N * head * QL * x.parts * (dv4 + 2) * 4;
+long long window_buffer(const WindowPlan& x, int N, int kv_head, int dv4) {
+    return x.parts == 1 ? 0 : (long long)N * kv_head * x.qtiles * x.parts * x.per * (dv4 + 2) * 4 + (long long)N * x.qtiles * 8;
 }
 
 }  // namespace
@@ -425,7 +544,7 @@ extern "C" {
 int64_t dragon_Cuda_attention_window_bufsize(int32_t N, int32_t head, int32_t kv_head, int32_t QL, int32_t VL, int32_t dK4,
                                              int32_t dV4, int32_t window, int32_t sinks) {
     if (!window_arguments_ok(N, head, kv_head, QL, VL, dK4, dV4, window, sinks)) return -1;
-    return window_buffer(window_plan(N, head, kv_head, QL, VL, window, sinks), N, head, QL, dV4);
+    return window_buffer(window_plan(N, head, kv_head, QL, VL, window, sinks), N, kv_head, dV4);
 }
 
 int dragon_Cuda_attention_window_forward(const int64_t* streams, int32_t length, int64_t dQ, int64_t dK, int64_t dV, int64_t dY,
@@ -439,7 +558,7 @@ int dragon_Cuda_attention_window_forward(const int64_t* streams, int32_t length,
     if (!window_arguments_ok(N, head, kv_head, QL, VL, dK4, dV4, window, sinks) || !(scale - scale == 0.0f))
         return hipErrorInvalidValue;
     const WindowPlan plan = window_plan(N, head, kv_head, QL, VL, window, sinks);
-    const long long need = window_buffer(plan, N, head, QL, dV4);
+    const long long need = window_buffer(plan, N, kv_head, dV4);
     if (need > 0 && (dBuf == 0 || !mix_aligned16(dBuf) || buf_size < need)) return hipErrorInvalidValue;
 
     WindowParams p;
@@ -462,6 +581,7 @@ int dragon_Cuda_attention_window_forward(const int64_t* streams, int32_t length,
     const int dmax = dK4 > dV4 ? dK4 : dV4;
     const dim3 block(NTHREADS);
     const dim3 grid((unsigned)((long long)N * kv_head * plan.qtiles * plan.parts));
+    const bool deal = !plan.rows && plan.parts > 1 && (p.QLens != nullptr || p.VLens != nullptr);
     if (plan.rows) {
         // keys and values that are read once and do not fit the Infinity Cache pass it by (stream_policy.h has the border):
         // 65536 keys of 8 heads of 128 in 84 us instead of 96, but 16 x 2048 in 66 instead of 50
@@ -475,18 +595,25 @@ int dragon_Cuda_attention_window_forward(const int64_t* streams, int32_t length,
             else hipLaunchKernelGGL((window_rows<2, false>), grid, block, 0, s, p);
         }
     } else {
+#define TILES(...)                                                                                        \
+    do {                                                                                                  \
+        if (deal) hipLaunchKernelGGL((window_tiles<__VA_ARGS__, true>), grid, block, 0, s, p);            \
+        else hipLaunchKernelGGL((window_tiles<__VA_ARGS__, false>), grid, block, 0, s, p);                \
+    } while (0)
         switch ((dmax + 31) / 32) {
-            case 1: hipLaunchKernelGGL((window_tiles<1, 1, 2>), grid, block, 0, s, p); break;
-            case 2: hipLaunchKernelGGL((window_tiles<2, 2, 1>), grid, block, 0, s, p); break;
-            case 3: hipLaunchKernelGGL((window_tiles<4, 3, 1>), grid, block, 0, s, p); break;
-            default: hipLaunchKernelGGL((window_tiles<4, 4, 1>), grid, block, 0, s, p); break;
+            case 1: TILES(1, 1, 2); break;
+            case 2: TILES(2, 2, 1); break;
+            case 3: TILES(4, 3, 1); break;
+            default: TILES(4, 4, 1); break;
         }
+#undef TILES
     }
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && plan.parts > 1) {
         const int across = (long long)N * head * QL >= JOIN_ROWS ? 1 : plan.parts >= 8 ? 8 : plan.parts >= 4 ? 4 : 2;
         const int wide = dV4 <= 64 ? 16 : 32, rows = NTHREADS / wide / across;
-        hipLaunchKernelGGL(window_join, dim3((unsigned)(((long long)N * head * QL + rows - 1) / rows)), block, 0, s, p, wide, across);
+        const WindowCutting cutting = plan.rows ? ROWS_CUTTING : tile_cutting(32, deal);     // (the keys of a step are not asked for)
+        hipLaunchKernelGGL(window_join, dim3((unsigned)(((long long)N * head * QL + rows - 1) / rows)), block, 0, s, p, cutting, wide, across);
         e = hipGetLastError();
     }
     return e;

@@ -47,6 +47,10 @@ WINDOW = [
     (1, 4, 2, 1, 400, 128, 128, 0, 0, None, None),                 # cut in three
     (1, 4, 4, 300, 2500, 96, 72, 0, 0, None, None),                # cut, and many rows to join
     (1, 2, 1, 150, 150, 32, 32, 1000, 5, None, None),              # a window beyond the sequence
+    (5, 2, 1, 100, 3000, 32, 32, 0, 0, [100, 1, 50, 0, 100], [3000, 1, 200, 0, 64]),     # parts dealt by length
+    (3, 1, 1, 200, 2000, 64, 64, 700, 20, [200, 150, 3], [2000, 900, 10]),               # and under a window
+    (80, 1, 1, 70, 300, 16, 16, 0, 0, [70 - i % 71 for i in range(80)], [300 - 3 * i for i in range(80)]),   # 80 pairs
+    (2, 4, 2, 700, 900, 128, 128, 0, 0, None, [900, 700]),         # lengths of keys alone; a triangle
     (12, 8, 8, 500, 500, 16, 16, 40, 2, None, None),               # many tiles: nothing is cut, in either direction
 ]
 
