@@ -367,11 +367,15 @@ __global__ __launch_bounds__(NTHREADS, 2) void window_rows(const WindowParams p)
 #pragma unroll
         for (int s2 = 0; s2 < 4 * DE; s2++) vc[s2] = vr[s2];
         if (s + 4 < last) fetch(s + 4);
-        v4f sc = (v4f)(0.0f);
+        v4f sc = (v4f)(0.0f), odd = (v4f)(0.0f);                // two sums: half the roundings in a row, half the wait
 #pragma unroll
         for (int s2 = 0; s2 < NS; s2++)
 #pragma unroll
-            for (int u = 0; u < 4; u++) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kc[s2][u], qf[s2][u], sc, 0, 0, 0);
+            for (int u = 0; u < 4; u += 2) {
+                sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kc[s2][u], qf[s2][u], sc, 0, 0, 0);
+                odd = __builtin_amdgcn_mfma_f32_16x16x4f32(kc[s2][u + 1], qf[s2][u + 1], odd, 0, 0, 0);
+            }
+        sc += odd;
 #pragma unroll
         for (int v = 0; v < 4; v++) {
             const int j = key0 + 4 * k4 + v;
