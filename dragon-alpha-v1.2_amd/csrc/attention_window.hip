@@ -89,12 +89,11 @@ __device__ __forceinline__ WindowPart window_part(const WindowParams& p, const W
         return x;
     }
     const int slots = min(pairs * p.parts, c.want / p.kv_head), at = mix_uniform(id / p.kv_head);   // >= pairs (window_plan)
-    int steps[PAIRS / 64], sum = 0, most = 0;
+    int steps[PAIRS / 64];
 #pragma unroll
     for (int k = 0; k < PAIRS / 64; k++) {
         steps[k] = 0;
         if (64 * k < pairs && 64 * k + lane < pairs) steps[k] = window_pair_steps(p, c, 64 * k + lane);
-        most = max(most, steps[k]);
     }
     // The least `longest` for which the parts fit the slots: with hi they do.  (A pair has at most one part more than its steps /
     // longest, so all / (slots - pairs) is enough, and all / slots is needed; their sum may be beyond 32 bits.)
@@ -107,7 +106,7 @@ __device__ __forceinline__ WindowPart window_part(const WindowParams& p, const W
     hi = max(hi, lo);
     while (lo < hi) {
         const int longest = (lo + hi) >> 1;
-        sum = 0;
+        int sum = 0;
 #pragma unroll
         for (int k = 0; k < PAIRS / 64; k++)
             if (64 * k < pairs) sum += 64 * k + lane < pairs ? parts_of(steps[k], longest) : 0;
