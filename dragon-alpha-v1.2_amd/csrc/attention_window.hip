@@ -21,6 +21,7 @@
 #include "runtime_internal.h"
 #include "stream_policy.h"
 #include "../../include/dragon_hip_gemm.h"
+#include "../../include/dragon_hip_testing.h"
 
 namespace dragon {
 namespace {
@@ -51,6 +52,18 @@ __device__ __forceinline__ int window_pair_steps(const WindowParams& p, const Wi
     const int end = min(row0 + c.per, ql * group), off = vl - ql;
     const WindowRange range = window_range(p, row0 / group + off, (end - 1) / group + off, end > row0, vl);
     return (range.sink_end + c.ak - 1) / c.ak + (max(range.hi - range.low, 0) + c.ak - 1) / c.ak;
+}
+// Between which numbers of steps the longest part is looked for, so that the pairs' parts fit the slots: with hi they do.  (A pair
+// has at most one part more than its steps / longest, so all / (slots - pairs) is enough, and all / slots is needed; beside
+// few spare slots the former leaves 32 bits where the keys are more than 10^8, so it ends at more steps than a tile can have.)
+struct WindowDealBounds { int lo, hi; };
+__host__ __device__ inline WindowDealBounds window_deal_bounds(double all, int slots, int pairs, int least) {
+    constexpr int MOST = 0x3fffffff;
+    WindowDealBounds x;
+    x.lo = max(least, (int)(all / slots));
+    x.hi = slots > pairs ? (int)min(all / (slots - pairs), (double)(MOST - 1)) + 1 : MOST;
+    x.hi = max(x.hi, x.lo);
+    return x;
 }
 // sum over this lane and those below it
 __device__ __forceinline__ int wave_scan(int x) {
@@ -95,15 +108,14 @@ __device__ __forceinline__ WindowPart window_part(const WindowParams& p, const W
         steps[k] = 0;
         if (64 * k < pairs && 64 * k + lane < pairs) steps[k] = window_pair_steps(p, c, 64 * k + lane);
     }
-    // The least `longest` for which the parts fit the slots: with hi they do.  (A pair has at most one part more than its steps /
-    // longest, so all / (slots - pairs) is enough, and all / slots is needed; their sum may be beyond 32 bits.)
+    // the least `longest` for which the parts fit the slots (the steps' sum may be beyond 32 bits)
     double all = 0.0;
 #pragma unroll
     for (int k = 0; k < PAIRS / 64; k++)
         if (64 * k < pairs) all += (double)wave_sum(steps[k] >> 12) * 4096.0 + (double)wave_sum(steps[k] & 4095);
     auto parts_of = [](int steps, int longest) { return max((int)((unsigned)(steps + longest - 1) / (unsigned)longest), 1); };
-    int lo = max(c.least, (int)(all / slots)), hi = slots > pairs ? (int)(all / (slots - pairs)) + 1 : 0x3fffffff;
-    hi = max(hi, lo);
+    const WindowDealBounds bounds = window_deal_bounds(all, slots, pairs, c.least);
+    int lo = bounds.lo, hi = bounds.hi;
     while (lo < hi) {
         const int longest = (lo + hi) >> 1;
         int sum = 0;
@@ -543,6 +555,12 @@ bool window_arguments_ok(int N, int head, int kv_head, int QL, int VL, int dk4, 
 using namespace dragon;
 
 extern "C" {
+
+void dragon_window_deal_bounds(double all, int32_t slots, int32_t pairs, int32_t least, int32_t* lo, int32_t* hi) {
+    const WindowDealBounds x = window_deal_bounds(all, slots, pairs, least);
+    *lo = x.lo;
+    *hi = x.hi;
+}
 
 int64_t dragon_Cuda_attention_window_bufsize(int32_t N, int32_t head, int32_t kv_head, int32_t QL, int32_t VL, int32_t dK4,
                                              int32_t dV4, int32_t window, int32_t sinks) {

@@ -103,6 +103,7 @@ SIGNATURES = {
     "dragon_gemm_release_workspaces": (i32, []),
     "dragon_gemm_choose_tile": (i32, [i32, i32, i32, i32, i32, i32]),
     "dragon_gemm_paired_form_fits": (i32, [i32, i32, i32, i32, i32]),
+    "dragon_window_deal_bounds": (None, [ctypes.c_double, i32, i32, i32, p_i32, p_i32]),
     "dragon_gemm_tile_divisor": (None, [ctypes.c_uint32, POINTER(ctypes.c_uint32), POINTER(ctypes.c_uint32)]),
     # include/dragon_hip_runtime.h
     "dragon_Cuda_malloc": (i64, [i64]),

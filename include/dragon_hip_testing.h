@@ -85,6 +85,9 @@ double dragon_gemm_estimate_us(int32_t variant, int32_t rows, int32_t cols, int3
  * tile-per-workgroup kernel instead. */
 int32_t dragon_gemm_workspace_count(void);
 int64_t dragon_gemm_workspaces_refused(void);
+/* Where windowed attention deals the keys by the sequences' lengths: the numbers of steps between which it looks for the
+ * longest part, for `all` steps of `pairs` (tile, sequence) pairs on `slots` parts of at least `least` steps.  Host arithmetic. */
+void dragon_window_deal_bounds(double all, int32_t slots, int32_t pairs, int32_t least, int32_t* lo, int32_t* hi);
 /* Free and total device memory of the current device in bytes (hipMemGetInfo). */
 int dragon_test_mem_get_info(int64_t* free_bytes, int64_t* total_bytes);
 /* Device-to-device copy of `length` floats (a multiple of 4, 16-byte aligned) done by an ordinary
