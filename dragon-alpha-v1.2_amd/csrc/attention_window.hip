@@ -59,10 +59,10 @@ __device__ __forceinline__ int window_pair_steps(const WindowParams& p, const Wi
 struct WindowDealBounds { int lo, hi; };
 __host__ __device__ inline WindowDealBounds window_deal_bounds(double all, int slots, int pairs, int least) {
     constexpr int MOST = 0x3fffffff;
+    const double enough = slots > pairs ? all / (slots - pairs) + 1.0 : (double)MOST;
     WindowDealBounds x;
     x.lo = max(least, (int)(all / slots));
-    x.hi = slots > pairs ? (int)min(all / (slots - pairs), (double)(MOST - 1)) + 1 : MOST;
-    x.hi = max(x.hi, x.lo);
+    x.hi = max(enough < MOST ? (int)enough : MOST, x.lo);
     return x;
 }
 // sum over this lane and those below it
