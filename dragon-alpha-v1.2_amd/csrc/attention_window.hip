@@ -533,6 +533,23 @@ WindowPlan window_plan(int N, int head, int kv_head, int QL, int VL, int window,
     return x;
 }
 
+long long window_workgroups(const WindowPlan& x, int N, int kv_head) { return (long long)N * kv_head * x.qtiles * x.parts; }
+// the join's: rows a workgroup, threads side by side for a row's parts
+struct WindowJoin { int wide, across; long long workgroups; };
+WindowJoin window_join_plan(const WindowPlan& x, int N, int head, int QL, int dv4) {
+    const long long rows = (long long)N * head * QL;
+    WindowJoin j;
+    j.wide = dv4 <= 64 ? 16 : 32;
+    j.across = rows >= JOIN_ROWS ? 1 : x.parts >= 8 ? 8 : x.parts >= 4 ? 4 : 2;
+    const int per = NTHREADS / j.wide / j.across;
+    j.workgroups = x.parts == 1 ? 0 : (rows + per - 1) / per;
+    return j;
+}
+bool window_launches_fit(const WindowPlan& x, int N, int head, int kv_head, int QL, int dv4) {
+    return mix_launch_fits(window_workgroups(x, N, kv_head), NTHREADS) &&
+           mix_launch_fits(window_join_plan(x, N, head, QL, dv4).workgroups, NTHREADS);
+}
+
 long long window_buffer(const WindowPlan& x, int N, int kv_head, int dv4) {
     return x.parts == 1 ? 0 : (long long)N * kv_head * x.qtiles * x.parts * x.per * (dv4 + 2) * 4 + (long long)N * x.qtiles * 8;
 }
@@ -543,7 +560,8 @@ bool window_arguments_ok(int N, int head, int kv_head, int QL, int VL, int dk4, 
     if (N <= 0 || head <= 0 || kv_head <= 0 || head % kv_head != 0 || QL <= 0 || VL <= 0 || dk4 <= 0 || dv4 <= 0 || (dk4 & 3) ||
         (dv4 & 3) || dk4 > 128 || dv4 > 128 || window < 0 || sinks < 0)
         return false;
-    // positions and rows are 32-bit, a tile's offsets 32-bit bytes, a launch's workgroups 31 bits
+    // positions and rows are 32-bit, a tile's offsets 32-bit bytes, key tiles over all sequences and rows over 16 31 bits.  (What a
+    // launch takes is asked of the forward pass's and the gradient's own plans.)
     const long long row = (long long)head * (dk4 > dv4 ? dk4 : dv4);
     return (long long)QL + VL < 0x3fffff00LL && row * AQ * 4 < 0x7ffffff0LL && (long long)QL * (head / kv_head) < 0x7fffff00LL &&
            (long long)N * kv_head * ((VL + 127LL) / 128) < 0x7fffffffLL &&
@@ -565,7 +583,8 @@ void dragon_window_deal_bounds(double all, int32_t slots, int32_t pairs, int32_t
 int64_t dragon_Cuda_attention_window_bufsize(int32_t N, int32_t head, int32_t kv_head, int32_t QL, int32_t VL, int32_t dK4,
                                              int32_t dV4, int32_t window, int32_t sinks) {
     if (!window_arguments_ok(N, head, kv_head, QL, VL, dK4, dV4, window, sinks)) return -1;
-    return window_buffer(window_plan(N, head, kv_head, QL, VL, window, sinks), N, kv_head, dV4);
+    const WindowPlan plan = window_plan(N, head, kv_head, QL, VL, window, sinks);
+    return window_launches_fit(plan, N, head, kv_head, QL, dV4) ? window_buffer(plan, N, kv_head, dV4) : -1;
 }
 
 int dragon_Cuda_attention_window_forward(const int64_t* streams, int32_t length, int64_t dQ, int64_t dK, int64_t dV, int64_t dY,
@@ -579,6 +598,7 @@ int dragon_Cuda_attention_window_forward(const int64_t* streams, int32_t length,
     if (!window_arguments_ok(N, head, kv_head, QL, VL, dK4, dV4, window, sinks) || !(scale - scale == 0.0f))
         return hipErrorInvalidValue;
     const WindowPlan plan = window_plan(N, head, kv_head, QL, VL, window, sinks);
+    if (!window_launches_fit(plan, N, head, kv_head, QL, dV4)) return hipErrorInvalidValue;
     const long long need = window_buffer(plan, N, kv_head, dV4);
     if (need > 0 && (dBuf == 0 || !mix_aligned16(dBuf) || buf_size < need)) return hipErrorInvalidValue;
 
@@ -601,7 +621,7 @@ int dragon_Cuda_attention_window_forward(const int64_t* streams, int32_t length,
     hipStream_t s = (hipStream_t)(intptr_t)streams[0];
     const int dmax = dK4 > dV4 ? dK4 : dV4;
     const dim3 block(NTHREADS);
-    const dim3 grid((unsigned)((long long)N * kv_head * plan.qtiles * plan.parts));
+    const dim3 grid((unsigned)window_workgroups(plan, N, kv_head));
     const bool deal = !plan.rows && plan.parts > 1 && (p.QLens != nullptr || p.VLens != nullptr);
     if (plan.rows) {
         // keys and values that are read once and do not fit the Infinity Cache pass it by (stream_policy.h has the border):
@@ -631,10 +651,9 @@ int dragon_Cuda_attention_window_forward(const int64_t* streams, int32_t length,
     }
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && plan.parts > 1) {
-        const int across = (long long)N * head * QL >= JOIN_ROWS ? 1 : plan.parts >= 8 ? 8 : plan.parts >= 4 ? 4 : 2;
-        const int wide = dV4 <= 64 ? 16 : 32, rows = NTHREADS / wide / across;
+        const WindowJoin join = window_join_plan(plan, N, head, QL, dV4);
         const WindowCutting cutting = plan.rows ? ROWS_CUTTING : tile_cutting(32, deal);     // (the keys of a step are not asked for)
-        hipLaunchKernelGGL(window_join, dim3((unsigned)(((long long)N * head * QL + rows - 1) / rows)), block, 0, s, p, cutting, wide, across);
+        hipLaunchKernelGGL(window_join, dim3((unsigned)join.workgroups), block, 0, s, p, cutting, join.wide, join.across);
         e = hipGetLastError();
     }
     return e;

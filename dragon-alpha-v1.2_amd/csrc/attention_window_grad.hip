@@ -655,7 +655,13 @@ int window_grad_parts(int N, int head, int kv_head, int QL, int VL, int workers,
 // The caller's buffer, in floats: the statistics, the running sum (64-bit), the pieces and whose they are, the sinks' parts,
 // the parts of dQ.
 constexpr int SINKS_APART = 64;      // up to here window_grad_sinks takes the queries beyond the window
-struct WindowGradBuffer { int ktiles, workers, sink_blocks, sink_parts, parts; long long stats, before, pieces, cut, sinks, all; };
+// also the workgroups of every launch: rows' statistics, dQ, sinks, joins (window_grad_kv: the workers)
+struct WindowGradBuffer {
+    int ktiles, workers, qtiles, sink_blocks, sink_parts, parts;
+    long long stats, before, pieces, cut, sinks, all;
+    long long run_delta, run_q, run_sinks, run_join;
+    bool fits;
+};
 WindowGradBuffer window_grad_buffer(int N, int head, int kv_head, int QL, int VL, int dk4, int dv4, int window, int sinks) {
     WindowGradBuffer b;
     b.ktiles = (VL + GK - 1) / GK;
@@ -672,7 +678,15 @@ WindowGradBuffer window_grad_buffer(int N, int head, int kv_head, int QL, int VL
     b.cut = ((long long)N * b.ktiles * kv_head * 2 + 3) / 4 * 4;
     b.sinks = (long long)N * kv_head * b.sink_blocks * b.sink_parts * 16 * (dk4 + dv4);
     b.parts = window_grad_parts(N, head, kv_head, QL, VL, (int)hold, window, sinks);
-    b.all = b.stats + b.before + b.pieces + b.cut + b.sinks + (b.parts > 1 ? (long long)N * head * QL * b.parts * dk4 : 0);
+    const long long rows = (long long)N * head * QL;
+    b.all = b.stats + b.before + b.pieces + b.cut + b.sinks + (b.parts > 1 ? rows * b.parts * dk4 : 0);
+    b.qtiles = (int)(((long long)QL * (head / kv_head) + GQ - 1) / GQ);
+    b.run_delta = (rows + NTHREADS / 32 - 1) / (NTHREADS / 32) + 1;
+    b.run_q = (long long)N * kv_head * b.qtiles * b.parts;
+    b.run_sinks = (long long)N * kv_head * b.sink_blocks * b.sink_parts;
+    b.run_join = tiles + (b.parts == 1 ? 0 : (rows * (dk4 / 4) + 4 * NTHREADS - 1) / (4 * NTHREADS));
+    b.fits = mix_launch_fits(b.run_delta, NTHREADS) && mix_launch_fits(b.run_q, GT) && mix_launch_fits(b.run_sinks, NTHREADS) &&
+             mix_launch_fits(b.run_join, NTHREADS);
     return b;
 }
 
@@ -686,7 +700,8 @@ extern "C" {
 int64_t dragon_Cuda_attention_window_backward_bufsize(int32_t N, int32_t head, int32_t kv_head, int32_t QL, int32_t VL, int32_t dK4,
                                                       int32_t dV4, int32_t window, int32_t sinks) {
     if (!window_arguments_ok(N, head, kv_head, QL, VL, dK4, dV4, window, sinks)) return -1;
-    return window_grad_buffer(N, head, kv_head, QL, VL, dK4, dV4, window, sinks).all * 4;
+    const WindowGradBuffer b = window_grad_buffer(N, head, kv_head, QL, VL, dK4, dV4, window, sinks);
+    return b.fits ? b.all * 4 : -1;
 }
 
 int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length, int64_t dQ, int64_t dK, int64_t dV, int64_t dY,
@@ -703,6 +718,7 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
         return hipErrorInvalidValue;
     const WindowGradBuffer b = window_grad_buffer(N, head, kv_head, QL, VL, dK4, dV4, window, sinks);
     const long long need = b.all * 4;
+    if (!b.fits) return hipErrorInvalidValue;
     if (dBuf == 0 || !mix_aligned16(dBuf) || buf_size < need) return hipErrorInvalidValue;
 
     WindowGrad a;
@@ -716,7 +732,7 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
     p.window = window == 0 || window > QL + VL ? QL + VL : window;
     p.sinks = sinks;
     p.c = scale * MIX_LOG2E;
-    p.qtiles = (int)(((long long)QL * (head / kv_head) + GQ - 1) / GQ); p.parts = b.parts;
+    p.qtiles = b.qtiles; p.parts = b.parts;
     a.dY = (const float*)(intptr_t)dDeltaY;
     a.dQ = (float*)(intptr_t)dDeltaQ; a.dK = (float*)(intptr_t)dDeltaK; a.dV = (float*)(intptr_t)dDeltaV;
     a.stats = (float*)(intptr_t)dBuf;
@@ -737,10 +753,10 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
 
     hipStream_t s = (hipStream_t)(intptr_t)streams[0];
     const dim3 block(NTHREADS);
-    hipLaunchKernelGGL(window_delta, dim3((unsigned)((a.rows + NTHREADS / 32 - 1) / (NTHREADS / 32) + 1)), block, 0, s, a);
+    hipLaunchKernelGGL(window_delta, dim3((unsigned)b.run_delta), block, 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const dim3 gq((unsigned)((long long)N * kv_head * p.qtiles * p.parts)), gk((unsigned)b.workers);
+    const dim3 gq((unsigned)b.run_q), gk((unsigned)b.workers);
     const int dmax = dK4 > dV4 ? dK4 : dV4;
 #define GRAD_CASE(DB_, DC_, B_)                                                        \
     do {                                                                              \
@@ -759,14 +775,13 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
     }
 #undef GRAD_CASE
     if (b.sink_blocks > 0) {
-        const dim3 gs((unsigned)((long long)N * kv_head * b.sink_blocks * b.sink_parts));
+        const dim3 gs((unsigned)b.run_sinks);
         if (dmax <= 64) hipLaunchKernelGGL(window_grad_sinks<1>, gs, block, 0, s, a);
         else hipLaunchKernelGGL(window_grad_sinks<2>, gs, block, 0, s, a);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    const long long join_q = p.parts == 1 ? 0 : (a.rows * (dK4 / 4) + 4 * NTHREADS - 1) / (4 * NTHREADS);
-    hipLaunchKernelGGL(window_grad_join, dim3((unsigned)((long long)N * b.ktiles * kv_head + join_q), 4), block, 0, s, a);
+    hipLaunchKernelGGL(window_grad_join, dim3((unsigned)b.run_join, 4), block, 0, s, a);
     e = hipGetLastError();
     return e;
 }

@@ -491,9 +491,21 @@ long long decay_state_bytes(int N, int head, const DecayCut& cut, int dK4, int d
 bool decay_arguments_ok(int N, int head, int L, int dK4, int dV4) {
     if (N <= 0 || head <= 0 || L <= 0 || dK4 <= 0 || dV4 <= 0 || (dK4 & 3) || (dV4 & 3) || dK4 > 128 || dV4 > 128) return false;
     const long long row = (long long)head * (dK4 > dV4 ? dK4 : dV4);
-    // a tile's offsets are 32-bit bytes, positions 32-bit, a launch's workgroups 31 bits
+    // a tile's offsets are 32-bit bytes, positions 32-bit, image-head pairs 25 bits
     return L < 0x3fffff00 && row * 32 * 4 < 0x7ffffff0LL && (long long)N * head * 64 < 0x7fffffffLL &&
            (long long)N * head * dK4 * dV4 / 4 < 0x7fffffffLL * 128;
+}
+// a walk has a wavefront for 32 columns of z, of a workgroup for each pair and segment (which are many only where the pairs are
+// few); decay_steps a workgroup of four for 64 columns of V where it has to
+bool decay_walk_fits(int N, int head, int zd) { return mix_launch_fits((long long)N * head, 64 * ((zd + 31) / 32)); }
+bool decay_steps_fit(int N, int head, int dV4, int cols) {
+    return mix_launch_fits((long long)N * head * ((dV4 + cols - 1) / cols), NTHREADS);
+}
+bool decay_forward_ok(int N, int head, int L, int dK4, int dV4) {
+    return decay_arguments_ok(N, head, L, dK4, dV4) && (L <= STEPS_MAX ? decay_steps_fit(N, head, dV4, 64) : decay_walk_fits(N, head, dV4));
+}
+bool decay_backward_ok(int N, int head, int L, int dK4, int dV4) {
+    return decay_arguments_ok(N, head, L, dK4, dV4) && decay_walk_fits(N, head, dK4 > dV4 ? dK4 : dV4);
 }
 
 hipError_t launch_states(hipStream_t s, const float* A, MixLayout la, int ad, const float* B, MixLayout lb, int bd, const float* g,
@@ -541,11 +553,11 @@ using namespace dragon;
 extern "C" {
 
 int64_t dragon_Cuda_linear_attention_bufsize(int32_t N, int32_t head, int32_t L, int32_t dK4, int32_t dV4) {
-    if (!decay_arguments_ok(N, head, L, dK4, dV4)) return -1;
+    if (!decay_forward_ok(N, head, L, dK4, dV4)) return -1;
     return L <= STEPS_MAX ? 0 : decay_state_bytes(N, head, decay_cut(N, head, L, dV4), dK4, dV4);
 }
 int64_t dragon_Cuda_linear_attention_backward_bufsize(int32_t N, int32_t head, int32_t L, int32_t dK4, int32_t dV4) {
-    if (!decay_arguments_ok(N, head, L, dK4, dV4)) return -1;
+    if (!decay_backward_ok(N, head, L, dK4, dV4)) return -1;
     return 2 * decay_state_bytes(N, head, decay_cut(N, head, L, dK4 > dV4 ? dK4 : dV4), dK4, dV4);
 }
 
@@ -557,7 +569,7 @@ int dragon_Cuda_linear_attention_forward(const int64_t* streams, int32_t length,
     if (dQ == 0 || dK == 0 || dV == 0 || dDecay == 0 || dY == 0 || !mix_aligned16(dQ) || !mix_aligned16(dK) || !mix_aligned16(dV) ||
         !mix_aligned16(dY) || !mix_aligned16(dState) || !mix_aligned16(dStateOut) || (dDecay & 3) || (dLens & 3))
         return hipErrorInvalidValue;
-    if (!decay_arguments_ok(N, head, L, dK4, dV4) || !(scale - scale == 0.0f)) return hipErrorInvalidValue;
+    if (!decay_forward_ok(N, head, L, dK4, dV4) || !(scale - scale == 0.0f)) return hipErrorInvalidValue;
     const long long need = dragon_Cuda_linear_attention_bufsize(N, head, L, dK4, dV4);
     if (need > 0 && (dBuf == 0 || !mix_aligned16(dBuf) || buf_size < need)) return hipErrorInvalidValue;
     const float* Q = (const float*)(intptr_t)dQ; const float* K = (const float*)(intptr_t)dK; const float* V = (const float*)(intptr_t)dV;
@@ -571,7 +583,9 @@ int dragon_Cuda_linear_attention_forward(const int64_t* streams, int32_t length,
     if (need > 0) split_ledger_touch(U, (size_t)need);
     hipStream_t s = (hipStream_t)(intptr_t)streams[0];
     if (L <= STEPS_MAX) {
-        const bool nt = first != nullptr && last != nullptr && stream_nt(first, last, (long long)N * head * state * 4);
+        // (also where the states are so many that only workgroups of 64 columns fit a launch)
+        const bool nt = (first != nullptr && last != nullptr && stream_nt(first, last, (long long)N * head * state * 4)) ||
+                        !decay_steps_fit(N, head, dV4, 32);
         const int cols = nt ? 64 : 32;
         DecaySteps p = {Q, K, V, Y, lk, lk, lv, lv, g, lens, first, last, head, L, dK4, dV4, (dV4 + cols - 1) / cols, scale};
         const dim3 grid((unsigned)((long long)N * head * p.slabs));
@@ -603,7 +617,7 @@ int dragon_Cuda_linear_attention_backward(const int64_t* streams, int32_t length
         !mix_aligned16(dDeltaStateOut) || !mix_aligned16(dDeltaQ) || !mix_aligned16(dDeltaK) || !mix_aligned16(dDeltaV) ||
         !mix_aligned16(dDeltaState) || (dDecay & 3) || (dLens & 3))
         return hipErrorInvalidValue;
-    if (!decay_arguments_ok(N, head, L, dK4, dV4) || !(scale - scale == 0.0f)) return hipErrorInvalidValue;
+    if (!decay_backward_ok(N, head, L, dK4, dV4) || !(scale - scale == 0.0f)) return hipErrorInvalidValue;
     const DecayCut cut = decay_cut(N, head, L, dK4 > dV4 ? dK4 : dV4);
     const long long need = 2 * decay_state_bytes(N, head, cut, dK4, dV4);
     if (need > 0 && (dBuf == 0 || !mix_aligned16(dBuf) || buf_size < need)) return hipErrorInvalidValue;

@@ -163,6 +163,8 @@ __device__ __forceinline__ void mix_load_cols(v4f (&c)[NG], const float* row, bo
 }
 
 inline bool mix_aligned16(int64_t a) { return (a & 15) == 0; }
+// HIP takes fewer than 2^32 threads along a grid's dimension
+inline bool mix_launch_fits(long long workgroups, int threads) { return workgroups * threads < 0x100000000LL; }
 
 // element strides of a tensor [N, L, head, d4] (head_inner) or [N, head, L, d4]
 struct MixLayout {
