@@ -1701,6 +1701,13 @@ void mixer_length(Tensor* t, const char* name, long long length) {
         throw IllegalArgumentException(std::string(name) + ".length { got " + std::to_string(t->length) + " } must be " + std::to_string(length));
 }
 
+// an operand that the kernels read value after value: the rows of a tensor are padded to multiples of 4
+void mixer_dense(Tensor* t, const char* name, long long length) {
+    mixer_length(t, name, length);
+    if (t->ndim() > 1 && (t->lastDim() & 3) && t->length != t->lastDim())
+        throw IllegalArgumentException(std::string(name) + ".lastDim { got " + std::to_string(t->lastDim()) + " } must be a multiple of 4, or the tensor a row");
+}
+
 std::vector<int> with_last(std::vector<int> dim, int last) {
     dim.back() = last;
     return dim;
@@ -1740,7 +1747,7 @@ void Engine::attention_window_delta(Tensor* deltaY, Tensor* Y, Tensor* Q, Tensor
     mixer_equals(deltaY->lastDim(), "deltaY.lastDim", head * d.dv, "head * V.head_dim");
     mixer_length(Y, "Y", (long long)d.N * d.QL * head * d.dv);
     mixer_length(deltaY, "deltaY", Y->length);
-    mixer_length(Lse, "Lse", (long long)d.N * head * d.QL);
+    mixer_dense(Lse, "Lse", (long long)d.N * head * d.QL);
     if (scale == 0.0f) scale = 1.0f / sqrtf((float)d.dk);
     const int dk4 = pad4(d.dk), dv4 = pad4(d.dv);
     const int64_t need = dragon_Cuda_attention_window_backward_bufsize(d.N, head, kv_head, d.QL, d.VL, dk4, dv4, window, sinks);
@@ -1760,7 +1767,7 @@ static MixerDims decay_dims(Tensor* Q, Tensor* K, Tensor* V, Tensor* Decay, Tens
     const MixerDims d = mixer_dims(Q, K, V, head, head);
     mixer_equals(d.QL, "Q.seq_len", d.VL, "K.seq_len");
     if ((d.dk & 3) || (d.dv & 3)) throw IllegalArgumentException("head dimensions must be multiples of 4");   // rows of the state
-    mixer_length(Decay, "Decay", head);
+    mixer_dense(Decay, "Decay", head);
     if (State) {
         mixer_equals(State->lastDim(), "State.lastDim", d.dv, "V.head_dim");
         mixer_length(State, "State", (long long)d.N * head * d.dk * d.dv);

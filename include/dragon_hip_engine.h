@@ -144,7 +144,8 @@ dragon_tensor* dragon_engine_attention_masked(dragon_engine* eg, dragon_tensor* 
  * error code like the other int entries; on an error no output is set.
  * Q[N, QL, head*dk], K[N, VL, kv_head*dk], V[N, VL, kv_head*dv] -> *Y[N, QL, head*dv]; scale = 0: 1/sqrt(dk); head
  * dimensions up to 128, multiples of 4 with several heads.  Lse (NULL: not wanted) gets a tensor of N*head*QL values that
- * the gradient takes; out: deltaQ, deltaK, deltaV. */
+ * the gradient takes (as a row, or in any shape whose last dimension is a multiple of 4: Decay below likewise); out: deltaQ,
+ * deltaK, deltaV. */
 int dragon_engine_attention_window(dragon_engine* eg, dragon_tensor* Q, dragon_tensor* K, dragon_tensor* V, int32_t head,
                                    int32_t kv_head, int32_t window, int32_t sinks, float scale, dragon_tensor** Y,
                                    dragon_tensor** Lse);
