@@ -263,7 +263,7 @@ class Engine:
         K[N, VL, kv_head*dk], V[N, VL, kv_head*dv]; lse=True: (Y, Lse), which the gradient takes."""
         hs = [x._h if x is not None else None for x in (Q, K, V)]
         y, l = (ctypes.c_void_p * 1)(), (ctypes.c_void_p * 1)()
-        rc = lib.dragon_engine_attention_window(self._h, *hs, head, kv_head or head, window, sinks, scale, y, l if lse else None)
+        rc = lib.dragon_engine_attention_window(self._h, *hs, head, head if kv_head is None else kv_head, window, sinks, scale, y, l if lse else None)
         if rc:
             _raise(rc)
         return (Tensor(self, y[0]), Tensor(self, l[0])) if lse else Tensor(self, y[0])
@@ -271,7 +271,7 @@ class Engine:
     def attention_window_delta(self, deltaY, Y, Q, K, V, Lse, head, kv_head=None, window=0, sinks=0, scale=0.0):
         """(deltaQ, deltaK, deltaV) of attention_window."""
         hs = [x._h if x is not None else None for x in (deltaY, Y, Q, K, V, Lse)]
-        return self._outputs(lambda out: lib.dragon_engine_attention_window_delta(self._h, *hs, head, kv_head or head, window,
+        return self._outputs(lambda out: lib.dragon_engine_attention_window_delta(self._h, *hs, head, head if kv_head is None else kv_head, window,
                                                                                   sinks, scale, out), 3)
 
     def linear_attention(self, Q, K, V, Decay, head, State=None, scale=0.0, state=False):

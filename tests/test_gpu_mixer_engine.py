@@ -48,3 +48,15 @@ def test_an_lse_whose_rows_are_padded_is_refused(eg, QL):
         grads = eg.attention_window_delta(t[3], y, *t[:3], again, H, window=4, scale=0.5)
         want = window_reference(Q, K, V, 0.5, 4, 0, [QL] * N, [QL] * N, dY)
         check({n: apart(x.c().value(), N, H, QL, d) for n, x in zip(("dQ", "dK", "dV"), grads)}, want)
+
+
+def test_no_key_value_heads_are_refused(eg):
+    from dragon_hip import engine
+    q, k = eg.zeros(1, 5, 16).c(), eg.zeros(1, 5, 16).c()
+    y, lse = eg.attention_window(q, k, k, 2, lse=True)
+    y.c(), lse.c()
+    for bad in (0, -1):
+        with pytest.raises(engine.IllegalArgumentException):
+            eg.attention_window(q, k, k, 2, bad)
+        with pytest.raises(engine.IllegalArgumentException):
+            eg.attention_window_delta(y, y, q, k, k, lse, 2, bad)
