@@ -20,7 +20,9 @@
 // so decay_walk takes its operands x, y, z by name, a direction, and the beginning state either way round.
 //
 // Every power e^{g n} is computed as such (n >= 0: it cannot overflow), never as a quotient of two powers.  States, sums and
-// powers are FP32; the exponent g n is rounded once, which is an error of |g n| 2^-24 in a factor e^{g n}.
+// powers are FP32.  An exponent is g times log2(e), rounded, times n, rounded: with the constant's own error up to 2.2 |g n| 2^-24
+// in a power, beside the last bit of exp2, and a power of decay_states is the product of two.  Those errors meet a token's share
+// once; the factors that meet the state again and again are another matter (decay_slow).
 #include "token_mixer.h"
 #include "runtime_internal.h"
 #include "stream_policy.h"
@@ -31,7 +33,7 @@ namespace {
 
 struct DecayWalk {
     const float* x; const float* y; const float* z; float* out;   // [L, xd], [L, xd], [L, zd], [L, zd] per (image, head)
-    MixLayout lx, ly, lz, lo;
+    MixLayout lx, lz;                                             // of x and y, of z and out
     const float* g; const int* lens;
     int head, L, xd, zd;
     int segment, segments;     // tokens of a segment, a multiple of 32
@@ -42,12 +44,39 @@ struct DecayWalk {
     int nh;                    // image-head pairs
 };
 
-__device__ __forceinline__ float decay_log2(const float* g, int hd) {
+__device__ __forceinline__ float decay_log2(float g) {
     // not below -1e30: 0 * g has to be 0 where the head forgets at once (g = -infinity); NaN stays NaN
-    const float g2 = g[hd] * MIX_LOG2E;
+    const float g2 = g * MIX_LOG2E;
     return g2 < -1.0e30f ? -1.0e30f : g2;
 }
 __device__ __forceinline__ float decay_pow(float g2, int n) { return __builtin_amdgcn_exp2f(g2 * (float)n); }
+// What n >= 1 tokens leave of a state.  The same factor meets it again and again, so an error of the factor adds up in one
+// direction: rounded to FP32, a factor near 1 is off by up to 2^-25 every time (a state of a head that remembers them was off
+// by 6e-5 after 1800 factors).  So a head that keeps at least half takes (1 - e^{gn}) S off instead, a difference with a small error of
+// its own, and only the rounding of S itself is left, which goes up as often as down: 7e-8 there.  (Below a half the difference
+// would cancel; such a head forgets its errors too.)
+__device__ __forceinline__ bool decay_slow(float g, int n) { return fabsf(g * (float)n) < MIX_LN2; }
+// e^{gn} - 1 of such a head: Taylor's series to x^10, what is left out is below 2^-26 of it
+__device__ __forceinline__ float decay_less(float g, int n) {
+    const float x = g * (float)n;
+    float s = 1.0f / 3628800.0f;
+    s = __builtin_fmaf(s, x, 1.0f / 362880.0f);
+    s = __builtin_fmaf(s, x, 1.0f / 40320.0f);
+    s = __builtin_fmaf(s, x, 1.0f / 5040.0f);
+    s = __builtin_fmaf(s, x, 1.0f / 720.0f);
+    s = __builtin_fmaf(s, x, 1.0f / 120.0f);
+    s = __builtin_fmaf(s, x, 1.0f / 24.0f);
+    s = __builtin_fmaf(s, x, 1.0f / 6.0f);
+    s = __builtin_fmaf(s, x, 0.5f);
+    return __builtin_fmaf(x * x, s, x);
+}
+// for both kinds of heads in one expression: S <- keep S + f S, keep 1 or 0
+struct DecayFactor { float keep, f; };
+__device__ __forceinline__ DecayFactor decay_factor(float g, int n) {
+    const bool slow = decay_slow(g, n);
+    const float less = decay_less(g, n), power = decay_pow(decay_log2(g), n);
+    return {slow ? 1.0f : 0.0f, slow ? less : power};
+}
 __device__ __forceinline__ int decay_len(const int* lens, int n, int L) { return lens ? min(max(lens[n], 0), L) : L; }
 
 // ---------------------------------------------------------------- along the sequence
@@ -72,164 +101,179 @@ __global__ __launch_bounds__(64 * ZB, XB == 4 && ZB < 3 ? 1 : 2) void decay_walk
     const int n = mix_uniform(nh / p.head), hd = nh - n * p.head;
     const int len = mix_uniform(decay_len(p.lens, n, p.L));
     const int from = segment * p.segment, end = min(from + p.segment, p.L), to = max(min(end, len), from);
-    const float g2 = decay_log2(p.g, hd);
+    const float g = p.g[hd], g2 = decay_log2(g);
     const int col = 32 * wave + r;                              // this lane's column of the state
     const float* const xb = p.x + n * p.lx.n + hd * p.lx.h;
-    const float* const yb = p.y + n * p.ly.n + hd * p.ly.h;
+    const float* const yb = p.y + n * p.lx.n + hd * p.lx.h;
     const float* const zb = p.z + n * p.lz.n + hd * p.lz.h;
-    float* const ob = p.out + n * p.lo.n + hd * p.lo.h + 32 * wave;
+    float* const ob = p.out + n * p.lz.n + hd * p.lz.h + 32 * wave;
     const int mine = p.zd - 32 * wave;                          // floats of a row of `out` from this wavefront's on
 
-    MixTile<XW, 32, true, 64 * ZB> xt, yt;
+    MixTile<XW, 32, true, 64 * ZB> xt;                          // x and y lie alike, z and out too
     MixTile<ZW, 32, false, 64 * ZB> zt;
     MixColumns<XW, true> cols;
     cols.init(r, h);
     xt.init(t, p.lx.l, p.xd);
-    yt.init(t, p.ly.l, p.xd);
     zt.init(t, p.lz.l, p.zd);
     const unsigned xlds = mix_lds(Xs) + wave * 1024, ylds = mix_lds(Ys[0]) + wave * 1024, zlds = mix_lds(Zs) + wave * 1024;
     auto fetch_xy = [&](int t0, int into) {
         xt.fetch(xb + (size_t)t0 * p.lx.l, to - t0, p.lx.l, xlds, wave);
-        yt.fetch(yb + (size_t)t0 * p.ly.l, to - t0, p.ly.l, ylds + into * (32 * XW * 4), wave);
+        xt.fetch(yb + (size_t)t0 * p.lx.l, to - t0, p.lx.l, ylds + into * (32 * XW * 4), wave);
     };
     auto fetch_z = [&](int t0) { zt.fetch(zb + (size_t)t0 * p.lz.l, to - t0, p.lz.l, zlds, wave); };
-
-    // ---- the state that the segment begins with: register v of block k is row 32k + mix_row(v, h), column col ----
-    v16f S[XB];
-    bool any = p.state != nullptr;                              // the state is not zero all over
-#pragma unroll
-    for (int k = 0; k < XB; k++) S[k] = (v16f)(0.0f);
-    if (any) {
-        const float* s0 = p.state + ((size_t)nh * p.segments + segment) * p.xd * p.zd;
-#pragma unroll
-        for (int k = 0; k < XB; k++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const int row = 32 * k + 8 * q + 4 * h;
-                if (row < p.xd && col < p.zd) {
-                    if constexpr (ST) {
-                        const v4f s = *(const v4f*)(s0 + (size_t)col * p.xd + row);
-#pragma unroll
-                        for (int w = 0; w < 4; w++) S[k][4 * q + w] = s[w];
-                    } else {
-#pragma unroll
-                        for (int w = 0; w < 4; w++) S[k][4 * q + w] = s0[(size_t)(row + w) * p.zd + col];
-                    }
-                }
-            }
-    }
-    // powers: between tokens of the 32 (masked), of a token's entry into the state
-    float near[16], enter[16];
-#pragma unroll
-    for (int v = 0; v < 16; v++) {
-        const int row = mix_row(v, h), far = p.back ? row - r : r - row;
-        near[v] = far < 0 ? 0.0f : decay_pow(g2, far) * p.near_scale;
-        enter[v] = decay_pow(g2, p.back ? row + 1 : 31 - row) * p.add_scale;
-    }
-
     const int chunks = (to - from + 31) / 32;
     auto start = [&](int c) { return from + 32 * (p.back ? chunks - 1 - c : c); };
     if (chunks > 0) {
         fetch_xy(start(0), 0);
         fetch_z(start(0));
     }
-    mix_wait();
-    __syncthreads();
-    for (int c = 0; c < chunks; c++) {
-        const int t0 = start(c), count = min(32, to - t0), buf = c & 1;
-        const bool more = c + 1 < chunks;
 
-        // ---- this wavefront's part of the scores: groups of 8 of the head dimension ----
-        {
-            const unsigned at = r * (XW * 4) + 16 * (h ^ kin_swizzle<XW>(r));
-            typedef const __attribute__((address_space(3))) v4f* lds_v4f;
-            v16f s = (v16f)(0.0f);
-#pragma unroll
-            for (int i = 0; i < SHARE; i++) {
-                const int g = wave * SHARE + i;
-                if (NG % ZB == 0 || g < NG) {
-                    const unsigned place = (at ^ (32 * (g & 7))) + 256 * (g >> 3);
-                    const v4f a = *(lds_v4f)(size_t)(mix_lds(Ys[buf]) + place), b = *(lds_v4f)(size_t)(mix_lds(Xs) + place);
-                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, b.x, s, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, b.y, s, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, b.z, s, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, b.w, s, 0, 0, 0);
-                }
-            }
-#pragma unroll
-            for (int q = 0; q < 4; q++) *(v4f*)&Ps[wave][q * 256 + 4 * lane] = (v4f){s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
-        }
-        // ---- x . S ----
-        v16f o[1] = {(v16f)(0.0f)};
+    // Everything from here on for either kind of head by itself: a branch around the state in every step costs registers that
+    // a state of 128 x 96 does not have (378 us became 473).
+    auto along = [&](auto slowc) {
+        constexpr bool SLOW = decltype(slowc)::value;
+        // ---- the state that the segment begins with: register v of block k is row 32k + mix_row(v, h), column col ----
+        v16f S[XB];
+        bool any = p.state != nullptr;                              // the state is not zero all over
+    #pragma unroll
+        for (int k = 0; k < XB; k++) S[k] = (v16f)(0.0f);
         if (any) {
-            const unsigned at = mix_lds(Xs) + r * (XW * 4) + 16 * (h ^ kin_swizzle<XW>(r));
-            typedef const __attribute__((address_space(3))) v4f* lds_v4f;
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const v4f b = *(lds_v4f)(size_t)((at ^ (32 * (g & 7))) + 256 * (g >> 3));
-#pragma unroll
-                for (int w = 0; w < 4; w++) o[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(S[g / 4][4 * (g % 4) + w], b[w], o[0], 0, 0, 0);
-            }
-            mix_order<2, NG, 4>();
-            o[0] *= decay_pow(g2, p.back ? max(count - 1 - r, 0) : r + 1) * p.far_scale;
+            const float* s0 = p.state + ((size_t)nh * p.segments + segment) * p.xd * p.zd;
+    #pragma unroll
+            for (int k = 0; k < XB; k++)
+    #pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int row = 32 * k + 8 * q + 4 * h;
+                    if (row < p.xd && col < p.zd) {
+                        if constexpr (ST) {
+                            const v4f s = *(const v4f*)(s0 + (size_t)col * p.xd + row);
+    #pragma unroll
+                            for (int w = 0; w < 4; w++) S[k][4 * q + w] = s[w];
+                        } else {
+    #pragma unroll
+                            for (int w = 0; w < 4; w++) S[k][4 * q + w] = s0[(size_t)(row + w) * p.zd + col];
+                        }
+                    }
+                }
         }
-        mix_wait();                                             // z
+        // powers: between tokens of the 32 (masked), of a token's entry into the state
+        float near[16], enter[16];
+    #pragma unroll
+        for (int v = 0; v < 16; v++) {
+            const int row = mix_row(v, h), far = p.back ? row - r : r - row;
+            near[v] = far < 0 ? 0.0f : decay_pow(g2, far) * p.near_scale;
+            enter[v] = decay_pow(g2, p.back ? row + 1 : 31 - row) * p.add_scale;
+        }
+
+        mix_wait();
         __syncthreads();
-        if (more) fetch_xy(start(c + 1), buf ^ 1);
-        __builtin_amdgcn_sched_barrier(0);
-        // ---- the near tokens ----
-        v16f s;
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            v4f sum = *(const v4f*)&Ps[0][q * 256 + 4 * lane];
-#pragma unroll
-            for (int w = 1; w < ZB; w++) sum += *(const v4f*)&Ps[w][q * 256 + 4 * lane];
-#pragma unroll
-            for (int w = 0; w < 4; w++) s[4 * q + w] = sum[w] * near[4 * q + w];
-        }
-        float z[16];
-#pragma unroll
-        for (int v = 0; v < 16; v++) z[v] = Zs[mix_row(v, h) * ZW + col];
-#pragma unroll
-        for (int v = 0; v < 16; v++) o[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(z[v], s[v], o[0], 0, 0, 0);
-        // ---- into the state ----
-        if (more || p.last != nullptr) {
-            v16f zw;
-            if (count == 32 || p.back) {
-#pragma unroll
-                for (int v = 0; v < 16; v++) zw[v] = z[v] * enter[v];
-            } else {                                            // the sequence's last, shorter run
-#pragma unroll
-                for (int v = 0; v < 16; v++) zw[v] = z[v] * (decay_pow(g2, max(count - 1 - mix_row(v, h), 0)) * p.add_scale);
+        const float less = decay_less(g, 32);
+        for (int c = 0; c < chunks; c++) {
+            const int t0 = start(c), count = min(32, to - t0), buf = c & 1;
+            const bool more = c + 1 < chunks;
+
+            // ---- this wavefront's part of the scores: groups of 8 of the head dimension ----
+            {
+                const unsigned at = r * (XW * 4) + 16 * (h ^ kin_swizzle<XW>(r));
+                typedef const __attribute__((address_space(3))) v4f* lds_v4f;
+                v16f s = (v16f)(0.0f);
+    #pragma unroll
+                for (int i = 0; i < SHARE; i++) {
+                    const int g = wave * SHARE + i;
+                    if (NG % ZB == 0 || g < NG) {
+                        const unsigned place = (at ^ (32 * (g & 7))) + 256 * (g >> 3);
+                        const v4f a = *(lds_v4f)(size_t)(mix_lds(Ys[buf]) + place), b = *(lds_v4f)(size_t)(mix_lds(Xs) + place);
+                        s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, b.x, s, 0, 0, 0);
+                        s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, b.y, s, 0, 0, 0);
+                        s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, b.z, s, 0, 0, 0);
+                        s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, b.w, s, 0, 0, 0);
+                    }
+                }
+    #pragma unroll
+                for (int q = 0; q < 4; q++) *(v4f*)&Ps[wave][q * 256 + 4 * lane] = (v4f){s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
             }
+            // ---- x . S ----
+            v16f o[1] = {(v16f)(0.0f)};
             if (any) {
-                const float f = decay_pow(g2, count);
-#pragma unroll
-                for (int k = 0; k < XB; k++) S[k] *= f;
+                const unsigned at = mix_lds(Xs) + r * (XW * 4) + 16 * (h ^ kin_swizzle<XW>(r));
+                typedef const __attribute__((address_space(3))) v4f* lds_v4f;
+                __builtin_amdgcn_sched_barrier(0);
+    #pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    const v4f b = *(lds_v4f)(size_t)((at ^ (32 * (g & 7))) + 256 * (g >> 3));
+    #pragma unroll
+                    for (int w = 0; w < 4; w++) o[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(S[g / 4][4 * (g % 4) + w], b[w], o[0], 0, 0, 0);
+                }
+                mix_order<2, NG, 4>();
+                o[0] *= decay_pow(g2, p.back ? max(count - 1 - r, 0) : r + 1) * p.far_scale;
             }
-            mix_columns_product<XW, XB, true>(S, Ys[buf], zw, cols);
-            any = true;
+            mix_wait();                                             // z
+            __syncthreads();
+            if (more) fetch_xy(start(c + 1), buf ^ 1);
+            __builtin_amdgcn_sched_barrier(0);
+            // ---- the near tokens ----
+            v16f s;
+    #pragma unroll
+            for (int q = 0; q < 4; q++) {
+                v4f sum = *(const v4f*)&Ps[0][q * 256 + 4 * lane];
+    #pragma unroll
+                for (int w = 1; w < ZB; w++) sum += *(const v4f*)&Ps[w][q * 256 + 4 * lane];
+    #pragma unroll
+                for (int w = 0; w < 4; w++) s[4 * q + w] = sum[w] * near[4 * q + w];
+            }
+            float z[16];
+    #pragma unroll
+            for (int v = 0; v < 16; v++) z[v] = Zs[mix_row(v, h) * ZW + col];
+    #pragma unroll
+            for (int v = 0; v < 16; v++) o[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(z[v], s[v], o[0], 0, 0, 0);
+            // ---- into the state ----
+            if (more || p.last != nullptr) {
+                v16f zw;
+                if (count == 32 || p.back) {
+    #pragma unroll
+                    for (int v = 0; v < 16; v++) zw[v] = z[v] * enter[v];
+                } else {                                            // the sequence's last, shorter run
+    #pragma unroll
+                    for (int v = 0; v < 16; v++) zw[v] = z[v] * (decay_pow(g2, max(count - 1 - mix_row(v, h), 0)) * p.add_scale);
+                }
+                if (any) {
+                    if constexpr (SLOW) {
+                        const float f = count == 32 ? less : decay_less(g, count);
+    #pragma unroll
+                        for (int k = 0; k < XB; k++)
+    #pragma unroll
+                            for (int v = 0; v < 16; v++) S[k][v] = __builtin_fmaf(S[k][v], f, S[k][v]);
+                    } else {
+                        const float f = decay_pow(g2, count);
+    #pragma unroll
+                        for (int k = 0; k < XB; k++) S[k] *= f;
+                    }
+                }
+                mix_columns_product<XW, XB, true>(S, Ys[buf], zw, cols);
+                any = true;
+            }
+            mix_wait();                                             // the next x and y
+            __syncthreads();
+            if (more) fetch_z(start(c + 1));
+            if (t0 + r < end) mix_store_row<1>(ob + (size_t)(t0 + r) * p.lz.l, o, 1.0f, mine, h);
         }
-        mix_wait();                                             // the next x and y
-        __syncthreads();
-        if (more) fetch_z(start(c + 1));
-        if (t0 + r < end) mix_store_row<1>(ob + (size_t)(t0 + r) * p.lo.l, o, 1.0f, mine, h);
-    }
-    // ---- rows behind the sequence's end; the state at the other end ----
-    for (int t0 = from + 32 * chunks; t0 < end; t0 += 32)
-        if (t0 + r < end)
-            for (int d = 4 * h; d < min(mine, 32); d += 8) *(v4f*)(ob + (size_t)(t0 + r) * p.lo.l + d) = (v4f)(0.0f);
-    if (p.last != nullptr) {
-        float* s1 = p.last + (size_t)nh * p.xd * p.zd;
-#pragma unroll
-        for (int k = 0; k < XB; k++)
-#pragma unroll
-            for (int v = 0; v < 16; v++) {
-                const int row = 32 * k + mix_row(v, h);
-                if (row < p.xd && col < p.zd) s1[(size_t)row * p.zd + col] = S[k][v];
-            }
-    }
+        // ---- rows behind the sequence's end; the state at the other end ----
+        for (int t0 = from + 32 * chunks; t0 < end; t0 += 32)
+            if (t0 + r < end)
+                for (int d = 4 * h; d < min(mine, 32); d += 8) *(v4f*)(ob + (size_t)(t0 + r) * p.lz.l + d) = (v4f)(0.0f);
+        if (p.last != nullptr) {
+            float* s1 = p.last + (size_t)nh * p.xd * p.zd;
+    #pragma unroll
+            for (int k = 0; k < XB; k++)
+    #pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    const int row = 32 * k + mix_row(v, h);
+                    if (row < p.xd && col < p.zd) s1[(size_t)row * p.zd + col] = S[k][v];
+                }
+        }
+    };
+    if (mix_uniform(decay_slow(g, 32))) along(std::true_type{});
+    else along(std::false_type{});
 }
 
 // ---------------------------------------------------------------- a segment's own sum
@@ -257,7 +301,7 @@ __global__ __launch_bounds__(NTHREADS, 2) void decay_states(const DecayStates p)
     const int n = mix_uniform(nh / p.head), hd = nh - n * p.head;
     const int c0 = segment * p.segment, cnt = min(p.segment, mix_uniform(decay_len(p.lens, n, p.L)) - c0);
     if (cnt <= 0) return;                                // decay_scan does not read it
-    const float g2 = decay_log2(p.g, hd);
+    const float g2 = decay_log2(p.g[hd]);
     const float* ab = p.A + n * p.la.n + hd * p.la.h + (size_t)c0 * p.la.l;
     const float* bb = p.B + n * p.lb.n + hd * p.lb.h + (size_t)c0 * p.lb.l;
     MixTile<DW, 32, false> at, bt;
@@ -349,8 +393,7 @@ __global__ __launch_bounds__(NTHREADS) void decay_scan(const DecayScan p) {
     const int e = (int)(x - nh * p.size4);
     const int n = (int)(nh / p.head), hd = (int)(nh - (long long)n * p.head);
     const int len = decay_len(p.lens, n, p.L), used = (len + p.segment - 1) / p.segment;
-    const float g2 = decay_log2(p.g, hd);
-    const float whole = decay_pow(g2, p.segment), tail = decay_pow(g2, len - (used - 1) * p.segment);
+    const DecayFactor whole = decay_factor(p.g[hd], p.segment), tail = decay_factor(p.g[hd], len - (used - 1) * p.segment);
     v4f* U = (v4f*)p.U + (size_t)nh * p.segments * p.size4 + e;
     v4f s = p.first ? ((const v4f*)p.first)[nh * p.size4 + e] : (v4f)(0.0f);
     constexpr int AHEAD = 8;       // loads in flight: each would otherwise wait for the one before
@@ -366,7 +409,8 @@ __global__ __launch_bounds__(NTHREADS) void decay_scan(const DecayScan p) {
             if (k0 + i >= used) break;
             const int c = p.back ? used - 1 - (k0 + i) : k0 + i;
             U[(size_t)c * p.size4] = s;
-            s = s * (c == used - 1 ? tail : whole) + u[i];
+            const DecayFactor f = c == used - 1 ? tail : whole;
+            s = s * f.f + (s * f.keep + u[i]);
         }
     }
     if (p.last) ((v4f*)p.last)[nh * p.size4 + e] = s;
@@ -392,10 +436,10 @@ __global__ __launch_bounds__(NTHREADS) void decay_steps(const DecaySteps p) {
     const int t = threadIdx.x, wave = t >> 6;
     const int nh = blockIdx.x / p.slabs, slab = blockIdx.x - nh * p.slabs;
     const int n = nh / p.head, hd = nh - n * p.head;
+    const float g = p.g[hd];
     const int len = decay_len(p.lens, n, p.L);
     const int col = slab * COLS + 4 * (t % ACROSS), row0 = t / ACROSS;
     const bool mine = col < p.dv;
-    const float lam = decay_pow(decay_log2(p.g, hd), 1);
     const size_t base = (size_t)nh * p.dk * p.dv + col;
     v4f s[STEP_ROWS];
 #pragma unroll
@@ -422,6 +466,7 @@ __global__ __launch_bounds__(NTHREADS) void decay_steps(const DecaySteps p) {
         }
     };
     if (len > 0) read(0);
+    const DecayFactor lam = decay_factor(g, 1);
     for (int i = 0; i < len; i++) {
         const v4f vv = vn;
         v4f out = (v4f)(0.0f);
@@ -429,7 +474,7 @@ __global__ __launch_bounds__(NTHREADS) void decay_steps(const DecaySteps p) {
 #pragma unroll
         for (int a = 0; a < STEP_ROWS; a++) {
             qi[a] = qn[a];
-            s[a] = s[a] * lam + vv * kn[a];
+            s[a] = vv * kn[a] + (s[a] * lam.f + s[a] * lam.keep);
         }
         if (i + 1 < len) read(i + 1);
 #pragma unroll
@@ -594,7 +639,7 @@ int dragon_Cuda_linear_attention_forward(const int64_t* streams, int32_t length,
         return hipGetLastError();
     }
     const DecayCut cut = decay_cut(N, head, L, dV4);
-    DecayWalk p = {Q, K, V, Y, lk, lk, lv, lv, g, lens, head, L, dK4, dV4, cut.segment, cut.segments, 0, scale, scale, 1.0f,
+    DecayWalk p = {Q, K, V, Y, lk, lv, g, lens, head, L, dK4, dV4, cut.segment, cut.segments, 0, scale, scale, 1.0f,
                    first, last, N * head};
     if (cut.segments > 1) {
         hipError_t e = launch_states(s, K, lk, dK4, V, lv, dV4, g, lens, N, head, L, cut, 0, 1.0f, U);
@@ -649,14 +694,14 @@ int dragon_Cuda_linear_attention_backward(const int64_t* streams, int32_t length
         before = S;
         behind = R;
     }
-    DecayWalk p = {G, V, K, gQ, lv, lv, lk, lk, g, lens, head, L, dV4, dK4, cut.segment, cut.segments, 0, scale, scale, 1.0f,
+    DecayWalk p = {G, V, K, gQ, lv, lk, g, lens, head, L, dV4, dK4, cut.segment, cut.segments, 0, scale, scale, 1.0f,
                    before, nullptr, N * head};
     e = launch_walk<true>(s, p);
     p.back = 1; p.far_scale = 1.0f; p.add_scale = scale;
     p.state = behind;
     p.x = V; p.y = G; p.z = Q; p.out = gK;
     if (e == hipSuccess) e = launch_walk<true>(s, p);
-    p.x = K; p.y = Q; p.z = G; p.out = gV; p.lx = p.ly = lk; p.lz = p.lo = lv; p.xd = dK4; p.zd = dV4;
+    p.x = K; p.y = Q; p.z = G; p.out = gV; p.lx = lk; p.lz = lv; p.xd = dK4; p.zd = dV4;
     p.last = cut.segments == 1 ? gfirst : nullptr;
     if (e == hipSuccess) e = launch_walk<false>(s, p);
     return e;

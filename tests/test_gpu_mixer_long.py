@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from mixers import check, decay_reference, run_decay, run_window
-from mixers_exact import few, undecayed, uniform_window, whole_values
+from mixers_exact import U, few, undecayed, uniform_window, whole_values
 from test_gpu_mixers import DECAY
 
 pytestmark = pytest.mark.gpu
@@ -87,3 +87,41 @@ def test_decay_results_do_not_depend_on_who_wants_the_states(dh, gpu, case):
     assert set(b) == {"Y", "dQ", "dK", "dV"}
     for name in b:
         assert np.array_equal(a[name], b[name]), name
+
+
+# Tokens a call, calls, multiplications of the state in all: 12 tokens multiply it each (decay_steps; the gradient at once), 192
+# every 32 (decay_walk), 4096 in 64 segments once each (decay_scan).
+@pytest.mark.parametrize("tokens, calls, forward, backward", [(12, 1500, 18000, 1500), (192, 300, 1800, 1800), (4096, 20, 1280, 1280)])
+def test_a_slow_decay_does_not_drift(dh, gpu, tokens, calls, forward, backward):
+    """A state that nothing is added to, e^{gT} of it after T tokens, call after call.  Every multiplication rounds an element
+    by at most U, up or down as its digits happen to lie (a step takes hundreds of units in the last place off it), so the
+    mean over E elements after M of them is off by U sqrt(M / E / 3) or so; six times that are allowed.  (Elements whole steps
+    apart run through the same values and round alike, so no more count than a step has units.)  What is the same for all
+    elements is the factor's own error, 4 U of what it takes off each time, |g| T of it in all.  A factor near 1 that is itself
+    rounded to FP32 is off by up to U / 2 every time, in one direction, hundreds of U in the end."""
+    H, d = 8, 64
+    rng = np.random.default_rng(tokens)
+    T = tokens * calls
+    g = (-np.linspace(0.7, 2.0, H) / T).astype(np.float32)
+    zero = dh.DeviceArray(size=tokens * H * d)
+    out = [dh.DeviceArray(size=tokens * H * d) for _ in range(3)]
+    dec = dh.DeviceArray(g)
+    first = rng.uniform(0.5, 2.0, (H, d, d)).astype(np.float32)
+    A = dh.Cuda_linear_attention
+    sizes = (1, H, tokens, d, d)
+    need, gneed = A.bufsize(*sizes), A.backward_bufsize(*sizes)
+    buf = dh.DeviceArray(size=max(need, gneed, 16) // 4)
+    state = dh.DeviceArray(first)
+    grads = [dh.DeviceArray(first), dh.DeviceArray(size=first.size)]
+    z = zero.address
+    for i in range(calls):
+        A.forward([0], 1, z, z, z, dec.address, state.address, out[0].address, state.address, 0, buf.address, need, *sizes, 1, 1.0)
+        A.backward([0], 1, z, z, z, dec.address, 0, z, grads[i % 2].address, *(x.address for x in out), grads[1 - i % 2].address, 0,
+                   buf.address, gneed, *sizes, 1, 1.0)
+    dh.Cuda.deviceSynchronize()
+    want = first * np.exp(g.astype(np.float64) * T)[:, None, None]
+    for name, got, times in (("state", state, forward), ("gradient", grads[calls % 2], backward)):
+        off = np.mean(got.get(first.shape) / want - 1.0, (1, 2))
+        apart = np.minimum(np.abs(g) * T / times * 2.0 ** 23, d * d)
+        bound = U * (4 * np.abs(g) * T + 6 * np.sqrt(times / (3 * apart)) + 4)
+        assert (np.abs(off) <= bound).all(), "%s: off by %s U, %s U allowed" % (name, np.round(off / U, 1), np.round(bound / U, 1))
