@@ -507,12 +507,21 @@ __global__ __launch_bounds__(NTHREADS) void decay_steps(const DecaySteps p) {
 // 105 (13.0 and 99), 16 in 13.2 and 127 (13.0 and 101).
 constexpr int STEPS_MAX = 12;
 
-// How a sequence is cut: into as many segments as fill the chip with workgroups, where that is faster than walking along
-// it whole -- the segments' sums cost one product more to the walk's two and a half, and two launches.
+// The workgroups of decay_walk that the chip holds, x being xd columns wide and z zd: two a compute unit where either is above 64
+// (LDS).  500 pairs of 128 x 64 and 4096 tokens take 885 us whole; cut in two, as if four a unit had room, 1871.  (At 64 x 32 LDS
+// holds five, not eight, but with five the estimate below is no better: 170 us for 475 at 960 pairs, 268 for 205 at 1440.)
+constexpr int decay_slots(int xd, int zd) { return xd > 64 || zd > 64 ? 512 : zd > 32 ? 1024 : 2048; }
+// How a sequence is cut: into as many segments as fill the chip with workgroups, where that is taken to be faster than walking along
+// it whole -- the segments' sums cost one product more to the walk's two and a half, and two launches (3.7 and 12 runs of 32
+// tokens' time).  Cut against whole: 16 heads of 128 and 300 tokens 30 us against 66, 4 x 16 of 64 and 1000 43 against 122,
+// 8 x 16 of 128 and 2000 289 against 408.  The estimate counts rounds of workgroups and does not know that
+// one alone on a compute unit walks faster than two: from half a round on it cuts too early (16 x 16 of 128 and 2000 tokens: 557
+// against 416).
+// At most 64 segments, which bounds the work buffer: one head of 128 and 32768 tokens takes 152 us (32: 280; 256 would take
+// 82), 4 heads 160 (284; 158), 16 heads 540 (547; 546).
 struct DecayCut { int segment, segments; };
-DecayCut decay_cut(int N, int head, int L, int zd) {
+DecayCut decay_cut(int N, int head, int L, int slots) {
     const long long nh = (long long)N * head, chunks = (L + 31LL) / 32;
-    const long long slots = zd > 64 ? 512 : zd > 32 ? 1024 : 2048;    // workgroups (of zd / 32 wavefronts) that the chip holds
     DecayCut best = {(int)(chunks * 32), 1};
     double least = 0.0;
     for (long long want = 1; want <= 64; want++) {
@@ -599,11 +608,11 @@ extern "C" {
 
 int64_t dragon_Cuda_linear_attention_bufsize(int32_t N, int32_t head, int32_t L, int32_t dK4, int32_t dV4) {
     if (!decay_forward_ok(N, head, L, dK4, dV4)) return -1;
-    return L <= STEPS_MAX ? 0 : decay_state_bytes(N, head, decay_cut(N, head, L, dV4), dK4, dV4);
+    return L <= STEPS_MAX ? 0 : decay_state_bytes(N, head, decay_cut(N, head, L, decay_slots(dK4, dV4)), dK4, dV4);
 }
 int64_t dragon_Cuda_linear_attention_backward_bufsize(int32_t N, int32_t head, int32_t L, int32_t dK4, int32_t dV4) {
     if (!decay_backward_ok(N, head, L, dK4, dV4)) return -1;
-    return 2 * decay_state_bytes(N, head, decay_cut(N, head, L, dK4 > dV4 ? dK4 : dV4), dK4, dV4);
+    return 2 * decay_state_bytes(N, head, decay_cut(N, head, L, decay_slots(dK4, dK4 > dV4 ? dK4 : dV4)), dK4, dV4);
 }
 
 int dragon_Cuda_linear_attention_forward(const int64_t* streams, int32_t length, int64_t dQ, int64_t dK, int64_t dV, int64_t dDecay,
@@ -638,7 +647,7 @@ int dragon_Cuda_linear_attention_forward(const int64_t* streams, int32_t length,
         else hipLaunchKernelGGL((decay_steps<false, 32>), grid, dim3(NTHREADS), 0, s, p);
         return hipGetLastError();
     }
-    const DecayCut cut = decay_cut(N, head, L, dV4);
+    const DecayCut cut = decay_cut(N, head, L, decay_slots(dK4, dV4));
     DecayWalk p = {Q, K, V, Y, lk, lv, g, lens, head, L, dK4, dV4, cut.segment, cut.segments, 0, scale, scale, 1.0f,
                    first, last, N * head};
     if (cut.segments > 1) {
@@ -663,7 +672,7 @@ int dragon_Cuda_linear_attention_backward(const int64_t* streams, int32_t length
         !mix_aligned16(dDeltaState) || (dDecay & 3) || (dLens & 3))
         return hipErrorInvalidValue;
     if (!decay_backward_ok(N, head, L, dK4, dV4) || !(scale - scale == 0.0f)) return hipErrorInvalidValue;
-    const DecayCut cut = decay_cut(N, head, L, dK4 > dV4 ? dK4 : dV4);
+    const DecayCut cut = decay_cut(N, head, L, decay_slots(dK4, dK4 > dV4 ? dK4 : dV4));   // (either width is x in one of the walks)
     const long long need = 2 * decay_state_bytes(N, head, cut, dK4, dV4);
     if (need > 0 && (dBuf == 0 || !mix_aligned16(dBuf) || buf_size < need)) return hipErrorInvalidValue;
     const float* Q = (const float*)(intptr_t)dQ; const float* K = (const float*)(intptr_t)dK; const float* V = (const float*)(intptr_t)dV;

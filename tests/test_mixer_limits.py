@@ -105,3 +105,11 @@ def test_decay_gradient_sizes_beyond_a_launch(dh, case):
         dh.Cuda_linear_attention.backward_bufsize(**decay_sizes(case))
     with pytest.raises(dh.CudaException):
         dh.Cuda_linear_attention.backward(**decay_grad_args(**decay_sizes(case)))
+
+
+@pytest.mark.parametrize("dk, dv", [(128, 64), (128, 32), (68, 4), (128, 128), (4, 128)])
+def test_a_sequence_is_not_cut_where_the_whole_walks_fill_the_chip(dh, dk, dv):
+    """Two workgroups a compute unit where a head dimension is above 64: with 500 pairs there is no room for segments."""
+    assert dh.Cuda_linear_attention.bufsize(N=500, head=1, L=4096, dK4=dk, dV4=dv) == 0
+    assert dh.Cuda_linear_attention.backward_bufsize(N=500, head=1, L=4096, dK4=dk, dV4=dv) == 0
+    assert dh.Cuda_linear_attention.bufsize(N=100, head=1, L=4096, dK4=dk, dV4=dv) > 0
