@@ -36,7 +36,8 @@ constexpr float LOWEST = -3.402823466e38f;   // not above any score but -infinit
 // lengths window_tiles deals them by the steps that a tile has, so that the longest part is as short as can be: pieces of 500 and
 // 250 on 9000 and 4500 keys of 16 heads of 96 in 305 us instead of 418, prompts of 1000 to 250 of 8 heads of 64 in 47 instead of
 // 65.  Every wavefront works the deal out for itself, a pair (tile, sequence) a lane; the first workgroup of a pair writes it
-// down for window_join.  (window_rows reads so little that the deal costs it more: 16.2 -> 17.8 us at 8 sequences of up to 4096.)
+// down for window_join.  (window_rows reads so little that the deal costs it more: 16.2 -> 17.8 us at 8 sequences of up to 4096.
+// Nothing is dealt where the sizes alone fill the chip: there a long sequence among short ones keeps its own workgroups busy.)
 constexpr int PAIRS = 512;      // at most, where there are parts (window_plan)
 struct WindowCutting {
     int per, ak, least, want;   // rows of a tile, keys of a step, steps worth a part, workgroups on the chip
@@ -516,6 +517,8 @@ struct WindowPlan { bool rows; int qtiles, parts, per; };
 // A part of window_rows is worth its launch of window_join from 8 steps on, if there are 24 to cut: one token on 1024 keys of 4
 // heads of 64 in 10.0 us (cuts of 16: 11.2), but on 256 keys 7.9 whole and 9.4 cut.  More parts than compute units gain nothing
 // there (16384 keys of 8 heads of 128: 29 us, with twice as many 33).
+// At most 64 parts, which bounds the work buffer: one token on 65536 keys of one head of 128 takes 33 us (32 parts: 54; 256, as
+// many as compute units, would take 26, and 128 queries of one head there 52 instead of 138); on 4 heads, which fill the units, 51.
 WindowPlan window_plan(int N, int head, int kv_head, int QL, int VL, int window, int sinks) {
     WindowPlan x;
     const long long group = head / kv_head, rows = QL * group;

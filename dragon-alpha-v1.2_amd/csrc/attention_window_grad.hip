@@ -654,7 +654,10 @@ int window_grad_parts(int N, int head, int kv_head, int QL, int VL, int workers,
 }
 // The caller's buffer, in floats: the statistics, the running sum (64-bit), the pieces and whose they are, the sinks' parts,
 // the parts of dQ.
-constexpr int SINKS_APART = 64;      // up to here window_grad_sinks takes the queries beyond the window
+// Up to here window_grad_sinks takes the queries beyond the window.  Training 4 x 1024, 16 heads of 64 under a window of 256: with 4
+// sinks 294 us (in the tiles 334), with 64 325 (342), with 100 367 (363); 8192, 32 heads of 128 on 8 under 1024: with 4 sinks 5188
+// (5350), with 64 5441 (5416), with 100 5754 (5546).
+constexpr int SINKS_APART = 64;
 // also the workgroups of every launch: rows' statistics, dQ, sinks, joins (window_grad_kv: the workers)
 struct WindowGradBuffer {
     int ktiles, workers, qtiles, sink_blocks, sink_parts, parts;
@@ -739,7 +742,7 @@ int dragon_Cuda_attention_window_backward(const int64_t* streams, int32_t length
     a.rows = (long long)N * head * QL;
     a.scale = scale;
     a.ktiles = b.ktiles; a.workers = b.workers;
-    a.snap = 2;
+    a.snap = 2;     // (0: level on seven shapes but 294 us for 302 on 3 ragged 1500; 5: 2 to 6 % slower wherever tiles are cut)
     a.before = (long long*)(a.stats + b.stats);
     a.pieces = a.stats + b.stats + b.before;
     a.cut = (int2*)(a.pieces + b.pieces);
