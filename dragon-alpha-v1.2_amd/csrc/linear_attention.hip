@@ -3,14 +3,15 @@
 // and its gradient.
 //
 // Few tokens (decay_steps): the recurrence itself, the state in registers; bound by reading and writing the states: a token of
-// 256 x 32 states of 128 x 128 in 190 us, 5.7 TB/s.
+// 256 x 32 states of 128 x 128 in 193 us, 5.6 TB/s; from the third token or so on by the vector instructions, four an element
+// and token (64 x 32 states: 44 us for one token, 59 for four, 108 for twelve).
 // Many tokens (decay_walk): 32 at a time.  With S the state before them and t a token's place among them,
 //     Y[t] = scale * (e^{g(t+1)} Q[t] S  +  sum_{j <= t} e^{g(t-j)} <Q[t], K[j]> V[j]),    S' = e^{32g} S + sum_j e^{g(31-j)} K[j]^T V[j]
 // A workgroup walks along a sequence with the state in its registers, a wavefront for each 32 columns of V.  Where there are
 // fewer (image, head) pairs than the chip takes workgroups the sequence is cut into segments that walk at the same time:
 // decay_states forms each segment's own sum, decay_scan runs over them and leaves the state that each begins with.
 // Bound by the FP32 matrix pipe: 2.5 products of [dk, dv] size a token, and one more where there are segments.  16 heads of 128
-// and 32768 tokens: the states 155 us (111 TFLOP/s), the scan 13, the walk 400 to 420 (103), the pipes busy for 74 % of both; the
+// and 32768 tokens: the states 146 to 157 us (113 TFLOP/s), the scan 13, the walk 380 to 420 (106), the pipes busy for 74 % of both; the
 // rest of the walk goes to vector instructions (powers, decay of the state) and to two barriers for 32 tokens.
 //
 // The gradient is the same walk with other operands (G = gradient of Y, sums over j >= t in the last two, from the end):
@@ -129,28 +130,28 @@ __global__ __launch_bounds__(64 * ZB, XB == 4 && ZB < 3 ? 1 : 2) void decay_walk
     }
 
     // Everything from here on for either kind of head by itself: a branch around the state in every step costs registers that
-    // a state of 128 x 96 does not have (378 us became 473).
+    // a state of 128 x 96 does not have (16 x 32 heads of 96, 1024 tokens: 473 us, so 375).
     auto along = [&](auto slowc) {
         constexpr bool SLOW = decltype(slowc)::value;
         // ---- the state that the segment begins with: register v of block k is row 32k + mix_row(v, h), column col ----
         v16f S[XB];
         bool any = p.state != nullptr;                              // the state is not zero all over
-    #pragma unroll
+#pragma unroll
         for (int k = 0; k < XB; k++) S[k] = (v16f)(0.0f);
         if (any) {
             const float* s0 = p.state + ((size_t)nh * p.segments + segment) * p.xd * p.zd;
-    #pragma unroll
+#pragma unroll
             for (int k = 0; k < XB; k++)
-    #pragma unroll
+#pragma unroll
                 for (int q = 0; q < 4; q++) {
                     const int row = 32 * k + 8 * q + 4 * h;
                     if (row < p.xd && col < p.zd) {
                         if constexpr (ST) {
                             const v4f s = *(const v4f*)(s0 + (size_t)col * p.xd + row);
-    #pragma unroll
+#pragma unroll
                             for (int w = 0; w < 4; w++) S[k][4 * q + w] = s[w];
                         } else {
-    #pragma unroll
+#pragma unroll
                             for (int w = 0; w < 4; w++) S[k][4 * q + w] = s0[(size_t)(row + w) * p.zd + col];
                         }
                     }
@@ -158,7 +159,7 @@ __global__ __launch_bounds__(64 * ZB, XB == 4 && ZB < 3 ? 1 : 2) void decay_walk
         }
         // powers: between tokens of the 32 (masked), of a token's entry into the state
         float near[16], enter[16];
-    #pragma unroll
+#pragma unroll
         for (int v = 0; v < 16; v++) {
             const int row = mix_row(v, h), far = p.back ? row - r : r - row;
             near[v] = far < 0 ? 0.0f : decay_pow(g2, far) * p.near_scale;
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(64 * ZB, XB == 4 && ZB < 3 ? 1 : 2) void decay_walk
                 const unsigned at = r * (XW * 4) + 16 * (h ^ kin_swizzle<XW>(r));
                 typedef const __attribute__((address_space(3))) v4f* lds_v4f;
                 v16f s = (v16f)(0.0f);
-    #pragma unroll
+#pragma unroll
                 for (int i = 0; i < SHARE; i++) {
                     const int g = wave * SHARE + i;
                     if (NG % ZB == 0 || g < NG) {
@@ -189,7 +190,7 @@ __global__ __launch_bounds__(64 * ZB, XB == 4 && ZB < 3 ? 1 : 2) void decay_walk
                         s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, b.w, s, 0, 0, 0);
                     }
                 }
-    #pragma unroll
+#pragma unroll
                 for (int q = 0; q < 4; q++) *(v4f*)&Ps[wave][q * 256 + 4 * lane] = (v4f){s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
             }
             // ---- x . S ----
@@ -198,10 +199,10 @@ __global__ __launch_bounds__(64 * ZB, XB == 4 && ZB < 3 ? 1 : 2) void decay_walk
                 const unsigned at = mix_lds(Xs) + r * (XW * 4) + 16 * (h ^ kin_swizzle<XW>(r));
                 typedef const __attribute__((address_space(3))) v4f* lds_v4f;
                 __builtin_amdgcn_sched_barrier(0);
-    #pragma unroll
+#pragma unroll
                 for (int g = 0; g < NG; g++) {
                     const v4f b = *(lds_v4f)(size_t)((at ^ (32 * (g & 7))) + 256 * (g >> 3));
-    #pragma unroll
+#pragma unroll
                     for (int w = 0; w < 4; w++) o[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(S[g / 4][4 * (g % 4) + w], b[w], o[0], 0, 0, 0);
                 }
                 mix_order<2, NG, 4>();
@@ -213,39 +214,39 @@ __global__ __launch_bounds__(64 * ZB, XB == 4 && ZB < 3 ? 1 : 2) void decay_walk
             __builtin_amdgcn_sched_barrier(0);
             // ---- the near tokens ----
             v16f s;
-    #pragma unroll
+#pragma unroll
             for (int q = 0; q < 4; q++) {
                 v4f sum = *(const v4f*)&Ps[0][q * 256 + 4 * lane];
-    #pragma unroll
+#pragma unroll
                 for (int w = 1; w < ZB; w++) sum += *(const v4f*)&Ps[w][q * 256 + 4 * lane];
-    #pragma unroll
+#pragma unroll
                 for (int w = 0; w < 4; w++) s[4 * q + w] = sum[w] * near[4 * q + w];
             }
             float z[16];
-    #pragma unroll
+#pragma unroll
             for (int v = 0; v < 16; v++) z[v] = Zs[mix_row(v, h) * ZW + col];
-    #pragma unroll
+#pragma unroll
             for (int v = 0; v < 16; v++) o[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(z[v], s[v], o[0], 0, 0, 0);
             // ---- into the state ----
             if (more || p.last != nullptr) {
                 v16f zw;
                 if (count == 32 || p.back) {
-    #pragma unroll
+#pragma unroll
                     for (int v = 0; v < 16; v++) zw[v] = z[v] * enter[v];
                 } else {                                            // the sequence's last, shorter run
-    #pragma unroll
+#pragma unroll
                     for (int v = 0; v < 16; v++) zw[v] = z[v] * (decay_pow(g2, max(count - 1 - mix_row(v, h), 0)) * p.add_scale);
                 }
                 if (any) {
                     if constexpr (SLOW) {
                         const float f = count == 32 ? less : decay_less(g, count);
-    #pragma unroll
+#pragma unroll
                         for (int k = 0; k < XB; k++)
-    #pragma unroll
+#pragma unroll
                             for (int v = 0; v < 16; v++) S[k][v] = __builtin_fmaf(S[k][v], f, S[k][v]);
                     } else {
                         const float f = decay_pow(g2, count);
-    #pragma unroll
+#pragma unroll
                         for (int k = 0; k < XB; k++) S[k] *= f;
                     }
                 }
@@ -263,9 +264,9 @@ __global__ __launch_bounds__(64 * ZB, XB == 4 && ZB < 3 ? 1 : 2) void decay_walk
                 for (int d = 4 * h; d < min(mine, 32); d += 8) *(v4f*)(ob + (size_t)(t0 + r) * p.lz.l + d) = (v4f)(0.0f);
         if (p.last != nullptr) {
             float* s1 = p.last + (size_t)nh * p.xd * p.zd;
-    #pragma unroll
+#pragma unroll
             for (int k = 0; k < XB; k++)
-    #pragma unroll
+#pragma unroll
                 for (int v = 0; v < 16; v++) {
                     const int row = 32 * k + mix_row(v, h);
                     if (row < p.xd && col < p.zd) s1[(size_t)row * p.zd + col] = S[k][v];
@@ -427,7 +428,7 @@ struct DecaySteps {
 };
 // A thread holds 4 columns of rows row0, row0 + LANES, ... of the state; a token's output is added over the row groups of a
 // wavefront by exchange and over the wavefronts through LDS.  COLS: columns of the state per workgroup -- 32, and 64 (256
-// contiguous bytes a row) for states that pass the caches by: 256 x 32 states of 128 x 128 in 190 us instead of 202, but
+// contiguous bytes a row) for states that pass the caches by: 256 x 32 states of 128 x 128 in 193 us instead of 205, but
 // smaller batches are level or behind with it.
 template <bool NT, int COLS>
 __global__ __launch_bounds__(NTHREADS) void decay_steps(const DecaySteps p) {
@@ -503,8 +504,8 @@ __global__ __launch_bounds__(NTHREADS) void decay_steps(const DecaySteps p) {
 }
 
 // ---------------------------------------------------------------- host side
-// Up to here the recurrence: 8 tokens of 32 heads of 128 in 8.2 us and of 64 x 32 in 82 (the walk: 12.9 and 95), 12 in 10.8 and
-// 105 (13.0 and 99), 16 in 13.2 and 127 (13.0 and 101).
+// Up to here the recurrence: 8 tokens of 32 heads of 128 in 9.3 us and of 64 x 32 in 84 (the walk: 14.1 and 98), 12 in 12.0 and
+// 108 (14.1 and 104), 16 in 14.8 and 133 (14.1 and 108).
 constexpr int STEPS_MAX = 12;
 
 // The workgroups of decay_walk that the chip holds, x being xd columns wide and z zd: two a compute unit where either is above 64

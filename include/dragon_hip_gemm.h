@@ -265,8 +265,8 @@ int dragon_Cuda_attention_forward_masked(const int64_t* streams, int32_t length,
  *     (buf_size says how many there are); its content means nothing between calls.  Calls that may run at the same time,
  *     replays of graphs among them, need one each.  _bufsize returns -1 for sizes that the call refuses;
  *   - outputs overlap no operand and each other not at all, but dStateOut may be dState;
- *   - hipErrorInvalidValue: a null or misaligned address, a size out of range, a scale that is not finite, a buffer that is
- *     too small.  No kernel has run then;
+ *   - hipErrorInvalidValue: a null or misaligned address, a size out of range (or so large that a launch would have 2^32
+ *     threads), a scale that is not finite, a buffer that is too small.  No kernel has run then;
  *   - results have the same bits from call to call (no sum depends on who arrives first).
  */
 
